@@ -62,6 +62,13 @@ SIGNATURES = {
     "fathom_attention_combine": (I32, [P, I64, I64, P, P, P]),
     "fathom_gather_runs": (I32, [P, P, P, P, P, I64, I64, I64, P]),
     "fathom_stage_planes": (I32, [P, P, P, I64, I64, I64, I64, P, P, P]),
+    "fathom_kv8_write": (I32, [P, P, I32, I64, I64, I64, I64, I64, I64, I64, P, I64, P, P, P]),
+    "fathom_kv8_read": (I32, [P, P, I64, I64, I64, I64, I32, P, P, P]),
+    "fathom_kv8_attend_workspace_bytes": (SZ, [I64, I64, I32, I64]),
+    "fathom_kv8_attend": (I32, [P, I32, I64, I64, I32, I64, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, P, SZ,
+                                P]),
+    "fathom_kv8_attend_picks_workspace_bytes": (SZ, [I64, I64, I32, I64]),
+    "fathom_kv8_attend_picks": (I32, [P, I32, I64, I64, I32, P, I64, P, P, I64, I64, P, P, P, SZ, P]),
     "fathom_host_alloc_mapped": (I32, [SZ, ctypes.POINTER(P), ctypes.POINTER(P)]),
     "fathom_host_alloc_mapped_ex": (I32, [SZ, I32, ctypes.POINTER(P), ctypes.POINTER(P)]),
     "fathom_host_free": (I32, [P]),

@@ -1,0 +1,180 @@
+"""8-bit key/value cache: written as tokens come, read back, and attended to.
+
+Keys and values as e4m3 codes with one power-of-two scale per 64-token block, KV head and K or V (half the
+bytes of bf16 rows, in HBM or over the host link).  No counterpart in the reference, which keeps bf16 rows
+(scripts/B_e2e_offload_v2.py:272-300).  The sequence's positions may be device tensors, so a decode
+step over the cache can be captured in a CUDA graph.
+
+    cache = KVCache8(B, Hkv, cap)
+    cache.write(K, V, 0)                    # a prompt, or a chunk of one
+    cache.write(k, v, pos)                  # one token of every sequence; pos an int, or int64 [B] on the device
+    out = cache.attend(q, end)              # every key before `end`: prompt chunks, drafts, single tokens
+    out = cache.attend_picks(q, idx, end)   # the listed keys of each query head
+    K, V = cache.read(0, n)
+"""
+import torch
+
+from . import _lib
+from ._lib import check, lib, ptr, require_cuda, stream_of
+
+BLK, D = 64, 128
+
+
+def _position(x, B, device, what):
+    """(number, device tensor or None) of a position given as an int or as int64 [B] (or [1]) on `device`."""
+    if not torch.is_tensor(x):
+        return int(x), None
+    if x.device != device or x.dtype != torch.int64 or x.numel() not in (1, B) or x.dim() > 1:
+        raise ValueError(f"{what} must be an int or an int64 [{B}] tensor on {device}")
+    return 0, x.reshape(-1).expand(B).contiguous()
+
+
+class KVCache8:
+    """Room for `cap` tokens (rounded up to whole 64-token blocks) of B sequences with Hkv KV heads.
+
+    rows    uint8 [B * Hkv, cap, 2, 128]: e4m3 codes of each token's key (0) and value (1)
+    scales  fp32 [B * Hkv, cap / 64, 2]: powers of two; value = code * scale
+    Either both may be given (contiguous, of these shapes) or they are made, zeroed, on `device`.  Tokens past
+    the last written one are void: no call reads them.  Which tokens a sequence has is the caller's to
+    know: a write says where it begins, a read or an attention where it ends."""
+
+    def __init__(self, B, Hkv, cap, device="cuda", rows=None, scales=None):
+        if B < 1 or Hkv < 1 or cap < 1:
+            raise ValueError(f"KVCache8: B, Hkv and cap must be positive (got {B}, {Hkv}, {cap})")
+        self.B, self.Hkv, self.BH = B, Hkv, B * Hkv
+        self.nblk = -(-cap // BLK)
+        self.cap = self.nblk * BLK
+        if (rows is None) != (scales is None):
+            raise ValueError("KVCache8: rows and scales come together")
+        if rows is None:
+            rows = torch.zeros(self.BH, self.cap, 2, D, dtype=torch.uint8, device=device)
+            scales = torch.zeros(self.BH, self.nblk, 2, dtype=torch.float32, device=device)
+        require_cuda(rows, scales)
+        if rows.dtype != torch.uint8 or tuple(rows.shape) != (self.BH, self.cap, 2, D) or not rows.is_contiguous():
+            raise ValueError(f"KVCache8: rows must be contiguous uint8 [{self.BH}, {self.cap}, 2, {D}]")
+        if (scales.dtype != torch.float32 or tuple(scales.shape) != (self.BH, self.nblk, 2)
+                or not scales.is_contiguous() or scales.device != rows.device):
+            raise ValueError(f"KVCache8: scales must be contiguous float32 [{self.BH}, {self.nblk}, 2] beside the rows")
+        self.rows, self.scales, self.device = rows, scales, rows.device
+
+    def nbytes(self):
+        return self.rows.numel() + self.scales.numel() * 4
+
+    def _check_on(self, what, *tensors):
+        for t in tensors:
+            if t.device != self.device:
+                raise ValueError(f"{what}: expected tensors on {self.device}, got one on {t.device}")
+
+    def write(self, K, V, start=0):
+        """Write K, V [B, Hkv, T, 128] (fp32, bf16 or fp16, any strides) as tokens [start, start + T) of every
+        sequence.  start: an int, or int64 [B] on the device (then a sequence with a negative start is left
+        alone and tokens past cap are dropped).  The scale of a block covers every token written to it in
+        this and in earlier calls; a block written from its first token on starts afresh.  NaN and infinities
+        are stored as NaN and do not enter the scale."""
+        require_cuda(K, V)
+        self._check_on("KVCache8.write", K, V)
+        if K.dim() != 4 or K.shape[0] != self.B or K.shape[1] != self.Hkv or K.shape[3] != D or V.shape != K.shape:
+            raise ValueError(f"KVCache8.write: K and V must be [{self.B}, {self.Hkv}, T, {D}] "
+                             f"(got {tuple(K.shape)}, {tuple(V.shape)})")
+        if K.dtype not in _lib.DTYPE_CODE or V.dtype != K.dtype:
+            raise TypeError(f"KVCache8.write: K and V must both be fp32, bf16 or fp16 (got {K.dtype}, {V.dtype})")
+        T = K.shape[2]
+        num, dev = _position(start, self.B, self.device, "KVCache8.write: start")
+        if dev is None and not 0 <= num <= self.cap - T:
+            raise ValueError(f"KVCache8.write: tokens [{num}, {num + T}) are outside the cache's {self.cap}")
+        if T == 0:
+            return
+        K, V = _rows16(K), _rows16(V)
+        if K.stride() != V.stride():
+            K, V = K.contiguous(), V.contiguous()
+        check(lib().fathom_kv8_write(ptr(K), ptr(V), _lib.DTYPE_CODE[K.dtype], self.B, self.Hkv, T, *K.stride()[:3],
+                                     num, ptr(dev), self.cap, ptr(self.rows), ptr(self.scales), stream_of(self.device)),
+              "KVCache8.write")
+
+    def read(self, start=0, n=None, dtype=torch.bfloat16):
+        """Tokens [start, start + n) (to the end of the cache by default) as (K, V) [B, Hkv, n, 128] in dtype: fp32
+        and bf16 hold the cached values exactly, fp16 rounds."""
+        n = self.cap - start if n is None else n
+        if not 0 <= start <= self.cap or not 0 <= n <= self.cap - start:
+            raise ValueError(f"KVCache8.read: tokens [{start}, {start + n}) are outside the cache's {self.cap}")
+        if dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"KVCache8.read: unsupported dtype {dtype}")
+        K = torch.empty(self.B, self.Hkv, n, D, dtype=dtype, device=self.device)
+        V = torch.empty_like(K)
+        if n:
+            check(lib().fathom_kv8_read(ptr(self.rows), ptr(self.scales), self.BH, self.cap, start, n,
+                                        _lib.DTYPE_CODE[dtype], ptr(K), ptr(V), stream_of(self.device)),
+                  "KVCache8.read")
+        return K, V
+
+    def attend(self, q, end):
+        """softmax(q K^T / sqrt(128)) V of q [B, Hq, T, 128] (bf16 or fp16, any strides; Hq a multiple of Hkv):
+        the T queries of a sequence are its last T tokens, already written, and query t sees the keys
+        [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
+        that sees no key gives 0.  Returns [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
+        require_cuda(q)
+        self._check_on("KVCache8.attend", q)
+        if q.dim() != 4 or q.shape[0] != self.B or q.shape[1] < 1 or q.shape[1] % self.Hkv or q.shape[3] != D:
+            raise ValueError(f"KVCache8.attend: q must be [{self.B}, a multiple of {self.Hkv}, T, {D}] "
+                             f"(got {tuple(q.shape)})")
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"KVCache8.attend: q must be bf16 or fp16 (got {q.dtype})")
+        B, Hq, T, _ = q.shape
+        num, dev = _position(end, B, self.device, "KVCache8.attend: end")
+        if dev is None and not 0 <= num <= self.cap:
+            raise ValueError(f"KVCache8.attend: end {num} is outside the cache's {self.cap}")
+        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=self.device).transpose(1, 2)
+        if T == 0:
+            return out
+        q = _rows16(q)
+        G = Hq // self.Hkv
+        ws = _workspace(self.device, lib().fathom_kv8_attend_workspace_bytes(B, self.Hkv, G, T))
+        check(lib().fathom_kv8_attend(ptr(q), _lib.DTYPE_CODE[q.dtype], B, self.Hkv, G, T, *q.stride()[:3],
+                                      ptr(self.rows), ptr(self.scales), self.cap, num, ptr(dev), ptr(out),
+                                      *out.stride()[:3], ptr(ws), ws.numel(), stream_of(self.device)),
+              "KVCache8.attend")
+        return out
+
+    def attend_picks(self, q, idx, end=None):
+        """Attention over listed tokens, as decode_attention over bf16 rows: q [BH, G, 128] (fp32, bf16 or fp16),
+        idx [BH, G, k] int64.  Picks outside [0, end) are ignored (end: an int, int64 [B] on the device, or None
+        for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  fp32
+        arithmetic; returns [BH, G, 128] in q's dtype."""
+        require_cuda(q, idx)
+        self._check_on("KVCache8.attend_picks", q, idx)
+        if q.dim() != 3 or q.shape[0] != self.BH or q.shape[1] < 1 or q.shape[2] != D:
+            raise ValueError(f"KVCache8.attend_picks: q must be [{self.BH}, G, {D}] (got {tuple(q.shape)})")
+        if q.dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"KVCache8.attend_picks: q must be fp32, bf16 or fp16 (got {q.dtype})")
+        BH, G, _ = q.shape
+        if idx.dim() != 3 or tuple(idx.shape[:2]) != (BH, G) or idx.dtype != torch.int64:
+            raise ValueError(f"KVCache8.attend_picks: idx must be int64 [{BH}, {G}, k] (got {idx.dtype} "
+                             f"{tuple(idx.shape)})")
+        num, dev = _position(self.cap if end is None else end, self.B, self.device, "KVCache8.attend_picks: end")
+        if dev is None and not 0 <= num <= self.cap:
+            raise ValueError(f"KVCache8.attend_picks: end {num} is outside the cache's {self.cap}")
+        k = idx.shape[2]
+        if k == 0:
+            return torch.zeros(BH, G, D, dtype=q.dtype, device=self.device)
+        q, idx = q.contiguous(), idx.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        out = torch.empty(BH, G, D, dtype=q.dtype, device=self.device)
+        ws = _workspace(self.device, lib().fathom_kv8_attend_picks_workspace_bytes(self.B, self.Hkv, G, k))
+        check(lib().fathom_kv8_attend_picks(ptr(q), _lib.DTYPE_CODE[q.dtype], self.B, self.Hkv, G, ptr(idx), k,
+                                            ptr(self.rows), ptr(self.scales), self.cap, num, ptr(dev), ptr(out),
+                                            ptr(ws), ws.numel(), stream_of(self.device)), "KVCache8.attend_picks")
+        return out
+
+
+def _workspace(device, nbytes):
+    """Scratch of one call, from the allocator's pool of the current stream: calls on two streams share none."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _rows16(x):
+    """x with 16-byte aligned, contiguous 128-element rows (a copy where it has none)."""
+    per16 = 16 // x.element_size()
+    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % per16 for s in x.stride()[:-1]):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x

@@ -306,6 +306,52 @@ int fathom_stage_planes(const uint64_t* planes_src, const uint16_t* scales_src, 
                         int64_t nblk, int64_t b0, int64_t b1, uint64_t* planes_dst, uint16_t* scales_dst,
                         void* stream);
 
+/* ---------------------------------------------------------------- 8-bit key/value cache */
+
+/* No reference counterpart (the reference keeps bf16 rows).  A cache of B sequences with Hkv KV heads
+ * (row bh = b*Hkv + h) and room for cap tokens (a multiple of 64):
+ *   rows    [B*Hkv][cap][2][128] uint8  e4m3 codes of each token's key (0) and value (1)
+ *   scales  [B*Hkv][cap/64][2]   fp32   a power of two per 64-token block, for keys and for values
+ *   value = code * scale
+ * Positions come as one number, or as int64 [B] in device memory (`*_dev`, then the number is not read),
+ * which the host never looks at: such calls can be captured in a CUDA graph.  Tokens past the last
+ * written one are void: nothing reads them, whatever they hold. */
+
+/* Write K, V [B][Hkv][T][128] (fp32, bf16 or fp16; strides in elements, the last dimension contiguous,
+ * everything 16-byte aligned) as tokens [start, start + T).  Per block and K or V the scale is 2^e with
+ * the smallest e in [-120, 120] such that every finite |x| <= 448 * 2^e; where the block's first tokens were
+ * written by earlier calls, it is at least their scale, and if it grew their codes are rounded to it.
+ * code = x / scale to nearest, ties to even; NaN and infinities become NaN.  A write ends its sequence's
+ * last block: codes after start + T in that block are void.  With start_dev, a sequence whose start is
+ * negative is left alone and tokens past cap are dropped; with start they are an error. */
+int fathom_kv8_write(const void* K, const void* V, int dtype, int64_t B, int64_t Hkv, int64_t T, int64_t stride_b,
+                     int64_t stride_h, int64_t stride_t, int64_t start, const int64_t* start_dev, int64_t cap,
+                     uint8_t* rows, float* scales, void* stream);
+
+/* Read tokens [start, start + n) back: K, V [BH][n][128] in dtype, code * scale (exact in fp32 and bf16). */
+int fathom_kv8_read(const uint8_t* rows, const float* scales, int64_t BH, int64_t cap, int64_t start, int64_t n,
+                    int dtype, void* K, void* V, void* stream);
+
+/* Workspace bytes of fathom_kv8_attend. */
+size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t T);
+
+/* out = softmax(q K^T / sqrt(128)) V over the cache, for q, out [B][Hkv*G][T][128] (bf16 or fp16; strides in
+ * elements, last dimension contiguous): the T queries of a sequence are its last T tokens, query t sees
+ * the keys [0, end - (T - 1 - t)).  A query that sees no key gives 0.  end above cap is read as cap. */
+int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,
+                      int64_t q_stride_h, int64_t q_stride_t, const uint8_t* rows, const float* scales, int64_t cap,
+                      int64_t end, const int64_t* end_dev, void* out, int64_t o_stride_b, int64_t o_stride_h,
+                      int64_t o_stride_t, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of fathom_kv8_attend_picks. */
+size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k);
+
+/* The same over listed tokens: q, out [B*Hkv][G][128] (fp32, bf16 or fp16), idx [B*Hkv][G][k] int64 token indices.
+ * A pick outside [0, end) is ignored, one listed twice counts twice; no pick left gives 0. */
+int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int64_t Hkv, int G, const int64_t* idx, int64_t k,
+                            const uint8_t* rows, const float* scales, int64_t cap, int64_t end, const int64_t* end_dev,
+                            void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- host memory */
 
 /* Pinned, portable, mapped host allocation and its device alias (host_mapped,
