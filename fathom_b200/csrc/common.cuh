@@ -18,6 +18,11 @@ constexpr int NPLANES = 4;  // 4-bit codes -> 4 bit planes
 // Records a formatted message for fathom_last_error() and returns `status`.
 int set_error(int status, const char* fmt, ...);
 
+// Adds the bounded waits of the cache attention (kv8_attn.cu) that gave up to *count; zeroes them if reset.
+namespace kv8 {
+int wait_timeouts(unsigned long long* count, int reset);
+}
+
 // Checks the launch status of the kernels just enqueued.
 int check_launch(const char* what);
 

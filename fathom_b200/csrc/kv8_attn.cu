@@ -1,18 +1,11 @@
 // Attention over the 8-bit key/value cache (layout in kv8.cuh): over listed rows, and over every row.
 #include "kv8.cuh"
+#include "kv8_attn.cuh"
 
 #include <cooperative_groups.h>
 
 namespace fathom {
-namespace {
-
-namespace cg = cooperative_groups;
-
-constexpr int AW = 8;            // warps per CTA
-constexpr int PG = 4;            // rows per warp instruction: lane groups of 8, a lane holds 16 dims
-constexpr int DPL = 16;
-constexpr int DU = 4;            // rows per lane group per step
-constexpr float QSCALE = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128)
+namespace kv8 {
 
 int sm_count() {
   static int cached[64] = {0};
@@ -26,13 +19,16 @@ int sm_count() {
   return cached[dev];
 }
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ void from_f32(float x, float* p) { *p = x; }
-__device__ __forceinline__ void from_f32(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void from_f32(float x, __half* p) { *p = __float2half_rn(x); }
+namespace {
 
+__device__ unsigned long long g_timeouts = 0;    // waits of the attention kernels that gave up
+
+namespace cg = cooperative_groups;
+
+constexpr int AW = 8;            // warps per CTA
+constexpr int PG = 4;            // rows per warp instruction: lane groups of 8, a lane holds 16 dims
+constexpr int DPL = 16;
+constexpr int DU = 4;            // rows per lane group per step
 struct RowsArgs {
   const int64_t* idx;        // [BH*G][k], or NULL: rows 0 .. end
   int64_t k;
@@ -223,14 +219,53 @@ int dispatch_rows(int dtype, const void* q, const RowsArgs& a, int64_t rows, voi
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The rows as a 3-D tensor of bytes [BH][cap][256], read in 128-byte wide tiles of 128 tokens (the key or the
+// value half of each) in the 128-byte swizzle; tokens past cap read as 0.
+int rows_map(const Args& a, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e =
+        cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess || found != cudaDriverEntryPointSuccess || !fn)
+      return set_error(FATHOM_ERR_CUDA, "kv8_attend: the driver has no cuTensorMapEncodeTiled");
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  const cuuint64_t dims[3] = {(cuuint64_t)KV8_ROW, (cuuint64_t)a.cap, (cuuint64_t)a.B * a.Hkv};
+  const cuuint64_t strides[2] = {(cuuint64_t)KV8_ROW, (cuuint64_t)a.cap * KV8_ROW};
+  const cuuint32_t box[3] = {(cuuint32_t)D, 128, 1}, step[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(a.rows), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FATHOM_ERR_CUDA, "kv8_attend: tensor map: error %d", (int)r);
+  return FATHOM_OK;
+}
+
 }  // namespace
+
+// Adds the waits that gave up to *count, and zeroes them on request.
+int wait_timeouts(unsigned long long* count, int reset) {
+  unsigned long long v = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_timeouts, sizeof(v));
+  if (e == cudaSuccess && reset) e = cudaMemcpyToSymbol(g_timeouts, &zero, sizeof(zero));
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "wait_timeouts: %s", cudaGetErrorString(e));
+  *count += v;
+  return FATHOM_OK;
+}
+
+}  // namespace kv8
 }  // namespace fathom
 
 using namespace fathom;
+using namespace fathom::kv8;
 
 extern "C" size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t T) {
   if (B <= 0 || Hkv <= 0 || G <= 0 || T <= 0) return 0;
-  return 256;
+  return G * T <= TOKEN_ROWS ? token_workspace(B * Hkv, G * T) : 256;
 }
 
 extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,
@@ -251,9 +286,19 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
                  "kv8_attend: rows, q and out (with their strides) must be 16-byte aligned");
   FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_workspace_bytes(B, Hkv, G, T), FATHOM_ERR_WORKSPACE,
                  "kv8_attend: workspace too small");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (G * T <= TOKEN_ROWS) {
+    unsigned long long* timeouts = nullptr;
+    cudaGetSymbolAddress(reinterpret_cast<void**>(&timeouts), g_timeouts);
+    const Args a{q, q_stride_b, q_stride_h, q_stride_t, out, o_stride_b, o_stride_h, o_stride_t, rows, scales, cap, end,
+                 end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts};
+    CUtensorMap map;
+    const int r = rows_map(a, &map);
+    return r != FATHOM_OK ? r : token_attend(map, a, dtype, st);
+  }
   const RowsArgs a{nullptr, 0, rows, scales, cap, end, end_dev, (int)Hkv, G, T, q_stride_b, q_stride_h, q_stride_t,
                    o_stride_b, o_stride_h, o_stride_t};
-  return dispatch_rows(dtype, q, a, B * Hkv * G * T, out, reinterpret_cast<cudaStream_t>(stream));
+  return dispatch_rows(dtype, q, a, B * Hkv * G * T, out, st);
 }
 
 extern "C" size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k) {

@@ -1,0 +1,58 @@
+// What the attention kernels over the 8-bit cache share: their arguments, the softmax's units, conversions.
+#pragma once
+#include "kv8.cuh"
+
+#include <cuda.h>
+
+namespace fathom {
+namespace kv8 {
+
+constexpr float QSCALE = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128): base-2 scores
+constexpr int PART = D + 4;      // floats of a partial result: 128 dims, reference, denominator, padding
+
+// Attention over a whole cache: T queries for each of Hkv * G heads of B sequences.  Strides in elements.
+struct Args {
+  const void* q;
+  int64_t qb, qh, qt;
+  void* out;
+  int64_t ob, oh, ot;
+  const uint8_t* rows;
+  const float* scales;
+  int64_t cap, end;
+  const int64_t* end_dev;         // per sequence, or NULL
+  int B, Hkv, G;
+  int64_t T;
+  float* part;                    // workspace: partial results
+  unsigned long long* timeouts;   // counts waits that gave up
+};
+
+// Tokens of sequence b that exist.
+__device__ __forceinline__ int64_t seq_end(const Args& a, int b) {
+  int64_t e = a.end_dev ? a.end_dev[b] : a.end;
+  e = e > a.cap ? a.cap : e;
+  return e > 0 ? e : 0;
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ void from_f32(float x, float* p) { *p = x; }
+__device__ __forceinline__ void from_f32(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void from_f32(float x, __half* p) { *p = __float2half_rn(x); }
+
+// 2^x by the special-function unit (2 ulp; results below 2^-126 are 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+int sm_count();
+
+// kv8_token.cu: up to TOKEN_ROWS query rows (G * T) per KV head.
+constexpr int TOKEN_ROWS = 32;
+size_t token_workspace(int64_t BH, int64_t R);
+int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
+
+}  // namespace kv8
+}  // namespace fathom

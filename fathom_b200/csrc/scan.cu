@@ -736,6 +736,8 @@ extern "C" int fathom_wait_timeouts(unsigned long long* count, int reset) {
     e = cudaMemcpyToSymbol(g_wait_timeouts, &zero, sizeof(zero));
   }
   if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "wait_timeouts: %s", cudaGetErrorString(e));
+  const int r = kv8::wait_timeouts(&v, reset);     // the cache attention's waits
+  if (r != FATHOM_OK) return r;
   if (count) *count = v;
   return FATHOM_OK;
 }
