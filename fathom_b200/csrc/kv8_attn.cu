@@ -265,7 +265,7 @@ using namespace fathom::kv8;
 
 extern "C" size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t T) {
   if (B <= 0 || Hkv <= 0 || G <= 0 || T <= 0) return 0;
-  return G * T <= TOKEN_ROWS ? token_workspace(B * Hkv, G * T) : 256;
+  return G * T <= TOKEN_ROWS ? token_workspace(B * Hkv, G * T) : prompt_workspace();
 }
 
 extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,
@@ -287,18 +287,15 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
   FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_workspace_bytes(B, Hkv, G, T), FATHOM_ERR_WORKSPACE,
                  "kv8_attend: workspace too small");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (G * T <= TOKEN_ROWS) {
-    unsigned long long* timeouts = nullptr;
-    cudaGetSymbolAddress(reinterpret_cast<void**>(&timeouts), g_timeouts);
-    const Args a{q, q_stride_b, q_stride_h, q_stride_t, out, o_stride_b, o_stride_h, o_stride_t, rows, scales, cap, end,
-                 end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts};
-    CUtensorMap map;
-    const int r = rows_map(a, &map);
-    return r != FATHOM_OK ? r : token_attend(map, a, dtype, st);
-  }
-  const RowsArgs a{nullptr, 0, rows, scales, cap, end, end_dev, (int)Hkv, G, T, q_stride_b, q_stride_h, q_stride_t,
-                   o_stride_b, o_stride_h, o_stride_t};
-  return dispatch_rows(dtype, q, a, B * Hkv * G * T, out, st);
+  unsigned long long* timeouts = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&timeouts), g_timeouts);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  const Args a{q, q_stride_b, q_stride_h, q_stride_t, out, o_stride_b, o_stride_h, o_stride_t, rows, scales, cap, end,
+               end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts};
+  CUtensorMap map;
+  const int r = rows_map(a, &map);
+  if (r != FATHOM_OK) return r;
+  return G * T <= TOKEN_ROWS ? token_attend(map, a, dtype, st) : prompt_attend(map, a, dtype, st);
 }
 
 extern "C" size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k) {

@@ -53,6 +53,9 @@ int sm_count();
 constexpr int TOKEN_ROWS = 32;
 size_t token_workspace(int64_t BH, int64_t R);
 int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
+// kv8_prompt.cu: any number of query rows, 256 at a time.
+size_t prompt_workspace();
+int prompt_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace fathom

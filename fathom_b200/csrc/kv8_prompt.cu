@@ -1,0 +1,617 @@
+// Attention of many query rows per KV head over the 8-bit cache (layout in kv8.cuh): prompt chunks, long drafts.
+//
+// Bound by the tensor cores, and as closely by the special-function units: a 128-token tile against 256 query
+// rows is 2 x 2 products of 128 x 128 x 128, ~2048 cycles, and 32768 exponentials at 16 a cycle.  Rows are
+// the (token, head) pairs of one KV head, token-major, so G heads share every tile.  Per CTA:
+//
+//   S_i [128 rows x 128 tokens] = (q1 + q2 [+ q3]) K^T   e4m3 x e4m3: q as a sum of e4m3 terms (2 hold a bf16, 3 an
+//                                                        fp16), the key tile straight from TMA; 2 terms at twice
+//                                                        the rate cost one 16-bit product, and no key is converted
+//   O_i [128 rows x 128 dims]  += P_i V                  f16 x f16: an e4m3 value is exact in f16; weights in
+//                                                        tensor memory over the scores they came from
+//
+// for the two halves i of the rows, in turn: while one warpgroup takes the softmax of its scores, the tensor
+// cores work for the other.  A third warpgroup turns value tiles into f16.  The key scale multiplies the score and
+// the value scale 2^ev, a constant of each 64-token half of a tile, enters the weight's exponent, so a row sees its own
+// range whatever other blocks hold.  Softmax, thread = row: m, the reference of s + ev, follows the row's maximum
+// only when that exceeds it by 2^7 (then O is rescaled); weights are 2^(s + ev - m + 8), at most 2^15 in f16, rounded to
+// 11 bits; sums in fp32, the denominator taking each half's sum times 2^(largest ev - ev).  Blocks whose
+// scale is below 2^-40 of the sequence's largest count as 2^-40 there and have the rest multiplied into their
+// f16 values, which keeps the denominator in range.
+//
+// Work: the tiles of all (bh, 256 rows) items in a line, cut into equal contiguous shares, one per CTA; an item cut
+// by a share's end leaves parts in the workspace, which a second kernel joins in a fixed order.
+#include "kv8.cuh"
+#include "kv8_attn.cuh"
+#include "tc.cuh"
+
+namespace fathom {
+namespace kv8 {
+namespace {
+
+constexpr int TILE = 128;                    // tokens per tile
+constexpr int HALF = 128, ROWS = 2 * HALF;   // query rows of a warpgroup, of a CTA
+constexpr int KSTAGES = 3, VSTAGES = 2;
+constexpr int KBYTES = TILE * D, VBYTES = 2 * TILE * D;
+constexpr int THREADS = 512;                 // warps 0-3, 4-7: softmax; 8-11: values; 12: products; 13: key loads
+constexpr float SLACK = 7.0f;                // a row may exceed its reference by 2^7
+constexpr float HEAD = 8.0f;                 // weights at the reference are 2^8
+constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
+// registers per thread of the softmax, value and other warpgroups: together the 512 * 128 of the launch
+constexpr int REG_SOFT = 176, REG_VALUE = 104, REG_OTHER = 56;
+static_assert(2 * REG_SOFT + REG_VALUE + REG_OTHER == 4 * 128, "register split");
+
+template <int QT> struct Shape {
+  static constexpr int Q = 0, K = 2 * QT * HALF * D, V = K + KSTAGES * KBYTES, END = V + VSTAGES * VBYTES;
+  static constexpr int SMEM = END + 1024;
+};
+
+__device__ __forceinline__ int64_t items_per_bh(const Args& a) { return (a.G * a.T + ROWS - 1) / ROWS; }
+
+// Keys that row `row` (token-major) of a sequence with `end` tokens sees.
+__device__ __forceinline__ int64_t seen(const Args& a, int64_t end, int64_t row) { return end - (a.T - 1) + row / a.G; }
+
+// Tiles of item `it` of a row bh: up to its last row's last key, one at least.
+__device__ __forceinline__ int64_t tiles_of(const Args& a, int64_t end, int64_t it) {
+  const int64_t last = min((it + 1) * ROWS, a.G * a.T) - 1;
+  const int64_t n = (seen(a, end, last) + TILE - 1) / TILE;
+  return n > 1 ? n : 1;
+}
+
+// One warp: sum of f over [0, n); if at >= 0, also the first i whose running sum exceeds at (and the sum before it).
+template <typename F> __device__ int64_t warp_line(int64_t n, int64_t at, int64_t* where, int64_t* before, F f) {
+  const int lane = threadIdx.x & 31;
+  int64_t total = 0;
+  bool found = at < 0;
+  for (int64_t i0 = 0; i0 < n; i0 += 32) {
+    const int64_t mine = i0 + lane < n ? f(i0 + lane) : 0;
+    int64_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (!found) {
+      const unsigned hit = __ballot_sync(0xffffffffu, total + x > at);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        *where = i0 + l;
+        *before = total + __shfl_sync(0xffffffffu, x - mine, l);
+        found = true;
+      }
+    }
+    total += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return total;
+}
+
+struct Place {
+  int64_t item;      // bh * items_per_bh + it
+  int64_t tile;      // tile within the item
+};
+
+// One warp: tiles of all items.
+__device__ int64_t line_length(const Args& a) {
+  int64_t w, s;
+  const int64_t per = items_per_bh(a);
+  if (!a.end_dev) {
+    const int64_t end = seq_end(a, 0);
+    return warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); }) * a.B * a.Hkv;
+  }
+  int64_t total = 0;
+  for (int b = 0; b < a.B; ++b) {
+    const int64_t end = seq_end(a, b);
+    total += warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); }) * a.Hkv;
+  }
+  return total;
+}
+
+// One warp: the item that holds tile `at` of the line (at < its length).
+__device__ Place locate(const Args& a, int64_t at) {
+  int64_t w = 0, s = 0;
+  const int64_t per = items_per_bh(a);
+  int b = 0;
+  int64_t one = 0;
+  for (;; ++b) {
+    const int64_t end = seq_end(a, b);
+    if (b == 0 || a.end_dev) one = warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); });
+    if (at < one * a.Hkv || b + 1 == a.B) break;
+    at -= one * a.Hkv;
+  }
+  const int64_t h = at / one, end = seq_end(a, b);
+  at -= h * one;
+  warp_line(per, at, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); });
+  return Place{((int64_t)b * a.Hkv + h) * per + w, at - s};
+}
+
+// A share as its pieces of items, the same walk in every role.
+struct Walk {
+  const Args& a;
+  int64_t per, item, tile, left;
+  int b, bh;
+  int64_t it, end, n, j0, j1;      // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
+  __device__ Walk(const Args& a_, const Place& p, int64_t count) : a(a_), per(items_per_bh(a_)), item(p.item), tile(p.tile), left(count) {}
+  __device__ bool next() {
+    if (left <= 0) return false;
+    bh = (int)(item / per);
+    it = item % per;
+    b = bh / a.Hkv;
+    end = seq_end(a, b);
+    n = tiles_of(a, end, it);
+    j0 = tile;
+    j1 = min(n, j0 + left);
+    left -= j1 - j0;
+    ++item;
+    tile = 0;
+    return true;
+  }
+};
+
+// One warp: log2 of the largest value scale among the first `end` tokens' blocks.
+__device__ int largest_ev(const float2* sc, int64_t end) {
+  int ev = KV8_EMIN;
+#pragma unroll 8
+  for (int64_t b = threadIdx.x & 31; b < (end + BLK - 1) / BLK; b += 32)
+    ev = max(ev, (int)(__float_as_uint(sc[b].y) >> 23) - 127);
+  return __reduce_max_sync(0xffffffffu, ev);
+}
+// log2 of a block's value scale as the weights take it.
+__device__ __forceinline__ int weight_ev(float scale, int largest) {
+  return min(largest, max(largest - EV_SPAN, (int)(__float_as_uint(scale) >> 23) - 127));
+}
+
+template <int N> __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int QT>
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constant__ CUtensorMap map,
+                                                           const __grid_constant__ Args a) {
+  using S = Shape<QT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t sbase = tc::smem_u32(smem);
+  __shared__ __align__(8) uint64_t bars[2 * KSTAGES + 2 * VSTAGES + 7];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_gave_up;
+  __shared__ Place s_place;
+  __shared__ int64_t s_count;
+  __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];         // tokens whose value holds a NaN (tiles whose mask differs by row)
+  const uint32_t bar = tc::smem_u32(bars);
+  auto k_full = [&](int64_t i) { return bar + 8 * (uint32_t)(i % KSTAGES); };
+  auto k_free = [&](int64_t i) { return bar + 8 * (uint32_t)(KSTAGES + i % KSTAGES); };
+  const uint32_t bar2 = bar + 16 * KSTAGES;
+  auto v_full = [&](int64_t i) { return bar2 + 8 * (uint32_t)(i % VSTAGES); };
+  auto v_free = [&](int64_t i) { return bar2 + 8 * (uint32_t)(VSTAGES + i % VSTAGES); };
+  const uint32_t bar3 = bar2 + 16 * VSTAGES;
+  auto s_full = [&](int h) { return bar3 + 8 * h; };
+  auto p_full = [&](int h) { return bar3 + 16 + 8 * h; };
+  auto q_full = [&](int h) { return bar3 + 32 + 8 * h; };
+  const uint32_t drain = bar3 + 48;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp >> 2;
+  volatile int* gave_up = &s_gave_up;
+
+  if (tid == 0) {
+    for (int i = 0; i < KSTAGES; ++i) tc::mbar_init(k_full(i), 1), tc::mbar_init(k_free(i), 1);
+    for (int i = 0; i < VSTAGES; ++i) tc::mbar_init(v_full(i), 4), tc::mbar_init(v_free(i), 1);
+    for (int h = 0; h < 2; ++h) tc::mbar_init(s_full(h), 1), tc::mbar_init(p_full(h), 4), tc::mbar_init(q_full(h), 4);
+    tc::mbar_init(drain, 1);
+    tc::fence_mbar_init();
+    s_gave_up = 0;
+  }
+  if (warp == 12) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
+  if (warp == 0) {
+    const int64_t total = line_length(a), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
+    Place p{0, 0};
+    if (first < total) p = locate(a, first);
+    if (lane == 0) s_place = p, s_count = min(share, total - first);
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tm = s_tmem;                      // S_0, S_1, O_0, O_1: 128 columns each
+  Walk w(a, s_place, s_count);
+
+  if (group < 2) {
+    // ---- softmax of half `group`: thread = row
+    reg_more<REG_SOFT>();
+    const int h2 = group, r = tid & (HALF - 1);
+    const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tm_s = tm + h2 * 128 + my, tm_o = tm + 256 + h2 * 128 + my;
+    uint8_t* sq = smem + S::Q + h2 * QT * HALF * D;
+    int64_t phase = 0, vt = 0;                     // completions of s_full seen; tiles seen
+    bool ok = true;
+    while (w.next()) {
+      const int64_t total = a.G * a.T, row = w.it * ROWS + h2 * HALF + r;
+      const bool real = row < total;
+      const int64_t rr = real ? row : total - 1;
+      const int hq = (w.bh % a.Hkv) * a.G + (int)(rr % a.G);
+      const int64_t tt = rr / a.G, limit = seen(a, w.end, rr);
+      // the row's query as e4m3 terms of its own scale
+      float rs;
+      {
+        const T* qp = reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt;
+        uint4 v[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          v[i] = *reinterpret_cast<const uint4*>(qp + 8 * i);
+          const T* e = reinterpret_cast<const T*>(&v[i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f32(e[j])) & 0x7FFFFFFFu);
+        }
+        const int e2 = kv8_exponent(top);
+        const float inv = pow2i(-e2);
+        rs = pow2i(e2) * QSCALE;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          float x[16];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const T* e = reinterpret_cast<const T*>(&v[2 * c + i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[8 * i + j] = to_f32(e[j]) * inv;
+          }
+#pragma unroll
+          for (int term = 0; term < QT; ++term) {
+            uint32_t code[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              code[i] = kv8_encode2(x[4 * i], x[4 * i + 1]) | kv8_encode2(x[4 * i + 2], x[4 * i + 3]) << 16;
+              const float2 lo = kv8_decode2(code[i]), hi = kv8_decode2(code[i] >> 16);
+              x[4 * i] -= lo.x, x[4 * i + 1] -= lo.y, x[4 * i + 2] -= hi.x, x[4 * i + 3] -= hi.y;
+            }
+            *reinterpret_cast<uint4*>(sq + term * HALF * D + r * D + ((c ^ (r & 7)) << 4)) =
+                make_uint4(code[0], code[1], code[2], code[3]);
+          }
+        }
+      }
+      tc::fence_async_smem();
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(q_full(h2));
+      // keys that every row of the CTA sees need no mask
+      const int64_t all_see = seen(a, w.end, w.it * ROWS);
+      const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
+      const int ev = largest_ev(sc, w.end);
+      float m = -INFINITY, l = 0.0f;
+      for (int64_t j = w.j0; j < w.j1; ++j, ++vt) {
+        const int64_t blk = j * (TILE / BLK);
+        // above 0, so that a masked score stays -inf; void blocks may hold anything, NaN too
+        const float2 sc0 = sc[blk], sc1 = blk + 1 < a.cap / BLK ? sc[blk + 1] : make_float2(0.0f, 0.0f);
+        const float c0 = fmaxf(sc0.x * rs, 1e-37f), c1 = fmaxf(sc1.x * rs, 1e-37f);
+        const int ev0 = weight_ev(sc0.y, ev), ev1 = weight_ev(sc1.y, ev);
+        ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);
+        ++phase;
+        __syncwarp();
+        tc::fence_after();
+        uint32_t x[TILE];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc::Tmem<32>::ld(tm_s + 32 * i, x + 32 * i);
+        tc::wait_ld();
+        if ((j + 1) * TILE > all_see) {
+          const int64_t room = limit - j * TILE;   // keys of the tile that this row sees
+          const int see = room < 0 ? 0 : room > TILE ? TILE : (int)room;
+#pragma unroll
+          for (int i = 0; i < TILE; ++i)
+            if (i >= see) x[i] = 0xFF800000u;      // -inf
+          ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
+          __syncwarp();
+          for (int i = 0; i < TILE; i += 4)
+            if (const uint32_t f = *reinterpret_cast<const uint32_t*>(&s_nan[vt % VSTAGES][i]))
+              if (i + (__ffs(f) - 1) / 8 < see) l = __uint_as_float(0x7FFFFFFFu);
+          __syncwarp();
+        }
+        float m0[4], m1[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m0[i] = __uint_as_float(x[i]), m1[i] = __uint_as_float(x[64 + i]);
+#pragma unroll
+        for (int i = 4; i < 64; ++i) {
+          m0[i & 3] = fmaxf(m0[i & 3], __uint_as_float(x[i]));
+          m1[i & 3] = fmaxf(m1[i & 3], __uint_as_float(x[64 + i]));
+        }
+        const float t0 = fmaxf(fmaxf(m0[0], m0[1]), fmaxf(m0[2], m0[3])), t1 = fmaxf(fmaxf(m1[0], m1[1]), fmaxf(m1[2], m1[3]));
+        const float top = fmaxf(fmaf(t0, c0, (float)ev0), fmaf(t1, c1, (float)ev1));
+        const bool up = top > m + SLACK;           // also the first time: m = -inf
+        if (__any_sync(0xffffffffu, up)) {
+          const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+          if (up) m = top;
+          l *= f;
+          if (j > w.j0) {                          // O of the tiles before is complete: their products precede this S
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              uint32_t o[32];
+              tc::Tmem<32>::ld(tm_o + 32 * i, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc::Tmem<32>::st(tm_o + 32 * i, o);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : HEAD - m, off0 = off + (float)ev0, off1 = off + (float)ev1;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // of the first half's even and odd tokens, of the second's
+#pragma unroll
+        for (int i = 0; i < TILE; i += 2) {
+          const float c = i < 64 ? c0 : c1, o = i < 64 ? off0 : off1;
+          const float p0 = ex2(fmaf(__uint_as_float(x[i]), c, o)), p1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, o));
+          sum[i / 64 * 2] += p0;
+          sum[i / 64 * 2 + 1] += p1;
+          x[i / 2] = pack_h2(p0, p1);
+        }
+        l = fmaf(sum[0] + sum[1], pow2i(ev - ev0), l);
+        l = fmaf(sum[2] + sum[3], pow2i(ev - ev1), l);
+        tc::Tmem<32>::st(tm_s, x);
+        tc::Tmem<32>::st(tm_s + 32, x + 32);
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full(h2));
+      }
+      ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);      // the piece's last product
+      ++phase;
+      __syncwarp();
+      tc::fence_after();
+      const bool whole = w.j0 == 0 && w.j1 == w.n;
+      const float vscale = pow2i(ev);              // the denominator is relative to the largest scale
+      const float f = !ok ? __uint_as_float(0x7FFFFFFFu) : whole ? (l == 0.0f ? 0.0f : vscale / l) : vscale;
+      T* op = reinterpret_cast<T*>(a.out) + w.b * a.ob + hq * a.oh + tt * a.ot;
+      float* part = a.part + ((2 * (int64_t)blockIdx.x + (w.j0 == 0 ? 1 : 0)) * ROWS + h2 * HALF + r) * PART;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        uint32_t o[32];
+        __syncwarp();
+        tc::Tmem<32>::ld(tm_o + 32 * i, o);
+        tc::wait_ld();
+        if (!real) continue;
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            T y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) from_f32(l == 0.0f ? 0.0f : __uint_as_float(o[8 * c + e]) * f, &y[e]);
+            *reinterpret_cast<uint4*>(op + 32 * i + 8 * c) = *reinterpret_cast<const uint4*>(y);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(part + 32 * i + 4 * c) =
+                make_float4(__uint_as_float(o[4 * c]) * f, __uint_as_float(o[4 * c + 1]) * f,
+                            __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
+        }
+      }
+      if (real && !whole) part[D] = m, part[D + 1] = l;
+      __syncwarp();
+      tc::fence_before();
+    }
+  } else if (group == 2) {
+    // ---- values: e4m3 rows from memory to f16, MN-major tiles of two 64-dim halves.  Thread = 16 dims of 8 tokens.
+    reg_less<REG_VALUE>();
+    const int t = tid - 256, u = t & 7, row0 = t >> 3;
+    int64_t i = 0;
+    bool ok = true;
+    while (ok && w.next()) {
+      const uint8_t* base = a.rows + (int64_t)w.bh * a.cap * KV8_ROW + D + u * 16;
+      const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
+      const int ev = largest_ev(sc, w.end);
+      const int64_t all_see = seen(a, w.end, w.it * ROWS);
+      for (int64_t j = w.j0; j < w.j1; ++j, ++i) {
+        uint4 v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const int64_t tok = j * TILE + p * 16 + row0;
+          v[p] = tok < w.end ? *reinterpret_cast<const uint4*>(base + tok * KV8_ROW) : make_uint4(0, 0, 0, 0);
+        }
+        int rest[2];                               // log2 of what the weights leave of the block's scale
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t blk = j * 2 + e;
+          const float s = blk * BLK < w.end ? sc[blk].y : 1.0f;
+          rest[e] = blk * BLK < w.end ? (int)(__float_as_uint(s) >> 23) - 127 - weight_ev(s, ev) : 0;
+        }
+        ok = ok && tc::mbar_wait(v_free(i), ((i / VSTAGES) & 1) ^ 1, gave_up);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* vb = smem + S::V + (i % VSTAGES) * VBYTES + (u >> 2) * (TILE * 128);
+        const bool differs = (j + 1) * TILE > all_see;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const int tk = p * 16 + row0;
+          uint32_t x[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+          if (differs) {
+            // 0 * NaN would reach rows that do not see the token: its NaNs leave the product, and the rows that do
+            // see it become NaN by their denominators
+            bool nan = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t is = __vcmpeq4(x[e] & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+              nan = nan || is;
+              x[e] &= ~is;
+            }
+            const unsigned any = __ballot_sync(0xffffffffu, nan) >> (lane & 24) & 255u;
+            if (u == 0) s_nan[i % VSTAGES][tk] = any != 0;
+          }
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x[e >> 1] >> (16 * (e & 1))), __NV_E4M3);
+            y[e] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          if (rest[p >> 2] != 0) {
+            const __half2 k = __float2half2_rn(rest[p >> 2] < -40 ? 0.0f : pow2i(rest[p >> 2]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y[e]), k);
+              y[e] = *reinterpret_cast<const uint32_t*>(&z);
+            }
+          }
+          uint8_t* dst = vb + tk * 128;
+          const int c = (u & 3) * 2;
+          *reinterpret_cast<uint4*>(dst + ((c ^ (tk & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (tk & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(v_full(i));
+      }
+    }
+  } else {
+    reg_less<REG_OTHER>();
+    if (warp == 13 && lane == 0) {
+      // ---- key tiles
+      int64_t i = 0;
+      bool ok = true;
+      while (ok && w.next()) {
+        for (int64_t j = w.j0; j < w.j1; ++j, ++i) {
+          ok = tc::mbar_wait(k_free(i), ((i / KSTAGES) & 1) ^ 1, gave_up);
+          if (!ok) break;
+          tc::mbar_expect_tx(k_full(i), KBYTES);
+          tc::tma_load_3d(sbase + S::K + (uint32_t)(i % KSTAGES) * KBYTES, &map, 0, (int)(j * TILE), w.bh, k_full(i));
+        }
+      }
+      if (*gave_up) {
+        for (int64_t j = i > KSTAGES ? i - KSTAGES : 0; j < i; ++j) {   // copies in flight land first
+          const unsigned long long t0 = tc::now_ns();
+          while (!tc::mbar_try(k_full(j), (j / KSTAGES) & 1) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
+        }
+      }
+    } else if (warp == 12 && lane == 0) {
+      // ---- products
+      constexpr uint32_t id_s = tc::instr(TILE, false, false), id_o = tc::instr(D, false, true);
+      int64_t i = 0, pn = 0, seg = 0;              // key tile, weight tiles done, pieces begun
+      bool ok = true;
+      auto scores = [&](int h, int64_t i) {
+        const uint64_t dk = tc::operand(sbase + S::K + (uint32_t)(i % KSTAGES) * KBYTES);
+#pragma unroll
+        for (int term = 0; term < QT; ++term) {
+          const uint64_t dq = tc::operand(sbase + S::Q + (h * QT + term) * HALF * D);
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk)
+            tc::mma_fp8(tm + h * 128, dq + kk * 2, dk + kk * 2, id_s, term > 0 || kk > 0);
+        }
+      };
+      auto values = [&](int h, int64_t i, bool accumulate) {
+        const uint64_t dv = tc::operand(sbase + S::V + (uint32_t)(i % VSTAGES) * VBYTES, TILE * 128);
+#pragma unroll
+        for (int kk = 0; kk < TILE / 16; ++kk)     // 16 tokens a step: 8 columns of weights, 2 groups of 8 value rows
+          tc::mma_f16_ts(tm + 256 + h * 128, tm + h * 128 + kk * 8, dv + kk * (16 * 128 / 16), id_o, accumulate || kk > 0);
+      };
+      while (ok && w.next()) {
+        const int64_t n = w.j1 - w.j0;
+        for (int h = 0; h < 2; ++h) ok = ok && tc::mbar_wait(q_full(h), seg & 1, gave_up);
+        ++seg;
+        ok = ok && tc::mbar_wait(k_full(i), (i / KSTAGES) & 1, gave_up);
+        if (!ok) break;
+        tc::fence_after();
+        for (int h = 0; h < 2; ++h) {
+          scores(h, i);
+          tc::mma_commit(s_full(h));
+        }
+        tc::mma_commit(k_free(i));
+        for (int64_t j = 1; j <= n && ok; ++j) {
+          const int64_t v = i + j - 1;
+          const bool last = j == n;
+          if (!last) ok = tc::mbar_wait(k_full(i + j), ((i + j) / KSTAGES) & 1, gave_up);
+          ok = ok && tc::mbar_wait(v_full(v), (v / VSTAGES) & 1, gave_up);
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = tc::mbar_wait(p_full(h), pn & 1, gave_up);
+            if (!ok) break;
+            tc::fence_after();
+            values(h, v, j > 1);
+            if (h == 1) tc::mma_commit(v_free(v));
+            if (!last) {
+              scores(h, i + j);
+              if (h == 1) tc::mma_commit(k_free(i + j));
+            }
+            tc::mma_commit(s_full(h));             // the next scores, or the piece's last product
+          }
+          ++pn;
+        }
+        i += n;
+      }
+      if (*gave_up) {
+        tc::mma_commit(drain);
+        const unsigned long long t0 = tc::now_ns();
+        while (!tc::mbar_try(drain, 0) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
+      }
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 12) tc::tmem_free(tm, 512);
+  if (tid == 0 && s_gave_up) atomicAdd(a.timeouts, 1ull);
+}
+
+// Joins the items that shares cut: block (c, rows) looks at the cut before share c + 1, and joins the item it
+// falls into if that is the item's first cut.  Warp = row, lane = 4 dims.
+constexpr int JOIN_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args a, int ctas) {
+  __shared__ Place s_place;
+  __shared__ int64_t s_total, s_n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = items_per_bh(a);
+  if (warp == 0) {
+    const int64_t total = line_length(a), share = (total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
+    Place p{0, 0};
+    int64_t n = 0;
+    if (cut < total) {
+      p = locate(a, cut);
+      n = tiles_of(a, seq_end(a, (int)(p.item / per / a.Hkv)), p.item % per);
+    }
+    if (lane == 0) s_place = p, s_total = total, s_n = n;
+  }
+  __syncthreads();
+  const Place p = s_place;
+  const int64_t share = (s_total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
+  if (p.tile == 0 || p.tile > share) return;       // no item is cut here, or an earlier cut joins it
+  const int64_t first = cut - p.tile;              // the item's first tile in the line
+  const int64_t c0 = blockIdx.x, c1 = (first + s_n - 1) / share;
+  const int64_t bh = p.item / per, it = p.item % per, total = a.G * a.T;
+  const int64_t r = (int64_t)blockIdx.y * JOIN_WARPS + warp, row = it * ROWS + r;
+  if (row >= total) return;
+  // parts: share c0 holds the item's first tiles (its second slot), the others begin with it (first slot)
+  auto part = [&](int64_t c) { return a.part + ((2 * c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
+  float M = -INFINITY, L = 0.0f;
+  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, part(c)[D]);
+  for (int64_t c = c0; c <= c1; ++c) {
+    const float m = part(c)[D], e = m == -INFINITY ? 0.0f : exp2f(m - M);
+    const float4 o = *reinterpret_cast<const float4*>(part(c) + 4 * lane);
+    L = fmaf(part(c)[D + 1], e, L);
+    O.x = fmaf(o.x, e, O.x), O.y = fmaf(o.y, e, O.y), O.z = fmaf(o.z, e, O.z), O.w = fmaf(o.w, e, O.w);
+  }
+  const float f = L == 0.0f ? 0.0f : 1.0f / L;
+  T y[4];
+  from_f32(O.x * f, &y[0]), from_f32(O.y * f, &y[1]), from_f32(O.z * f, &y[2]), from_f32(O.w * f, &y[3]);
+  const int64_t b = bh / a.Hkv, hq = (bh % a.Hkv) * a.G + row % a.G;
+  T* op = reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + row / a.G * a.ot + 4 * lane;
+  *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
+}
+
+template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
+  using S = Shape<QT>;
+  static_assert(S::SMEM <= 226 * 1024, "shared memory");
+  const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
+  if (ctas > 1) prompt_join_kernel<T><<<dim3(ctas - 1, ROWS / JOIN_WARPS), JOIN_WARPS * 32, 0, st>>>(a, ctas);
+  return check_launch("kv8_attend");
+}
+
+}  // namespace
+
+size_t prompt_workspace() { return (size_t)sm_count() * 2 * ROWS * PART * sizeof(float); }
+
+int prompt_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st) {
+  const int ctas = sm_count();
+  return dtype == FATHOM_DTYPE_BF16 ? launch<__nv_bfloat16, 2>(map, a, ctas, st) : launch<__half, 3>(map, a, ctas, st);
+}
+
+}  // namespace kv8
+}  // namespace fathom
