@@ -36,10 +36,10 @@ constexpr int KBYTES = TILE * D, VBYTES = 2 * TILE * D;
 constexpr int THREADS = 512;                 // warps 0-3, 4-7: softmax; 8-11: values; 12: products; 13: key loads
 constexpr float SLACK = 7.0f;                // a row may exceed its reference by 2^7
 constexpr float HEAD = 8.0f;                 // weights at the reference are 2^8
-constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
 // registers per thread of the softmax, value and other warpgroups: together the 512 * 128 of the launch
-constexpr int REG_SOFT = 176, REG_VALUE = 104, REG_OTHER = 56;
+constexpr int REG_SOFT = 168, REG_VALUE = 88, REG_OTHER = 88;
 static_assert(2 * REG_SOFT + REG_VALUE + REG_OTHER == 4 * 128, "register split");
+constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
 
 template <int QT> struct Shape {
   static constexpr int Q = 0, K = 2 * QT * HALF * D, V = K + KSTAGES * KBYTES, END = V + VSTAGES * VBYTES;
@@ -127,17 +127,17 @@ __device__ Place locate(const Args& a, int64_t at) {
 // A share as its pieces of items, the same walk in every role.
 struct Walk {
   const Args& a;
-  int64_t per, item, tile, left;
-  int b, bh;
-  int64_t it, end, n, j0, j1;      // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
-  __device__ Walk(const Args& a_, const Place& p, int64_t count) : a(a_), per(items_per_bh(a_)), item(p.item), tile(p.tile), left(count) {}
+  int per, item, tile, left;
+  int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
+  __device__ Walk(const Args& a_, const Place& p, int count)
+      : a(a_), per((int)items_per_bh(a_)), item((int)p.item), tile((int)p.tile), left(count) {}
   __device__ bool next() {
     if (left <= 0) return false;
-    bh = (int)(item / per);
-    it = item % per;
+    bh = item / per;
+    it = item - bh * per;
     b = bh / a.Hkv;
-    end = seq_end(a, b);
-    n = tiles_of(a, end, it);
+    end = (int)seq_end(a, b);
+    n = (int)tiles_of(a, end, it);
     j0 = tile;
     j1 = min(n, j0 + left);
     left -= j1 - j0;
@@ -160,12 +160,38 @@ __device__ __forceinline__ int weight_ev(float scale, int largest) {
   return min(largest, max(largest - EV_SPAN, (int)(__float_as_uint(scale) >> 23) - 127));
 }
 
-template <int N> __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void reg_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
-
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <int N> __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+// Multiplies `n` of this thread's columns of tensor memory (fp32, or pairs of f16), 16 out of every `step`, by f.
+template <bool HALVES> __device__ __noinline__ void scale_columns(uint32_t at, int n, int step, float f) {
+#pragma unroll 1
+  for (; n > 0; n -= 16, at += step) {
+    uint32_t o[16];
+    tc::Tmem<16>::ld(at, o);
+    tc::wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if constexpr (HALVES) {
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
+        o[e] = pack_h2(p.x * f, p.y * f);
+      } else {
+        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+      }
+    }
+    tc::Tmem<16>::st(at, o);
+  }
+  tc::wait_st();
 }
 
 template <typename T, int QT>
@@ -179,20 +205,20 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
   __shared__ Place s_place;
-  __shared__ int64_t s_count;
+  __shared__ int s_count;
   __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];         // tokens whose value holds a NaN (tiles whose mask differs by row)
   const uint32_t bar = tc::smem_u32(bars);
-  auto k_full = [&](int64_t i) { return bar + 8 * (uint32_t)(i % KSTAGES); };
-  auto k_free = [&](int64_t i) { return bar + 8 * (uint32_t)(KSTAGES + i % KSTAGES); };
+  auto k_full = [&](uint32_t i) { return bar + 8 * (i % KSTAGES); };
+  auto k_free = [&](uint32_t i) { return bar + 8 * (KSTAGES + i % KSTAGES); };
   const uint32_t bar2 = bar + 16 * KSTAGES;
-  auto v_full = [&](int64_t i) { return bar2 + 8 * (uint32_t)(i % VSTAGES); };
-  auto v_free = [&](int64_t i) { return bar2 + 8 * (uint32_t)(VSTAGES + i % VSTAGES); };
+  auto v_full = [&](uint32_t i) { return bar2 + 8 * (i % VSTAGES); };
+  auto v_free = [&](uint32_t i) { return bar2 + 8 * (VSTAGES + i % VSTAGES); };
   const uint32_t bar3 = bar2 + 16 * VSTAGES;
   auto s_full = [&](int h) { return bar3 + 8 * h; };
   auto p_full = [&](int h) { return bar3 + 16 + 8 * h; };
   auto q_full = [&](int h) { return bar3 + 32 + 8 * h; };
   const uint32_t drain = bar3 + 48;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp >> 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = (int)tc::uniform(tid >> 5), group = warp >> 2;
   volatile int* gave_up = &s_gave_up;
 
   if (tid == 0) {
@@ -208,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     const int64_t total = line_length(a), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
     Place p{0, 0};
     if (first < total) p = locate(a, first);
-    if (lane == 0) s_place = p, s_count = min(share, total - first);
+    if (lane == 0) s_place = p, s_count = (int)min(share, total - first);
   }
   tc::fence_before();
   __syncthreads();
@@ -223,14 +249,13 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tm_s = tm + h2 * 128 + my, tm_o = tm + 256 + h2 * 128 + my;
     uint8_t* sq = smem + S::Q + h2 * QT * HALF * D;
-    int64_t phase = 0, vt = 0;                     // completions of s_full seen; tiles seen
+    uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
     while (w.next()) {
-      const int64_t total = a.G * a.T, row = w.it * ROWS + h2 * HALF + r;
+      const int total = a.G * (int)a.T, row = w.it * ROWS + h2 * HALF + r;
       const bool real = row < total;
-      const int64_t rr = real ? row : total - 1;
-      const int hq = (w.bh % a.Hkv) * a.G + (int)(rr % a.G);
-      const int64_t tt = rr / a.G, limit = seen(a, w.end, rr);
+      const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
+      const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
       // the row's query as e4m3 terms of its own scale
       float rs;
       {
@@ -275,78 +300,83 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full(h2));
       // keys that every row of the CTA sees need no mask
-      const int64_t all_see = seen(a, w.end, w.it * ROWS);
+      const int all_see = (int)seen(a, w.end, w.it * ROWS);
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       const int ev = largest_ev(sc, w.end);
       float m = -INFINITY, l = 0.0f;
-      for (int64_t j = w.j0; j < w.j1; ++j, ++vt) {
-        const int64_t blk = j * (TILE / BLK);
+      for (int j = w.j0; j < w.j1; ++j, ++vt) {
+        const int blk = j * (TILE / BLK);
         // above 0, so that a masked score stays -inf; void blocks may hold anything, NaN too
         const float2 sc0 = sc[blk], sc1 = blk + 1 < a.cap / BLK ? sc[blk + 1] : make_float2(0.0f, 0.0f);
         const float c0 = fmaxf(sc0.x * rs, 1e-37f), c1 = fmaxf(sc1.x * rs, 1e-37f);
         const int ev0 = weight_ev(sc0.y, ev), ev1 = weight_ev(sc1.y, ev);
+        const float e0 = (float)ev0, e1 = (float)ev1, l0 = pow2i(ev - ev0), l1 = pow2i(ev - ev1);
         ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);
         ++phase;
         __syncwarp();
         tc::fence_after();
-        uint32_t x[TILE];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tc::Tmem<32>::ld(tm_s + 32 * i, x + 32 * i);
-        tc::wait_ld();
+        int see = TILE;                            // tokens of the tile that this row sees
         if ((j + 1) * TILE > all_see) {
-          const int64_t room = limit - j * TILE;   // keys of the tile that this row sees
-          const int see = room < 0 ? 0 : room > TILE ? TILE : (int)room;
-#pragma unroll
-          for (int i = 0; i < TILE; ++i)
-            if (i >= see) x[i] = 0xFF800000u;      // -inf
+          see = min(max(limit - j * TILE, 0), TILE);
           ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
-          __syncwarp();
           for (int i = 0; i < TILE; i += 4)
             if (const uint32_t f = *reinterpret_cast<const uint32_t*>(&s_nan[vt % VSTAGES][i]))
               if (i + (__ffs(f) - 1) / 8 < see) l = __uint_as_float(0x7FFFFFFFu);
           __syncwarp();
         }
-        float m0[4], m1[4];
+        const bool masked = (j + 1) * TILE > all_see;
+        // 32 tokens at a time, the next 32 on their way, with the reference as it is, so that no exponential waits for a
+        // maximum; where a row turns out to have outgrown its reference, those 32 once more with a new one.  The
+        // weights of chunk c go over its own scores: columns 32 c .. 32 c + 15.
+        uint32_t x[2][32];
+        tc::Tmem<32>::ld(tm_s, x[0]);
+#pragma unroll 1                                  // one copy of two chunks: code that the instruction caches hold
+        for (int hf = 0; hf < 2; ++hf) {
+          const float cs = hf ? c1 : c0, es = hf ? e1 : e0, ls = hf ? l1 : l0;
+          float2 total = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m0[i] = __uint_as_float(x[i]), m1[i] = __uint_as_float(x[64 + i]);
+          for (int u = 0; u < 2; ++u) {
+            uint32_t* y = x[u];
+            const uint32_t at = tm_s + 64 * hf + 32 * u;
+            tc::wait_ld32(y);
+            if (u == 0 || hf == 0) tc::Tmem<32>::ld(at + 32, x[u ^ 1]);
+            if (masked) {
 #pragma unroll
-        for (int i = 4; i < 64; ++i) {
-          m0[i & 3] = fmaxf(m0[i & 3], __uint_as_float(x[i]));
-          m1[i & 3] = fmaxf(m1[i & 3], __uint_as_float(x[64 + i]));
-        }
-        const float t0 = fmaxf(fmaxf(m0[0], m0[1]), fmaxf(m0[2], m0[3])), t1 = fmaxf(fmaxf(m1[0], m1[1]), fmaxf(m1[2], m1[3]));
-        const float top = fmaxf(fmaf(t0, c0, (float)ev0), fmaf(t1, c1, (float)ev1));
-        const bool up = top > m + SLACK;           // also the first time: m = -inf
-        if (__any_sync(0xffffffffu, up)) {
-          const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-          if (up) m = top;
-          l *= f;
-          if (j > w.j0) {                          // O of the tiles before is complete: their products precede this S
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-              uint32_t o[32];
-              tc::Tmem<32>::ld(tm_o + 32 * i, o);
-              tc::wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tc::Tmem<32>::st(tm_o + 32 * i, o);
+              for (int i = 0; i < 32; ++i)
+                if (64 * hf + 32 * u + i >= see) y[i] = 0xFF800000u;      // -inf
             }
-          }
-        }
-        const float off = m == -INFINITY ? 0.0f : HEAD - m, off0 = off + (float)ev0, off1 = off + (float)ev1;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // of the first half's even and odd tokens, of the second's
+            uint32_t p[16];
+            float2 sum;
+            while (true) {
+              const float off = m == -INFINITY ? 0.0f : HEAD - m + es;
+              const float2 cc = make_float2(cs, cs), oo = make_float2(off, off);
+              sum = make_float2(0.0f, 0.0f);
+              float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < TILE; i += 2) {
-          const float c = i < 64 ? c0 : c1, o = i < 64 ? off0 : off1;
-          const float p0 = ex2(fmaf(__uint_as_float(x[i]), c, o)), p1 = ex2(fmaf(__uint_as_float(x[i + 1]), c, o));
-          sum[i / 64 * 2] += p0;
-          sum[i / 64 * 2 + 1] += p1;
-          x[i / 2] = pack_h2(p0, p1);
+              for (int i = 0; i < 16; ++i) {
+                const float2 s2 = make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
+                (i & 1 ? t1 : t0) = max3(i & 1 ? t1 : t0, s2.x, s2.y);
+                const float2 e2 = __ffma2_rn(s2, cc, oo);
+                const float2 w2 = make_float2(ex2(e2.x), ex2(e2.y));
+                sum = __fadd2_rn(sum, w2);
+                p[i] = pack_h2(w2.x, w2.y);
+              }
+              const float top = fmaf(max3(t0, t1, t1), cs, es);
+              const bool up = top > m + SLACK;     // also the first time: m = -inf
+              if (!__any_sync(0xffffffffu, up)) break;
+              const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+              if (up) m = top;
+              l *= f;
+              total = make_float2(total.x * f, total.y * f);
+              // O of the tiles before is complete, their products precede this S; and this tile's weights so far
+              if (j > w.j0) scale_columns<false>(tm_o, D, 16, f);
+              scale_columns<true>(tm_s, 16 * (2 * hf + u), 32, f);
+            }
+            total = __fadd2_rn(total, sum);
+            tc::Tmem<16>::st(at, p);
+          }
+          l = fmaf(total.x + total.y, ls, l);
         }
-        l = fmaf(sum[0] + sum[1], pow2i(ev - ev0), l);
-        l = fmaf(sum[2] + sum[3], pow2i(ev - ev1), l);
-        tc::Tmem<32>::st(tm_s, x);
-        tc::Tmem<32>::st(tm_s + 32, x + 32);
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
@@ -392,24 +422,24 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     // ---- values: e4m3 rows from memory to f16, MN-major tiles of two 64-dim halves.  Thread = 16 dims of 8 tokens.
     reg_less<REG_VALUE>();
     const int t = tid - 256, u = t & 7, row0 = t >> 3;
-    int64_t i = 0;
+    uint32_t i = 0;
     bool ok = true;
     while (ok && w.next()) {
       const uint8_t* base = a.rows + (int64_t)w.bh * a.cap * KV8_ROW + D + u * 16;
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       const int ev = largest_ev(sc, w.end);
-      const int64_t all_see = seen(a, w.end, w.it * ROWS);
-      for (int64_t j = w.j0; j < w.j1; ++j, ++i) {
+      const int all_see = (int)seen(a, w.end, w.it * ROWS);
+      for (int j = w.j0; j < w.j1; ++j, ++i) {
         uint4 v[8];
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-          const int64_t tok = j * TILE + p * 16 + row0;
-          v[p] = tok < w.end ? *reinterpret_cast<const uint4*>(base + tok * KV8_ROW) : make_uint4(0, 0, 0, 0);
+          const int tok = j * TILE + p * 16 + row0;
+          v[p] = tok < w.end ? *reinterpret_cast<const uint4*>(base + (int64_t)tok * KV8_ROW) : make_uint4(0, 0, 0, 0);
         }
         int rest[2];                               // log2 of what the weights leave of the block's scale
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int64_t blk = j * 2 + e;
+          const int blk = j * 2 + e;
           const float s = blk * BLK < w.end ? sc[blk].y : 1.0f;
           rest[e] = blk * BLK < w.end ? (int)(__float_as_uint(s) >> 23) - 127 - weight_ev(s, ev) : 0;
         }
@@ -463,77 +493,92 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     reg_less<REG_OTHER>();
     if (warp == 13 && lane == 0) {
       // ---- key tiles
-      int64_t i = 0;
+      uint32_t i = 0;
       bool ok = true;
       while (ok && w.next()) {
-        for (int64_t j = w.j0; j < w.j1; ++j, ++i) {
+        for (int j = w.j0; j < w.j1; ++j, ++i) {
           ok = tc::mbar_wait(k_free(i), ((i / KSTAGES) & 1) ^ 1, gave_up);
           if (!ok) break;
           tc::mbar_expect_tx(k_full(i), KBYTES);
-          tc::tma_load_3d(sbase + S::K + (uint32_t)(i % KSTAGES) * KBYTES, &map, 0, (int)(j * TILE), w.bh, k_full(i));
+          tc::tma_load_3d(sbase + S::K + (i % KSTAGES) * KBYTES, &map, 0, j * TILE, w.bh, k_full(i));
         }
       }
       if (*gave_up) {
-        for (int64_t j = i > KSTAGES ? i - KSTAGES : 0; j < i; ++j) {   // copies in flight land first
+        for (uint32_t j = i > KSTAGES ? i - KSTAGES : 0; j < i; ++j) {   // copies in flight land first
           const unsigned long long t0 = tc::now_ns();
           while (!tc::mbar_try(k_full(j), (j / KSTAGES) & 1) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
         }
       }
-    } else if (warp == 12 && lane == 0) {
-      // ---- products
+    } else if (warp == 12) {
+      // ---- products (the whole warp: elect_one)
       constexpr uint32_t id_s = tc::instr(TILE, false, false), id_o = tc::instr(D, false, true);
-      int64_t i = 0, pn = 0, seg = 0;              // key tile, weight tiles done, pieces begun
+      const uint32_t tmu = tc::uniform(tm);
+      uint32_t i = 0, pn = 0, seg = 0;             // tiles done, weight tiles done, pieces begun
+      uint32_t ks = 0, vs = 0;                     // stages of the next key tile, of the next value tile
       bool ok = true;
-      auto scores = [&](int h, int64_t i) {
-        const uint64_t dk = tc::operand(sbase + S::K + (uint32_t)(i % KSTAGES) * KBYTES);
+      // S_h of the next key tile, which is spent when h is 1
+      auto scores = [&](int h) {
+        const uint64_t dk = tc::operand(sbase + S::K + tc::uniform(ks) * KBYTES);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int term = 0; term < QT; ++term) {
-          const uint64_t dq = tc::operand(sbase + S::Q + (h * QT + term) * HALF * D);
+          for (int term = 0; term < QT; ++term) {
 #pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk)
-            tc::mma_fp8(tm + h * 128, dq + kk * 2, dk + kk * 2, id_s, term > 0 || kk > 0);
+            for (int kk = 0; kk < D / 32; ++kk)
+              tc::mma_fp8(tmu + h * 128, tc::operand(sbase + S::Q + (h * QT + term) * HALF * D) + kk * 2, dk + kk * 2, id_s,
+                          term > 0 || kk > 0);
+          }
+          if (h == 1) tc::mma_commit(bar + 8 * (KSTAGES + ks));
+          tc::mma_commit(s_full(h));
         }
+        __syncwarp();
+        if (h == 1) ks = ks + 1 == KSTAGES ? 0 : ks + 1;
       };
-      auto values = [&](int h, int64_t i, bool accumulate) {
-        const uint64_t dv = tc::operand(sbase + S::V + (uint32_t)(i % VSTAGES) * VBYTES, TILE * 128);
+      // O_h of the next value tile; the piece's last is announced as scores are
+      auto values = [&](int h, bool accumulate, bool last) {
+        const uint64_t dv = tc::operand(sbase + S::V + tc::uniform(vs) * VBYTES, TILE * 128);
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < TILE / 16; ++kk)     // 16 tokens a step: 8 columns of weights, 2 groups of 8 value rows
-          tc::mma_f16_ts(tm + 256 + h * 128, tm + h * 128 + kk * 8, dv + kk * (16 * 128 / 16), id_o, accumulate || kk > 0);
+          for (int kk = 0; kk < TILE / 16; ++kk)   // 16 tokens a step: 8 columns of weights, 2 groups of 8 value rows
+            tc::mma_f16_ts(tmu + 256 + h * 128, tmu + h * 128 + kk / 2 * 32 + kk % 2 * 8, dv + kk * (16 * 128 / 16), id_o,
+                           accumulate || kk > 0);
+          if (h == 1) tc::mma_commit(bar2 + 8 * (VSTAGES + vs));
+          if (last) tc::mma_commit(s_full(h));
+        }
+        __syncwarp();
+        if (h == 1) vs = vs + 1 == VSTAGES ? 0 : vs + 1;
       };
       while (ok && w.next()) {
-        const int64_t n = w.j1 - w.j0;
+        const int n = w.j1 - w.j0;
         for (int h = 0; h < 2; ++h) ok = ok && tc::mbar_wait(q_full(h), seg & 1, gave_up);
         ++seg;
         ok = ok && tc::mbar_wait(k_full(i), (i / KSTAGES) & 1, gave_up);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::fence_after();
-        for (int h = 0; h < 2; ++h) {
-          scores(h, i);
-          tc::mma_commit(s_full(h));
-        }
-        tc::mma_commit(k_free(i));
-        for (int64_t j = 1; j <= n && ok; ++j) {
-          const int64_t v = i + j - 1;
+        scores(0);
+        scores(1);
+        for (int j = 1; j <= n; ++j) {
+          const uint32_t v = i + j - 1;
           const bool last = j == n;
-          if (!last) ok = tc::mbar_wait(k_full(i + j), ((i + j) / KSTAGES) & 1, gave_up);
+          ok = last || tc::mbar_wait(k_full(i + j), ((i + j) / KSTAGES) & 1, gave_up);
           ok = ok && tc::mbar_wait(v_full(v), (v / VSTAGES) & 1, gave_up);
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = tc::mbar_wait(p_full(h), pn & 1, gave_up);
-            if (!ok) break;
-            tc::fence_after();
-            values(h, v, j > 1);
-            if (h == 1) tc::mma_commit(v_free(v));
-            if (!last) {
-              scores(h, i + j);
-              if (h == 1) tc::mma_commit(k_free(i + j));
-            }
-            tc::mma_commit(s_full(h));             // the next scores, or the piece's last product
-          }
+          ok = ok && tc::mbar_wait(p_full(0), pn & 1, gave_up);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc::fence_after();
+          values(0, j > 1, last);
+          if (!last) scores(0);
+          ok = tc::mbar_wait(p_full(1), pn & 1, gave_up);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc::fence_after();
+          values(1, j > 1, last);
+          if (!last) scores(1);
           ++pn;
         }
         i += n;
       }
-      if (*gave_up) {
+      if (*gave_up && tc::elect_one()) {
         tc::mma_commit(drain);
         const unsigned long long t0 = tc::now_ns();
         while (!tc::mbar_try(drain, 0) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}

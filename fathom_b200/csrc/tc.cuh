@@ -49,6 +49,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t mb, uint32_t parity, volatile
   return true;
 }
 
+// One lane of a converged warp, the same one every time.  Code that issues tensor-core work runs in the whole warp and
+// only the instructions themselves in this lane: their operands then stay in uniform registers (moved there one by
+// one, they cost more issue time than the products take).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }\n" : "=r"(r));
+  return r != 0;
+}
+// A value that is the same in the whole warp, as the compiler can see.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // ---- proxies -------------------------------------------------------------------------------------
 // Orders this thread's shared-memory writes before later reads by the tensor cores and TMA.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
@@ -86,6 +97,17 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {       
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+// The same, naming the registers of the loads so that none of their uses is moved before it.
+__device__ __forceinline__ void wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
 // Shared-memory operand in the 128-byte swizzle, rows (K-major) or K slices (MN-major) of 128 bytes in groups of
