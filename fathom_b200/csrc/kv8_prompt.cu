@@ -33,12 +33,13 @@ constexpr int TILE = 128;                    // tokens per tile
 constexpr int HALF = 128, ROWS = 2 * HALF;   // query rows of a warpgroup, of a CTA
 constexpr int KSTAGES = 3, VSTAGES = 2;
 constexpr int KBYTES = TILE * D, VBYTES = 2 * TILE * D;
-constexpr int THREADS = 512;                 // warps 0-3, 4-7: softmax; 8-11: values; 12: products; 13: key loads
+constexpr int SOFT = 256;                    // softmax threads of a half: two per row, one for each 64-token block of a tile
+constexpr int THREADS = 2 * SOFT + 256;      // warps 0-7, 8-15: softmax; 16-19: values; 20: products; 21: key loads
 constexpr float SLACK = 7.0f;                // a row may exceed its reference by 2^7
 constexpr float HEAD = 8.0f;                 // weights at the reference are 2^8
-// registers per thread of the softmax, value and other warpgroups: together the 512 * 128 of the launch
-constexpr int REG_SOFT = 168, REG_VALUE = 88, REG_OTHER = 88;
-static_assert(2 * REG_SOFT + REG_VALUE + REG_OTHER == 4 * 128, "register split");
+// registers per thread of the softmax, value and other warps: together no more than the 768 * 80 of the launch
+constexpr int REG_LAUNCH = 80, REG_SOFT = 88, REG_VALUE = 64, REG_OTHER = 64;
+static_assert(4 * REG_SOFT + REG_VALUE + REG_OTHER <= 6 * REG_LAUNCH, "register split");
 constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
 
 template <int QT> struct Shape {
@@ -173,27 +174,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 template <int N> __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
 
-// Multiplies `n` of this thread's columns of tensor memory (fp32, or pairs of f16), 16 out of every `step`, by f.
-template <bool HALVES> __device__ __noinline__ void scale_columns(uint32_t at, int n, int step, float f) {
-#pragma unroll 1
-  for (; n > 0; n -= 16, at += step) {
-    uint32_t o[16];
-    tc::Tmem<16>::ld(at, o);
-    tc::wait_ld();
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if constexpr (HALVES) {
-        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&o[e]));
-        o[e] = pack_h2(p.x * f, p.y * f);
-      } else {
-        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-      }
-    }
-    tc::Tmem<16>::st(at, o);
-  }
-  tc::wait_st();
-}
-
 template <typename T, int QT>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constant__ CUtensorMap map,
                                                            const __grid_constant__ Args a) {
@@ -207,6 +187,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __shared__ Place s_place;
   __shared__ int s_count;
   __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];         // tokens whose value holds a NaN (tiles whose mask differs by row)
+  __shared__ float s_pair[2][2][HALF];             // what the two threads of a row tell each other
   const uint32_t bar = tc::smem_u32(bars);
   auto k_full = [&](uint32_t i) { return bar + 8 * (i % KSTAGES); };
   auto k_free = [&](uint32_t i) { return bar + 8 * (KSTAGES + i % KSTAGES); };
@@ -224,12 +205,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   if (tid == 0) {
     for (int i = 0; i < KSTAGES; ++i) tc::mbar_init(k_full(i), 1), tc::mbar_init(k_free(i), 1);
     for (int i = 0; i < VSTAGES; ++i) tc::mbar_init(v_full(i), 4), tc::mbar_init(v_free(i), 1);
-    for (int h = 0; h < 2; ++h) tc::mbar_init(s_full(h), 1), tc::mbar_init(p_full(h), 4), tc::mbar_init(q_full(h), 4);
+    for (int h = 0; h < 2; ++h) tc::mbar_init(s_full(h), 1), tc::mbar_init(p_full(h), SOFT / 32), tc::mbar_init(q_full(h), SOFT / 32);
     tc::mbar_init(drain, 1);
     tc::fence_mbar_init();
     s_gave_up = 0;
   }
-  if (warp == 12) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
+  if (warp == 20) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
   if (warp == 0) {
     const int64_t total = line_length(a), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
     Place p{0, 0};
@@ -242,13 +223,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   const uint32_t tm = s_tmem;                      // S_0, S_1, O_0, O_1: 128 columns each
   Walk w(a, s_place, s_count);
 
-  if (group < 2) {
-    // ---- softmax of half `group`: thread = row
+  if (group < 4) {
+    // ---- softmax of half h2: two threads per row, thread `ch` for the tile's 64-token block ch and dims 64 ch ..
     reg_more<REG_SOFT>();
-    const int h2 = group, r = tid & (HALF - 1);
+    const int h2 = group >> 1, ch = group & 1, r = tid & (HALF - 1);
+    const int pair_bar = 1 + h2 * 4 + (warp & 3);  // the two warps of 32 rows
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tm_s = tm + h2 * 128 + my, tm_o = tm + 256 + h2 * 128 + my;
-    uint8_t* sq = smem + S::Q + h2 * QT * HALF * D;
+    const uint32_t tm_s = tm + h2 * 128 + 64 * ch + my, tm_o = tm + 256 + h2 * 128 + 64 * ch + my;
+    uint8_t* sq = smem + S::Q + h2 * QT * HALF * D + r * D;
+    float *s_mine = &s_pair[h2][ch][r], *s_other = &s_pair[h2][ch ^ 1][r];
     uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
     while (w.next()) {
@@ -256,24 +239,27 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
-      // the row's query as e4m3 terms of its own scale
+      // the row's query as e4m3 terms of its own scale: this thread's 64 dims
       float rs;
       {
-        const T* qp = reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt;
-        uint4 v[16];
+        const T* qp = reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt + 64 * ch;
+        uint4 v[8];
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 8; ++i) {
           v[i] = *reinterpret_cast<const uint4*>(qp + 8 * i);
           const T* e = reinterpret_cast<const T*>(&v[i]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f32(e[j])) & 0x7FFFFFFFu);
         }
+        *s_mine = __uint_as_float(top);
+        tc::named_sync(pair_bar, 64);
+        top = max(top, __float_as_uint(*s_other));
         const int e2 = kv8_exponent(top);
         const float inv = pow2i(-e2);
         rs = pow2i(e2) * QSCALE;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4; ++c) {
           float x[16];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -290,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
               const float2 lo = kv8_decode2(code[i]), hi = kv8_decode2(code[i] >> 16);
               x[4 * i] -= lo.x, x[4 * i + 1] -= lo.y, x[4 * i + 2] -= hi.x, x[4 * i + 3] -= hi.y;
             }
-            *reinterpret_cast<uint4*>(sq + term * HALF * D + r * D + ((c ^ (r & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(sq + term * HALF * D + (((4 * ch + c) ^ (r & 7)) << 4)) =
                 make_uint4(code[0], code[1], code[2], code[3]);
           }
         }
@@ -303,80 +289,95 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       const int all_see = (int)seen(a, w.end, w.it * ROWS);
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       const int ev = largest_ev(sc, w.end);
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f;               // m is the same in both threads of a row, l is this thread's share
       for (int j = w.j0; j < w.j1; ++j, ++vt) {
-        const int blk = j * (TILE / BLK);
+        const int blk = j * (TILE / BLK) + ch;
+        const float2 s2 = blk < a.cap / BLK ? sc[blk] : make_float2(0.0f, 0.0f);
         // above 0, so that a masked score stays -inf; void blocks may hold anything, NaN too
-        const float2 sc0 = sc[blk], sc1 = blk + 1 < a.cap / BLK ? sc[blk + 1] : make_float2(0.0f, 0.0f);
-        const float c0 = fmaxf(sc0.x * rs, 1e-37f), c1 = fmaxf(sc1.x * rs, 1e-37f);
-        const int ev0 = weight_ev(sc0.y, ev), ev1 = weight_ev(sc1.y, ev);
-        const float e0 = (float)ev0, e1 = (float)ev1, l0 = pow2i(ev - ev0), l1 = pow2i(ev - ev1);
+        const float cs = fmaxf(s2.x * rs, 1e-37f);
+        const int evb = weight_ev(s2.y, ev);
+        const float es = (float)evb;
         ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);
         ++phase;
         __syncwarp();
         tc::fence_after();
-        int see = TILE;                            // tokens of the tile that this row sees
-        if ((j + 1) * TILE > all_see) {
-          see = min(max(limit - j * TILE, 0), TILE);
+        int see = BLK;                             // tokens of the block that this row sees
+        const bool masked = (j + 1) * TILE > all_see;
+        if (masked) {
+          see = min(max(limit - blk * BLK, 0), BLK);
           ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
-          for (int i = 0; i < TILE; i += 4)
-            if (const uint32_t f = *reinterpret_cast<const uint32_t*>(&s_nan[vt % VSTAGES][i]))
+          for (int i = 0; i < BLK; i += 4)
+            if (const uint32_t f = *reinterpret_cast<const uint32_t*>(&s_nan[vt % VSTAGES][ch * BLK + i]))
               if (i + (__ffs(f) - 1) / 8 < see) l = __uint_as_float(0x7FFFFFFFu);
           __syncwarp();
         }
-        const bool masked = (j + 1) * TILE > all_see;
-        // 32 tokens at a time, the next 32 on their way, with the reference as it is, so that no exponential waits for a
-        // maximum; where a row turns out to have outgrown its reference, those 32 once more with a new one.  The
-        // weights of chunk c go over its own scores: columns 32 c .. 32 c + 15.
-        uint32_t x[2][32];
-        tc::Tmem<32>::ld(tm_s, x[0]);
-#pragma unroll 1                                  // one copy of two chunks: code that the instruction caches hold
-        for (int hf = 0; hf < 2; ++hf) {
-          const float cs = hf ? c1 : c0, es = hf ? e1 : e0, ls = hf ? l1 : l0;
-          float2 total = make_float2(0.0f, 0.0f);
+        uint32_t x[32];
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t* y = x[u];
-            const uint32_t at = tm_s + 64 * hf + 32 * u;
-            tc::wait_ld32(y);
-            if (u == 0 || hf == 0) tc::Tmem<32>::ld(at + 32, x[u ^ 1]);
+        for (int u = 0; u < 2; ++u) {
+          tc::Tmem<32>::ld(tm_s + 32 * u, x);
+          tc::wait_ld32(x);
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * u + i >= see) x[i] = 0xFF800000u;                  // -inf
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            t0 = max3(t0, __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+            t1 = max3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+          }
+        }
+        float top = fmaf(fmaxf(t0, t1), cs, es);
+        if (tc::named_or(pair_bar, 64, top > m + SLACK)) {        // also the first time: m = -inf
+          *s_mine = top;
+          tc::named_sync(pair_bar, 64);
+          top = fmaxf(top, *s_other);
+          tc::named_sync(pair_bar, 64);
+          const bool up = top > m + SLACK;
+          const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+          if (up) m = top;
+          l *= f;
+          __syncwarp();
+          if (j > w.j0) {                          // O of the tiles before is complete: their products precede this S
+#pragma unroll 1
+            for (int i = 0; i < 64; i += 16) {
+              uint32_t o[16];
+              tc::Tmem<16>::ld(tm_o + i, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc::Tmem<16>::st(tm_o + i, o);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : HEAD - m + es;
+        const float2 cc = make_float2(cs, cs), oo = make_float2(off, off);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        // weights over the scores they came from: columns 32 u .. 32 u + 15 of the block's 64
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int u = v ^ 1;                     // the second 32 are still in registers
+          if (v == 1) {
+            tc::Tmem<32>::ld(tm_s + 32 * u, x);
+            tc::wait_ld32(x);
             if (masked) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (64 * hf + 32 * u + i >= see) y[i] = 0xFF800000u;      // -inf
+                if (32 * u + i >= see) x[i] = 0xFF800000u;
             }
-            uint32_t p[16];
-            float2 sum;
-            while (true) {
-              const float off = m == -INFINITY ? 0.0f : HEAD - m + es;
-              const float2 cc = make_float2(cs, cs), oo = make_float2(off, off);
-              sum = make_float2(0.0f, 0.0f);
-              float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 s2 = make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
-                (i & 1 ? t1 : t0) = max3(i & 1 ? t1 : t0, s2.x, s2.y);
-                const float2 e2 = __ffma2_rn(s2, cc, oo);
-                const float2 w2 = make_float2(ex2(e2.x), ex2(e2.y));
-                sum = __fadd2_rn(sum, w2);
-                p[i] = pack_h2(w2.x, w2.y);
-              }
-              const float top = fmaf(max3(t0, t1, t1), cs, es);
-              const bool up = top > m + SLACK;     // also the first time: m = -inf
-              if (!__any_sync(0xffffffffu, up)) break;
-              const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-              if (up) m = top;
-              l *= f;
-              total = make_float2(total.x * f, total.y * f);
-              // O of the tiles before is complete, their products precede this S; and this tile's weights so far
-              if (j > w.j0) scale_columns<false>(tm_o, D, 16, f);
-              scale_columns<true>(tm_s, 16 * (2 * hf + u), 32, f);
-            }
-            total = __fadd2_rn(total, sum);
-            tc::Tmem<16>::st(at, p);
           }
-          l = fmaf(total.x + total.y, ls, l);
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 e2 = __ffma2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), cc, oo);
+            const float2 w2 = make_float2(ex2(e2.x), ex2(e2.y));
+            sum[i & 1] = __fadd2_rn(sum[i & 1], w2);
+            p[i] = pack_h2(w2.x, w2.y);
+          }
+          tc::Tmem<16>::st(tm_s + 32 * u, p);
         }
+        l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2i(ev - evb), l);
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
@@ -384,44 +385,46 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       }
       ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);      // the piece's last product
       ++phase;
-      __syncwarp();
+      *s_mine = l;
+      tc::named_sync(pair_bar, 64);
+      l += *s_other;
       tc::fence_after();
       const bool whole = w.j0 == 0 && w.j1 == w.n;
       const float vscale = pow2i(ev);              // the denominator is relative to the largest scale
       const float f = !ok ? __uint_as_float(0x7FFFFFFFu) : whole ? (l == 0.0f ? 0.0f : vscale / l) : vscale;
-      T* op = reinterpret_cast<T*>(a.out) + w.b * a.ob + hq * a.oh + tt * a.ot;
+      T* op = reinterpret_cast<T*>(a.out) + w.b * a.ob + hq * a.oh + tt * a.ot + 64 * ch;
       float* part = a.part + ((2 * (int64_t)blockIdx.x + (w.j0 == 0 ? 1 : 0)) * ROWS + h2 * HALF + r) * PART;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        uint32_t o[32];
+      for (int i = 0; i < 64; i += 16) {
+        uint32_t o[16];
         __syncwarp();
-        tc::Tmem<32>::ld(tm_o + 32 * i, o);
+        tc::Tmem<16>::ld(tm_o + i, o);
         tc::wait_ld();
         if (!real) continue;
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             T y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) from_f32(l == 0.0f ? 0.0f : __uint_as_float(o[8 * c + e]) * f, &y[e]);
-            *reinterpret_cast<uint4*>(op + 32 * i + 8 * c) = *reinterpret_cast<const uint4*>(y);
+            *reinterpret_cast<uint4*>(op + i + 8 * c) = *reinterpret_cast<const uint4*>(y);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(part + 32 * i + 4 * c) =
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<float4*>(part + 64 * ch + i + 4 * c) =
                 make_float4(__uint_as_float(o[4 * c]) * f, __uint_as_float(o[4 * c + 1]) * f,
                             __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
         }
       }
-      if (real && !whole) part[D] = m, part[D + 1] = l;
+      if (real && !whole && ch == 0) part[D] = m, part[D + 1] = l;
       __syncwarp();
       tc::fence_before();
     }
-  } else if (group == 2) {
+  } else if (group == 4) {
     // ---- values: e4m3 rows from memory to f16, MN-major tiles of two 64-dim halves.  Thread = 16 dims of 8 tokens.
     reg_less<REG_VALUE>();
-    const int t = tid - 256, u = t & 7, row0 = t >> 3;
+    const int t = tid - 2 * SOFT, u = t & 7, row0 = t >> 3;
     uint32_t i = 0;
     bool ok = true;
     while (ok && w.next()) {
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     }
   } else {
     reg_less<REG_OTHER>();
-    if (warp == 13 && lane == 0) {
+    if (warp == 21 && lane == 0) {
       // ---- key tiles
       uint32_t i = 0;
       bool ok = true;
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
           while (!tc::mbar_try(k_full(j), (j / KSTAGES) & 1) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
         }
       }
-    } else if (warp == 12) {
+    } else if (warp == 20) {
       // ---- products (the whole warp: elect_one)
       constexpr uint32_t id_s = tc::instr(TILE, false, false), id_o = tc::instr(D, false, true);
       const uint32_t tmu = tc::uniform(tm);
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (warp == 12) tc::tmem_free(tm, 512);
+  if (warp == 20) tc::tmem_free(tm, 512);
   if (tid == 0 && s_gave_up) atomicAdd(a.timeouts, 1ull);
 }
 
