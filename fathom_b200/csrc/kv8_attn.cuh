@@ -27,10 +27,10 @@ struct Args {
 };
 
 // Tokens of sequence b that exist.
-__device__ __forceinline__ int64_t seq_end(const Args& a, int b) {
+__device__ __forceinline__ int seq_end(const Args& a, int b) {
   int64_t e = a.end_dev ? a.end_dev[b] : a.end;
   e = e > a.cap ? a.cap : e;
-  return e > 0 ? e : 0;
+  return e > 0 ? (int)e : 0;
 }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -50,7 +50,7 @@ __device__ __forceinline__ float ex2(float x) {
 int sm_count();
 
 // kv8_token.cu: up to TOKEN_ROWS query rows (G * T) per KV head.
-constexpr int TOKEN_ROWS = 32;
+constexpr int TOKEN_ROWS = 16;
 size_t token_workspace(int64_t BH, int64_t R);
 int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
 // kv8_prompt.cu: any number of query rows, 256 at a time.

@@ -1,0 +1,153 @@
+// The work of the attention kernels over the whole 8-bit cache as a line of tiles, cut into equal shares.
+//
+// An item is up to 256 query rows (token-major pairs of token and head) of one cache row bh; its tiles are the 128-token
+// stretches up to the last key that any of its rows sees.  Items follow each other by bh, then by row; CTA c of C
+// takes tiles [c * share, (c + 1) * share) of the line, share = ceil(tiles / C), whatever the lengths are.
+#pragma once
+#include "kv8_attn.cuh"
+
+namespace fathom {
+namespace kv8 {
+
+constexpr int TILE = 128;                    // tokens per tile
+constexpr int ROWS = 256;                    // query rows per item
+
+__device__ __forceinline__ int rows_of(const Args& a) { return a.G * (int)a.T; }
+__device__ __forceinline__ int items_per_bh(const Args& a) { return (rows_of(a) - 1) / ROWS + 1; }
+
+// Keys that row `row` (token-major) of a sequence with `end` tokens sees.
+__device__ __forceinline__ int seen(const Args& a, int end, int row) { return end - ((int)a.T - 1) + row / a.G; }
+
+// Tiles of item `it` of a row bh: up to its last row's last key, one at least.
+__device__ __forceinline__ int tiles_of(const Args& a, int end, int it) {
+  const int last = min((int64_t)(it + 1) * ROWS, (int64_t)rows_of(a)) - 1;
+  return max(1, (seen(a, end, last) + TILE - 1) / TILE);
+}
+
+// One warp: sum of f over [0, n); if at >= 0, also the first i whose running sum exceeds at (and the sum before it).
+template <typename F> __device__ __forceinline__ int64_t warp_line(int n, int64_t at, int* where, int64_t* before, F f) {
+  const int lane = threadIdx.x & 31;
+  int64_t total = 0;
+  bool found = at < 0;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int64_t mine = i0 + lane < n ? f(i0 + lane) : 0;
+    int64_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (!found) {
+      const unsigned hit = __ballot_sync(0xffffffffu, total + x > at);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        *where = i0 + l;
+        *before = total + __shfl_sync(0xffffffffu, x - mine, l);
+        found = true;
+      }
+    }
+    total += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return total;
+}
+
+// One warp: tiles of the items of one bh of a sequence with `end` tokens; with at >= 0 also the item that holds tile `at`.
+__device__ __forceinline__ int64_t bh_line(const Args& a, int end, int64_t at, int* it, int64_t* before) {
+  const int per = items_per_bh(a);
+  if (per == 1) {
+    *it = 0, *before = 0;
+    return tiles_of(a, end, 0);
+  }
+  return warp_line(per, at, it, before, [&](int i) { return (int64_t)tiles_of(a, end, i); });
+}
+
+struct Place {
+  int item;      // bh * items_per_bh + it
+  int tile;      // tile within the item
+};
+
+// One warp: tiles of all items, and the place of tile `at` of the line (if at >= 0 and the line is longer).
+__device__ inline int64_t line(const Args& a, int64_t at, Place* place) {
+  const int per = items_per_bh(a);
+  int it = 0, b = 0;
+  int64_t before = 0, total = 0, one = 0;
+  if (!a.end_dev) {
+    one = bh_line(a, seq_end(a, 0), -1, &it, &before);
+    total = one * a.Hkv * a.B;
+    if (at < 0 || at >= total) return total;
+    b = (int)(at / (one * a.Hkv));
+    at -= b * one * a.Hkv;
+  } else if (per == 1) {
+    total = warp_line(a.B, at, &b, &before, [&](int i) { return (int64_t)tiles_of(a, seq_end(a, i), 0) * a.Hkv; });
+    if (at < 0 || at >= total) return total;
+    at -= before;
+  } else {
+    int64_t left = at;
+    bool found = false;
+    for (int i = 0; i < a.B; ++i) {
+      const int64_t n = bh_line(a, seq_end(a, i), -1, &it, &before);
+      if (!found && at >= 0 && left < n * a.Hkv) found = true, b = i, at = left;
+      left -= n * a.Hkv;
+      total += n * a.Hkv;
+    }
+    if (!found) return total;
+  }
+  const int end = seq_end(a, b);
+  one = bh_line(a, end, -1, &it, &before);
+  const int h = (int)(at / one);
+  at -= h * one;
+  bh_line(a, end, at, &it, &before);
+  *place = Place{(b * a.Hkv + h) * per + it, (int)(at - before)};
+  return total;
+}
+
+// One warp: where this CTA's share begins, and how many tiles it has (0 or less: none).
+__device__ inline Place my_share(const Args& a, int* count) {
+  Place p{0, 0};
+  const int64_t total = line(a, -1, &p), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
+  *count = (int)min(share, total - first);
+  if (*count > 0) line(a, first, &p);
+  return p;
+}
+
+// A share as its pieces of items, the same walk in every role.
+struct Walk {
+  const Args& a;
+  int per, item, tile, left;
+  int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
+  __device__ Walk(const Args& a_, const Place& p, int count)
+      : a(a_), per(items_per_bh(a_)), item(p.item), tile(p.tile), left(count) {}
+  __device__ bool next() {
+    if (left <= 0) return false;
+    bh = item / per;
+    it = item - bh * per;
+    b = bh / a.Hkv;
+    end = seq_end(a, b);
+    n = tiles_of(a, end, it);
+    j0 = tile;
+    j1 = min(n, j0 + left);
+    left -= j1 - j0;
+    ++item;
+    tile = 0;
+    return true;
+  }
+};
+
+// Launches the kernel that joins the parts of cut items; it may start while the kernel before still runs, and waits for it.
+template <typename K> int launch_join(K kernel, dim3 grid, int threads, const Args& a, int ctas, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, ctas);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  return check_launch("kv8_attend");
+}
+
+}  // namespace kv8
+}  // namespace fathom

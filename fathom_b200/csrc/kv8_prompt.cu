@@ -22,15 +22,14 @@
 // Work: the tiles of all (bh, 256 rows) items in a line, cut into equal contiguous shares, one per CTA; an item cut
 // by a share's end leaves parts in the workspace, which a second kernel joins in a fixed order.
 #include "kv8.cuh"
-#include "kv8_attn.cuh"
+#include "kv8_line.cuh"
 #include "tc.cuh"
 
 namespace fathom {
 namespace kv8 {
 namespace {
 
-constexpr int TILE = 128;                    // tokens per tile
-constexpr int HALF = 128, ROWS = 2 * HALF;   // query rows of a warpgroup, of a CTA
+constexpr int HALF = ROWS / 2;               // query rows that share an accumulator
 constexpr int KSTAGES = 3, VSTAGES = 2;
 constexpr int KBYTES = TILE * D, VBYTES = 2 * TILE * D;
 constexpr int SOFT = 256;                    // softmax threads of a half: two per row, one for each 64-token block of a tile
@@ -45,107 +44,6 @@ constexpr int EV_SPAN = 40;                  // value scales in the weights' exp
 template <int QT> struct Shape {
   static constexpr int Q = 0, K = 2 * QT * HALF * D, V = K + KSTAGES * KBYTES, END = V + VSTAGES * VBYTES;
   static constexpr int SMEM = END + 1024;
-};
-
-__device__ __forceinline__ int64_t items_per_bh(const Args& a) { return (a.G * a.T + ROWS - 1) / ROWS; }
-
-// Keys that row `row` (token-major) of a sequence with `end` tokens sees.
-__device__ __forceinline__ int64_t seen(const Args& a, int64_t end, int64_t row) { return end - (a.T - 1) + row / a.G; }
-
-// Tiles of item `it` of a row bh: up to its last row's last key, one at least.
-__device__ __forceinline__ int64_t tiles_of(const Args& a, int64_t end, int64_t it) {
-  const int64_t last = min((it + 1) * ROWS, a.G * a.T) - 1;
-  const int64_t n = (seen(a, end, last) + TILE - 1) / TILE;
-  return n > 1 ? n : 1;
-}
-
-// One warp: sum of f over [0, n); if at >= 0, also the first i whose running sum exceeds at (and the sum before it).
-template <typename F> __device__ int64_t warp_line(int64_t n, int64_t at, int64_t* where, int64_t* before, F f) {
-  const int lane = threadIdx.x & 31;
-  int64_t total = 0;
-  bool found = at < 0;
-  for (int64_t i0 = 0; i0 < n; i0 += 32) {
-    const int64_t mine = i0 + lane < n ? f(i0 + lane) : 0;
-    int64_t x = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (!found) {
-      const unsigned hit = __ballot_sync(0xffffffffu, total + x > at);
-      if (hit) {
-        const int l = __ffs(hit) - 1;
-        *where = i0 + l;
-        *before = total + __shfl_sync(0xffffffffu, x - mine, l);
-        found = true;
-      }
-    }
-    total += __shfl_sync(0xffffffffu, x, 31);
-  }
-  return total;
-}
-
-struct Place {
-  int64_t item;      // bh * items_per_bh + it
-  int64_t tile;      // tile within the item
-};
-
-// One warp: tiles of all items.
-__device__ int64_t line_length(const Args& a) {
-  int64_t w, s;
-  const int64_t per = items_per_bh(a);
-  if (!a.end_dev) {
-    const int64_t end = seq_end(a, 0);
-    return warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); }) * a.B * a.Hkv;
-  }
-  int64_t total = 0;
-  for (int b = 0; b < a.B; ++b) {
-    const int64_t end = seq_end(a, b);
-    total += warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); }) * a.Hkv;
-  }
-  return total;
-}
-
-// One warp: the item that holds tile `at` of the line (at < its length).
-__device__ Place locate(const Args& a, int64_t at) {
-  int64_t w = 0, s = 0;
-  const int64_t per = items_per_bh(a);
-  int b = 0;
-  int64_t one = 0;
-  for (;; ++b) {
-    const int64_t end = seq_end(a, b);
-    if (b == 0 || a.end_dev) one = warp_line(per, -1, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); });
-    if (at < one * a.Hkv || b + 1 == a.B) break;
-    at -= one * a.Hkv;
-  }
-  const int64_t h = at / one, end = seq_end(a, b);
-  at -= h * one;
-  warp_line(per, at, &w, &s, [&](int64_t it) { return tiles_of(a, end, it); });
-  return Place{((int64_t)b * a.Hkv + h) * per + w, at - s};
-}
-
-// A share as its pieces of items, the same walk in every role.
-struct Walk {
-  const Args& a;
-  int per, item, tile, left;
-  int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
-  __device__ Walk(const Args& a_, const Place& p, int count)
-      : a(a_), per((int)items_per_bh(a_)), item((int)p.item), tile((int)p.tile), left(count) {}
-  __device__ bool next() {
-    if (left <= 0) return false;
-    bh = item / per;
-    it = item - bh * per;
-    b = bh / a.Hkv;
-    end = (int)seq_end(a, b);
-    n = (int)tiles_of(a, end, it);
-    j0 = tile;
-    j1 = min(n, j0 + left);
-    left -= j1 - j0;
-    ++item;
-    tile = 0;
-    return true;
-  }
 };
 
 // One warp: log2 of the largest value scale among the first `end` tokens' blocks.
@@ -184,8 +82,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __shared__ __align__(8) uint64_t bars[2 * KSTAGES + 2 * VSTAGES + 7];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
-  __shared__ Place s_place;
-  __shared__ int s_count;
   __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];         // tokens whose value holds a NaN (tiles whose mask differs by row)
   __shared__ float s_pair[2][2][HALF];             // what the two threads of a row tell each other
   const uint32_t bar = tc::smem_u32(bars);
@@ -211,17 +107,14 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     s_gave_up = 0;
   }
   if (warp == 20) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
-  if (warp == 0) {
-    const int64_t total = line_length(a), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
-    Place p{0, 0};
-    if (first < total) p = locate(a, first);
-    if (lane == 0) s_place = p, s_count = (int)min(share, total - first);
-  }
+  int count;
+  const Place place = my_share(a, &count);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  tc::launch_dependents();
   const uint32_t tm = s_tmem;                      // S_0, S_1, O_0, O_1: 128 columns each
-  Walk w(a, s_place, s_count);
+  Walk w(a, place, count);
 
   if (group < 4) {
     // ---- softmax of half h2: two threads per row, thread `ch` for the tile's 64-token block ch and dims 64 ch ..
@@ -235,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
     while (w.next()) {
-      const int total = a.G * (int)a.T, row = w.it * ROWS + h2 * HALF + r;
+      const int total = rows_of(a), row = w.it * ROWS + h2 * HALF + r;
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
@@ -286,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full(h2));
       // keys that every row of the CTA sees need no mask
-      const int all_see = (int)seen(a, w.end, w.it * ROWS);
+      const int all_see = seen(a, w.end, w.it * ROWS);
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       const int ev = largest_ev(sc, w.end);
       float m = -INFINITY, l = 0.0f;               // m is the same in both threads of a row, l is this thread's share
@@ -431,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       const uint8_t* base = a.rows + (int64_t)w.bh * a.cap * KV8_ROW + D + u * 16;
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       const int ev = largest_ev(sc, w.end);
-      const int all_see = (int)seen(a, w.end, w.it * ROWS);
+      const int all_see = seen(a, w.end, w.it * ROWS);
       for (int j = w.j0; j < w.j1; ++j, ++i) {
         uint4 v[8];
 #pragma unroll
@@ -601,34 +494,30 @@ constexpr int JOIN_WARPS = 8;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args a, int ctas) {
   __shared__ Place s_place;
-  __shared__ int64_t s_total, s_n;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t per = items_per_bh(a);
+  __shared__ int64_t s_total;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = items_per_bh(a);
   if (warp == 0) {
-    const int64_t total = line_length(a), share = (total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
     Place p{0, 0};
-    int64_t n = 0;
-    if (cut < total) {
-      p = locate(a, cut);
-      n = tiles_of(a, seq_end(a, (int)(p.item / per / a.Hkv)), p.item % per);
-    }
-    if (lane == 0) s_place = p, s_total = total, s_n = n;
+    const int64_t total = line(a, -1, &p), share = (total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
+    if (cut < total) line(a, cut, &p);
+    if (lane == 0) s_place = p, s_total = total;
   }
   __syncthreads();
   const Place p = s_place;
   const int64_t share = (s_total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
-  if (p.tile == 0 || p.tile > share) return;       // no item is cut here, or an earlier cut joins it
+  tc::wait_dependency();                           // the parts are written; and nothing ends before they are
+  if (cut >= s_total || p.tile == 0 || p.tile > share) return;    // no item is cut here, or an earlier cut joins it
+  const int bh = p.item / per, it = p.item % per, b = bh / a.Hkv, total = rows_of(a);
   const int64_t first = cut - p.tile;              // the item's first tile in the line
-  const int64_t c0 = blockIdx.x, c1 = (first + s_n - 1) / share;
-  const int64_t bh = p.item / per, it = p.item % per, total = a.G * a.T;
-  const int64_t r = (int64_t)blockIdx.y * JOIN_WARPS + warp, row = it * ROWS + r;
+  const int c0 = blockIdx.x, c1 = (int)((first + tiles_of(a, seq_end(a, b), it) - 1) / share);
+  const int r = blockIdx.y * JOIN_WARPS + warp, row = it * ROWS + r;
   if (row >= total) return;
   // parts: share c0 holds the item's first tiles (its second slot), the others begin with it (first slot)
-  auto part = [&](int64_t c) { return a.part + ((2 * c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
+  auto part = [&](int c) { return a.part + ((2 * (int64_t)c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
   float M = -INFINITY, L = 0.0f;
   float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int64_t c = c0; c <= c1; ++c) M = fmaxf(M, part(c)[D]);
-  for (int64_t c = c0; c <= c1; ++c) {
+  for (int c = c0; c <= c1; ++c) M = fmaxf(M, part(c)[D]);
+  for (int c = c0; c <= c1; ++c) {
     const float m = part(c)[D], e = m == -INFINITY ? 0.0f : exp2f(m - M);
     const float4 o = *reinterpret_cast<const float4*>(part(c) + 4 * lane);
     L = fmaf(part(c)[D + 1], e, L);
@@ -637,7 +526,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args
   const float f = L == 0.0f ? 0.0f : 1.0f / L;
   T y[4];
   from_f32(O.x * f, &y[0]), from_f32(O.y * f, &y[1]), from_f32(O.z * f, &y[2]), from_f32(O.w * f, &y[3]);
-  const int64_t b = bh / a.Hkv, hq = (bh % a.Hkv) * a.G + row % a.G;
+  const int hq = (bh % a.Hkv) * a.G + row % a.G;
   T* op = reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + row / a.G * a.ot + 4 * lane;
   *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
 }
@@ -648,8 +537,9 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
   const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
   if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
   prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (ctas > 1) prompt_join_kernel<T><<<dim3(ctas - 1, ROWS / JOIN_WARPS), JOIN_WARPS * 32, 0, st>>>(a, ctas);
-  return check_launch("kv8_attend");
+  if (ctas == 1) return check_launch("kv8_attend");
+  const int rows = a.G * a.T < ROWS ? (int)(a.G * a.T) : ROWS;
+  return launch_join(prompt_join_kernel<T>, dim3(ctas - 1, (rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, a, ctas, st);
 }
 
 }  // namespace

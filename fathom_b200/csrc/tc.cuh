@@ -65,6 +65,10 @@ __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xf
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory"); }
 
+// Programmatic dependent launch: lets the next kernel of the stream start, and waits for the one before to finish.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 // Barrier `id` among `n` threads, and the same with an OR of a predicate.
 __device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ bool named_or(int id, int n, bool v) {
