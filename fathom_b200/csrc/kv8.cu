@@ -201,8 +201,8 @@ extern "C" int fathom_kv8_write(const void* K, const void* V, int dtype, int64_t
   FATHOM_REQUIRE(dtype >= FATHOM_DTYPE_F32 && dtype <= FATHOM_DTYPE_F16, FATHOM_ERR_UNSUPPORTED,
                  "kv8_write: dtype must be fp32, bf16 or fp16");
   FATHOM_REQUIRE(B >= 1 && Hkv >= 1 && B <= 65535 && Hkv <= 65535 && B * Hkv <= 65535 && T >= 0 && cap >= BLK &&
-                     cap % BLK == 0 && cap <= INT32_MAX, FATHOM_ERR_SHAPE,
-                 "kv8_write: need B*Hkv in 1..65535, T >= 0 and cap a multiple of 64 below 2^31");
+                     cap % BLK == 0 && cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE,
+                 "kv8_write: need B*Hkv in 1..65535, T >= 0 and cap a multiple of 64 up to 2^30");
   FATHOM_REQUIRE(start_dev || (start >= 0 && T <= cap && start <= cap - T), FATHOM_ERR_SHAPE,
                  "kv8_write: tokens [%lld, %lld + %lld) exceed the cache's %lld", (long long)start, (long long)start,
                  (long long)T, (long long)cap);
@@ -227,7 +227,7 @@ extern "C" int fathom_kv8_read(const uint8_t* rows, const float* scales, int64_t
   FATHOM_REQUIRE(rows && scales && K && V, FATHOM_ERR_NULL, "kv8_read: NULL pointer");
   FATHOM_REQUIRE(dtype >= FATHOM_DTYPE_F32 && dtype <= FATHOM_DTYPE_F16, FATHOM_ERR_UNSUPPORTED,
                  "kv8_read: dtype must be fp32, bf16 or fp16");
-  FATHOM_REQUIRE(BH >= 1 && BH <= 65535 && cap >= BLK && cap % BLK == 0 && cap <= INT32_MAX && start >= 0 && n >= 0 &&
+  FATHOM_REQUIRE(BH >= 1 && BH <= 65535 && cap >= BLK && cap % BLK == 0 && cap <= KV8_MAX_CAP && start >= 0 && n >= 0 &&
                      n <= cap && start <= cap - n, FATHOM_ERR_SHAPE,
                  "kv8_read: tokens [%lld, %lld + %lld) of a cache of %lld, BH = %lld", (long long)start, (long long)start,
                  (long long)n, (long long)cap, (long long)BH);

@@ -4,6 +4,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace fathom {
 namespace kv8 {
 
@@ -219,6 +221,19 @@ int dispatch_rows(int dtype, const void* q, const RowsArgs& a, int64_t rows, voi
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The current device's counter (its address is looked up once per device).
+unsigned long long* timeout_counter() {
+  static std::atomic<unsigned long long*> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+  unsigned long long* p = dev < 64 ? cached[dev].load(std::memory_order_relaxed) : nullptr;
+  if (!p) {
+    if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_timeouts) != cudaSuccess) return nullptr;
+    if (dev < 64) cached[dev].store(p, std::memory_order_relaxed);
+  }
+  return p;
+}
+
 // The rows as a 3-D tensor of bytes [BH][cap][256], read in 128-byte wide tiles of 128 tokens (the key or the
 // value half of each) in the 128-byte swizzle; tokens past cap read as 0.
 int rows_map(const Args& a, CUtensorMap* map) {
@@ -278,7 +293,7 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
                  "kv8_attend: queries must be bf16 or fp16");
   FATHOM_REQUIRE(B >= 1 && Hkv >= 1 && B <= 65535 && Hkv <= 65535 && B * Hkv <= 65535 && G >= 1 && G <= 65535 && T >= 1 &&
                      T <= INT32_MAX / G && B * Hkv * G * T <= INT32_MAX / 4 && cap >= BLK && cap % BLK == 0 &&
-                     cap <= INT32_MAX, FATHOM_ERR_SHAPE, "kv8_attend: bad shape");
+                     cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE, "kv8_attend: bad shape");
   FATHOM_REQUIRE(end_dev || (end >= 0 && end <= cap), FATHOM_ERR_SHAPE, "kv8_attend: end %lld is outside the cache's %lld",
                  (long long)end, (long long)cap);
   FATHOM_REQUIRE(aligned16(rows) && aligned16(q) && aligned16(out) && (q_stride_b | q_stride_h | q_stride_t) % 8 == 0 &&
@@ -287,9 +302,8 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
   FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_workspace_bytes(B, Hkv, G, T), FATHOM_ERR_WORKSPACE,
                  "kv8_attend: workspace too small");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  unsigned long long* timeouts = nullptr;
-  const cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void**>(&timeouts), g_timeouts);
-  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  unsigned long long* timeouts = timeout_counter();
+  if (!timeouts) return set_error(FATHOM_ERR_CUDA, "kv8_attend: no address of the wait counter");
   const Args a{q, q_stride_b, q_stride_h, q_stride_t, out, o_stride_b, o_stride_h, o_stride_t, rows, scales, cap, end,
                end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts};
   CUtensorMap map;
@@ -312,7 +326,7 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
                  "kv8_attend_picks: queries must be fp32, bf16 or fp16");
   FATHOM_REQUIRE(B >= 1 && Hkv >= 1 && B <= 65535 && Hkv <= 65535 && B * Hkv <= 65535 && G >= 1 && G <= 65535 &&
                      B * Hkv * G <= INT32_MAX / 8 && k >= 1 && k <= INT32_MAX && cap >= BLK && cap % BLK == 0 &&
-                     cap <= INT32_MAX, FATHOM_ERR_SHAPE, "kv8_attend_picks: bad shape");
+                     cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE, "kv8_attend_picks: bad shape");
   FATHOM_REQUIRE(end_dev || (end >= 0 && end <= cap), FATHOM_ERR_SHAPE,
                  "kv8_attend_picks: end %lld is outside the cache's %lld", (long long)end, (long long)cap);
   FATHOM_REQUIRE(aligned16(rows) && aligned16(q) && aligned16(out), FATHOM_ERR_SHAPE,

@@ -534,8 +534,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args
 template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   using S = Shape<QT>;
   static_assert(S::SMEM <= 226 * 1024, "shared memory");
-  const cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> told{0};
+  const int r = allow_smem(prompt_kernel<T, QT>, S::SMEM, told);
+  if (r != FATHOM_OK) return r;
   prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
   if (ctas == 1) return check_launch("kv8_attend");
   const int rows = a.G * a.T < ROWS ? (int)(a.G * a.T) : ROWS;

@@ -512,15 +512,18 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
 
+// Short rows of a known length have a CTA each: up to 8 tiles, ~0.5 us apiece, take less than the second kernel.
+bool whole_rows(const Args& a) { return !a.end_dev && a.end <= 8 * TILE; }
+
 template <typename T, int NR, int QT>
 int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   using S = Shape<NR, QT>;
   static_assert(S::SMEM <= 224 * 1024, "shared memory");
-  const cudaError_t e =
-      cudaFuncSetAttribute(token_kernel<T, NR, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> told{0};
+  const int r = allow_smem(token_kernel<T, NR, QT>, S::SMEM, told);
+  if (r != FATHOM_OK) return r;
   token_kernel<T, NR, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (!a.end_dev && a.end <= TILE) return check_launch("kv8_attend");   // one tile each: nothing to join
+  if (whole_rows(a)) return check_launch("kv8_attend");      // nothing to join
   return launch_join(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, a, ctas, st);
 }
 
@@ -532,17 +535,21 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   return launch<T, 16, QT>(map, a, ctas, st);
 }
 
+int token_launch(const CUtensorMap& map, const Args& a, int dtype, int ctas, cudaStream_t st) {
+  return dtype == FATHOM_DTYPE_BF16 ? launch_rows<__nv_bfloat16, 2>(map, a, ctas, st)
+                                    : launch_rows<__half, 3>(map, a, ctas, st);
+}
+
 }  // namespace
 
 size_t token_workspace(int64_t BH, int64_t R) { return (size_t)((sm_count() + BH) * R * PART * sizeof(float)); }
 
 int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st) {
   // one CTA per SM, but no more than there can be tiles
+  if (whole_rows(a)) return token_launch(map, a, dtype, a.B * a.Hkv, st);
   const int64_t per = cdiv(a.end_dev ? a.cap : a.end, TILE), most = (int64_t)a.B * a.Hkv * (per > 1 ? per : 1);
   const int64_t sms = sm_count() < MAX_CTAS ? sm_count() : MAX_CTAS;
-  const int ctas = (int)(most < sms ? most : sms);
-  return dtype == FATHOM_DTYPE_BF16 ? launch_rows<__nv_bfloat16, 2>(map, a, ctas, st)
-                                    : launch_rows<__half, 3>(map, a, ctas, st);
+  return token_launch(map, a, dtype, (int)(most < sms ? most : sms), st);
 }
 
 }  // namespace kv8

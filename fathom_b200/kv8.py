@@ -15,15 +15,17 @@ step over the cache can be captured in a CUDA graph.
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, require_cuda, stream_of
+from ._lib import check, lib, ptr, require_cuda
 
 BLK, D = 64, 128
 
 
 def _position(x, B, device, what):
     """(number, device tensor or None) of a position given as an int or as int64 [B] (or [1]) on `device`."""
-    if not torch.is_tensor(x):
+    if not isinstance(x, torch.Tensor):
         return int(x), None
+    if x.dtype == torch.int64 and x.dim() == 1 and x.shape[0] == B and x.device == device and x.is_contiguous():
+        return 0, x
     if x.device != device or x.dtype != torch.int64 or x.numel() not in (1, B) or x.dim() > 1:
         raise ValueError(f"{what} must be an int or an int64 [{B}] tensor on {device}")
     return 0, x.reshape(-1).expand(B).contiguous()
@@ -56,13 +58,25 @@ class KVCache8:
                 or not scales.is_contiguous() or scales.device != rows.device):
             raise ValueError(f"KVCache8: scales must be contiguous float32 [{self.BH}, {self.nblk}, 2] beside the rows")
         self.rows, self.scales, self.device = rows, scales, rows.device
+        self._ws = {}              # workspace bytes of a call's shape
 
     def nbytes(self):
         return self.rows.numel() + self.scales.numel() * 4
 
+    def _stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def _workspace(self, key, size, *args):
+        """Scratch of one call, from the allocator's pool of the current stream: calls on two streams share none."""
+        n = self._ws.get(key)
+        if n is None:
+            n = self._ws[key] = size(self.B, self.Hkv, *args)
+        return torch.empty(n, dtype=torch.uint8, device=self.device), n
+
     def _check_on(self, what, *tensors):
         for t in tensors:
             if t.device != self.device:
+                require_cuda(t)
                 raise ValueError(f"{what}: expected tensors on {self.device}, got one on {t.device}")
 
     def write(self, K, V, start=0):
@@ -71,7 +85,6 @@ class KVCache8:
         alone and tokens past cap are dropped).  The scale of a block covers every token written to it in
         this and in earlier calls; a block written from its first token on starts afresh.  NaN and infinities
         are stored as NaN and do not enter the scale."""
-        require_cuda(K, V)
         self._check_on("KVCache8.write", K, V)
         if K.dim() != 4 or K.shape[0] != self.B or K.shape[1] != self.Hkv or K.shape[3] != D or V.shape != K.shape:
             raise ValueError(f"KVCache8.write: K and V must be [{self.B}, {self.Hkv}, T, {D}] "
@@ -87,9 +100,10 @@ class KVCache8:
         K, V = _rows16(K), _rows16(V)
         if K.stride() != V.stride():
             K, V = K.contiguous(), V.contiguous()
-        check(lib().fathom_kv8_write(ptr(K), ptr(V), _lib.DTYPE_CODE[K.dtype], self.B, self.Hkv, T, *K.stride()[:3],
-                                     num, ptr(dev), self.cap, ptr(self.rows), ptr(self.scales), stream_of(self.device)),
-              "KVCache8.write")
+        sb, sh, st, _ = K.stride()
+        check(lib().fathom_kv8_write(K.data_ptr(), V.data_ptr(), _lib.DTYPE_CODE[K.dtype], self.B, self.Hkv, T, sb, sh,
+                                     st, num, ptr(dev), self.cap, self.rows.data_ptr(), self.scales.data_ptr(),
+                                     self._stream()), "KVCache8.write")
 
     def read(self, start=0, n=None, dtype=torch.bfloat16):
         """Tokens [start, start + n) (to the end of the cache by default) as (K, V) [B, Hkv, n, 128] in dtype: fp32
@@ -103,7 +117,7 @@ class KVCache8:
         V = torch.empty_like(K)
         if n:
             check(lib().fathom_kv8_read(ptr(self.rows), ptr(self.scales), self.BH, self.cap, start, n,
-                                        _lib.DTYPE_CODE[dtype], ptr(K), ptr(V), stream_of(self.device)),
+                                        _lib.DTYPE_CODE[dtype], ptr(K), ptr(V), self._stream()),
                   "KVCache8.read")
         return K, V
 
@@ -112,7 +126,6 @@ class KVCache8:
         the T queries of a sequence are its last T tokens, already written, and query t sees the keys
         [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
         that sees no key gives 0.  Returns [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
-        require_cuda(q)
         self._check_on("KVCache8.attend", q)
         if q.dim() != 4 or q.shape[0] != self.B or q.shape[1] < 1 or q.shape[1] % self.Hkv or q.shape[3] != D:
             raise ValueError(f"KVCache8.attend: q must be [{self.B}, a multiple of {self.Hkv}, T, {D}] "
@@ -123,15 +136,16 @@ class KVCache8:
         num, dev = _position(end, B, self.device, "KVCache8.attend: end")
         if dev is None and not 0 <= num <= self.cap:
             raise ValueError(f"KVCache8.attend: end {num} is outside the cache's {self.cap}")
-        out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=self.device).transpose(1, 2)
+        out = torch.empty_strided(q.shape, (T * Hq * D, D, Hq * D, 1), dtype=q.dtype, device=self.device)
         if T == 0:
             return out
         q = _rows16(q)
         G = Hq // self.Hkv
-        ws = _workspace(self.device, lib().fathom_kv8_attend_workspace_bytes(B, self.Hkv, G, T))
-        check(lib().fathom_kv8_attend(ptr(q), _lib.DTYPE_CODE[q.dtype], B, self.Hkv, G, T, *q.stride()[:3],
-                                      ptr(self.rows), ptr(self.scales), self.cap, num, ptr(dev), ptr(out),
-                                      *out.stride()[:3], ptr(ws), ws.numel(), stream_of(self.device)),
+        ws, nws = self._workspace((G, T), lib().fathom_kv8_attend_workspace_bytes, G, T)
+        sb, sh, st, _ = q.stride()
+        check(lib().fathom_kv8_attend(q.data_ptr(), _lib.DTYPE_CODE[q.dtype], B, self.Hkv, G, T, sb, sh, st,
+                                      self.rows.data_ptr(), self.scales.data_ptr(), self.cap, num, ptr(dev),
+                                      out.data_ptr(), T * Hq * D, D, Hq * D, ws.data_ptr(), nws, self._stream()),
               "KVCache8.attend")
         return out
 
@@ -140,7 +154,6 @@ class KVCache8:
         idx [BH, G, k] int64.  Picks outside [0, end) are ignored (end: an int, int64 [B] on the device, or None
         for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  fp32
         arithmetic; returns [BH, G, 128] in q's dtype."""
-        require_cuda(q, idx)
         self._check_on("KVCache8.attend_picks", q, idx)
         if q.dim() != 3 or q.shape[0] != self.BH or q.shape[1] < 1 or q.shape[2] != D:
             raise ValueError(f"KVCache8.attend_picks: q must be [{self.BH}, G, {D}] (got {tuple(q.shape)})")
@@ -160,21 +173,16 @@ class KVCache8:
         if q.data_ptr() % 16:
             q = q.clone()
         out = torch.empty(BH, G, D, dtype=q.dtype, device=self.device)
-        ws = _workspace(self.device, lib().fathom_kv8_attend_picks_workspace_bytes(self.B, self.Hkv, G, k))
+        ws, nws = self._workspace((G, k, "picks"), lib().fathom_kv8_attend_picks_workspace_bytes, G, k)
         check(lib().fathom_kv8_attend_picks(ptr(q), _lib.DTYPE_CODE[q.dtype], self.B, self.Hkv, G, ptr(idx), k,
                                             ptr(self.rows), ptr(self.scales), self.cap, num, ptr(dev), ptr(out),
-                                            ptr(ws), ws.numel(), stream_of(self.device)), "KVCache8.attend_picks")
+                                            ptr(ws), nws, self._stream()), "KVCache8.attend_picks")
         return out
-
-
-def _workspace(device, nbytes):
-    """Scratch of one call, from the allocator's pool of the current stream: calls on two streams share none."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 def _rows16(x):
     """x with 16-byte aligned, contiguous 128-element rows (a copy where it has none)."""
-    per16 = 16 // x.element_size()
-    if x.stride(-1) != 1 or x.data_ptr() % 16 or any(s % per16 for s in x.stride()[:-1]):
+    sb, sh, st, sd = x.stride()
+    if sd != 1 or (sb | sh | st) * x.element_size() % 16 or x.data_ptr() % 16:
         return x.clone(memory_format=torch.contiguous_format)
     return x
