@@ -103,10 +103,47 @@ __device__ inline int64_t line(const Args& a, int64_t at, Place* place) {
   return total;
 }
 
-// One warp: where this CTA's share begins, and how many tiles it has (0 or less: none).
+// n / d for 0 <= n, d > 0: in 32 bits where n allows it (a 64-bit division is ~100 cycles longer).
+__device__ __forceinline__ int64_t quotient(int64_t n, int d) {
+  return n >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
+
+// One warp: where this CTA's share begins, and how many tiles it has (0 or less: none).  A token's latency counts on
+// this: the common forms, one item per bh, equal lengths or up to 32 sequences, take one pass.
 __device__ inline Place my_share(const Args& a, int* count) {
+  const int lane = threadIdx.x & 31;
   Place p{0, 0};
-  const int64_t total = line(a, -1, &p), share = (total + gridDim.x - 1) / gridDim.x, first = share * blockIdx.x;
+  if (items_per_bh(a) == 1 && (!a.end_dev || a.B <= 32)) {
+    int64_t total, x = 0, mine = 0;
+    int nt = 0;
+    if (a.end_dev) {
+      nt = lane < a.B ? tiles_of(a, seq_end(a, lane), 0) : 0;
+      x = mine = (int64_t)nt * a.Hkv;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      total = __shfl_sync(0xffffffffu, x, 31);
+    } else {
+      nt = tiles_of(a, seq_end(a, 0), 0);
+      total = (int64_t)nt * a.Hkv * a.B;
+    }
+    const int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
+    int64_t at = share * blockIdx.x;
+    *count = (int)min(share, total - at);
+    if (*count <= 0) return p;
+    int b = 0;
+    if (a.end_dev) {
+      const unsigned hit = __ballot_sync(0xffffffffu, x > at);     // the first sequence that ends past `at`
+      b = __ffs(hit) - 1;
+      at -= __shfl_sync(0xffffffffu, x - mine, b);
+      nt = __shfl_sync(0xffffffffu, nt, b);
+    }
+    const int bh = (int)quotient(at, nt);
+    return Place{b * a.Hkv + bh, (int)(at - (int64_t)bh * nt)};
+  }
+  const int64_t total = line(a, -1, &p), share = quotient(total + gridDim.x - 1, gridDim.x), first = share * blockIdx.x;
   *count = (int)min(share, total - first);
   if (*count > 0) line(a, first, &p);
   return p;

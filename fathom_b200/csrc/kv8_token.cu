@@ -60,8 +60,6 @@ __device__ __forceinline__ float redux_max(float x) {      // over the warp; NaN
   return y;
 }
 
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
-
 template <typename T> __device__ __forceinline__ void unpack4(uint2 v, float (&x)[4]) {
   const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
@@ -80,7 +78,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
   __shared__ int s_gave_up;
   __shared__ float s_rs[NR];                     // scale of a row's scores: 2^e log2(e) / sqrt(128)
   __shared__ float s_top[2][4][NR];              // a tile's largest s + log2 vs, by warpgroup and warp
-  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR];   // at a row's end: references; denominators by warp
+  // at a row's end: references; denominators by warp; then the denominator, its reference, and what brings O^T there
+  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[NR], s_ref[NR], s_f[2][NR];
   const uint32_t bar0 = tc::smem_u32(bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   auto empty = [&](uint32_t s) { return bar0 + 8 * (STAGES + s); };
@@ -96,16 +95,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
   int count;
   const Place place = my_share(a, &count);
   Walk w(a, place, count);
-  uint32_t loaded = 0;                           // the load warp's tiles; the first STAGES need no wait
-  auto load = [&](int tile, int bh) {
-    const uint32_t s = loaded % STAGES;
-    tc::mbar_expect_tx(full(s), STAGE_BYTES);
-    tc::tma_load_3d(sbase + s * STAGE_BYTES, &map, 0, tile * TILE, bh, full(s));
-    tc::tma_load_3d(sbase + s * STAGE_BYTES + TILE * D, &map, D, tile * TILE, bh, full(s));
-    ++loaded;
-  };
-  bool more = false;
   if (warp == 8) {
+    // ---- loads: the share's tiles in order, as stages come free.  They begin while the CTA still sets itself up.
     if (lane == 0) {
       for (int s = 0; s < STAGES; ++s) tc::mbar_init(full(s), 1), tc::mbar_init(empty(s), 1);
       for (int k = 0; k < 2; ++k)
@@ -114,45 +105,37 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       tc::mbar_init(drain, 1);
       tc::fence_mbar_init();
       s_gave_up = 0;
-      more = w.next();
-      while (more && loaded < STAGES) {          // memory is at work while the CTA sets itself up
-        load(w.j0++, w.bh);
-        if (w.j0 == w.j1) more = w.next();
-      }
     }
     __syncwarp();
-  } else {
-    if (warp == 9) tc::tmem_alloc(tc::smem_u32(&s_tmem), S::TMEM);
-    else
-      for (int i = tid; i < (S::END - S::Q) / 16; i += 2 * GROUP)      // operand columns that no row writes stay 0
-        reinterpret_cast<uint4*>(smem + S::Q)[i] = make_uint4(0, 0, 0, 0);
-  }
-  tc::fence_async_smem();
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  tc::launch_dependents();
-  const uint32_t tm = s_tmem;
-
-  if (warp == 8) {
-    // ---- loads: the share's tiles in order, as stages come free
+    tc::named_arrive(4, THREADS);
     if (lane == 0) {
-      while (more) {
-        if (!tc::mbar_wait(empty(loaded % STAGES), ((loaded / STAGES) & 1) ^ 1, gave_up)) break;
-        load(w.j0++, w.bh);
-        if (w.j0 == w.j1) more = w.next();
+      uint32_t i = 0;
+      bool ok = true;
+      while (ok && w.next()) {
+        for (int tile = w.j0; tile < w.j1; ++tile, ++i) {
+          const uint32_t s = i % STAGES;
+          ok = tc::mbar_wait(empty(s), ((i / STAGES) & 1) ^ 1, gave_up);
+          if (!ok) break;
+          tc::mbar_expect_tx(full(s), STAGE_BYTES);
+          tc::tma_load_3d(sbase + s * STAGE_BYTES, &map, 0, tile * TILE, w.bh, full(s));
+          tc::tma_load_3d(sbase + s * STAGE_BYTES + TILE * D, &map, D, tile * TILE, w.bh, full(s));
+        }
       }
       if (*gave_up) {          // copies in flight land before the CTA ends (bounded: the flag is up, so by time alone)
-        for (uint32_t j = loaded > STAGES ? loaded - STAGES : 0; j < loaded; ++j) {
+        for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j) {
           const unsigned long long t0 = tc::now_ns();
           while (!tc::mbar_try(full(j % STAGES), (j / STAGES) & 1) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
         }
       }
     }
   } else if (warp == 9) {
+    tc::tmem_alloc(tc::smem_u32(&s_tmem), S::TMEM);
+    tc::fence_before();
+    tc::named_sync(4, THREADS);
+    tc::fence_after();
     // ---- products (the whole warp: elect_one): S^T of tile i, then O^T of tile i - 2, whose weights were made meanwhile
     constexpr uint32_t id_s = tc::instr(S::NQ, false, false), id_o = tc::instr(S::NP, true, true);
-    const uint32_t tmu = tc::uniform(tm);
+    const uint32_t tmu = tc::uniform(s_tmem);
     uint32_t seg = 0, ks = 0, vs = 0;             // rows begun: each fills q once; stages of the next S^T and O^T
     bool ok = true;
     auto scores = [&](uint32_t i) {
@@ -210,22 +193,46 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     // ---- softmax: warpgroup g has the tiles i = g mod 2 of the share; thread = token of the tile; lane of tensor memory =
     // token of S^T, dim of O^T
     const int R = rows_of(a), late = (int)a.T - 1, g = warp >> 2, t = tid & (GROUP - 1);
+    // A warp brings every eighth row of q, a lane 4 dims of it; the share's first row ahead of everything else.
+    constexpr int QR = (NR + 7) / 8;
+    uint2 qv[QR];
+    auto q_at = [&](int r, int h) {               // rows are token-major: row = token * G + head
+      const int tt = late ? r / a.G : 0;
+      return w.b * a.qb + (int64_t)(h * a.G + r - tt * a.G) * a.qh + tt * a.qt;
+    };
+    auto load_q = [&]() {
+      const int h = w.bh % a.Hkv;
+#pragma unroll
+      for (int i = 0; i < QR; ++i) {
+        const int r = warp + 8 * i;
+        if (r < R) qv[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(a.q) + q_at(r, h) + lane * 4);
+      }
+    };
+    bool more = w.next();
+    if (more) load_q();
+    for (int i = tid; i < (S::END - S::Q) / 16; i += 2 * GROUP)      // operand columns that no row writes stay 0
+      reinterpret_cast<uint4*>(smem + S::Q)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_async_smem();
+    tc::fence_before();
+    tc::named_sync(4, THREADS);
+    tc::fence_after();
+    tc::launch_dependents();
+    const uint32_t tm = s_tmem;
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tm_s = tm + g * S::NQ + my, tm_o = tm + 2 * S::NQ + my;
     uint8_t* pb = smem + S::P + g * S::NP * TILE + t * 16;
     uint32_t i0 = 0;                              // the share's tiles before this row
     bool ok = true, bad = false;                  // ok: this thread's waits; bad: some thread's gave up (uniform)
-    while (w.next()) {
+    while (more) {
       const int h = w.bh % a.Hkv, n = w.j1 - w.j0;
-      // this row's queries as terms: a warp takes every eighth, a lane 4 dims.  The products of the row before are
-      // complete (its O^T was read below), so its q may go.
+      // this row's queries as terms.  The products of the row before are complete (its O^T was read below), so its q
+      // may go.
 #pragma unroll
-      for (int rr = 0; rr < (NR + 7) / 8; ++rr) {
-        const int r = warp + 8 * rr;              // token-major: row = token * G + head
+      for (int rr = 0; rr < QR; ++rr) {
+        const int r = warp + 8 * rr;
         if (r >= R) break;
-        const int tt = r / a.G, hq = h * a.G + r - tt * a.G;
         float x[4];
-        unpack4<T>(*reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt + lane * 4), x);
+        unpack4<T>(qv[rr], x);
         uint32_t top = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
@@ -402,56 +409,63 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       tc::fence_before();
       bad = tc::named_or(3, 2 * GROUP, !ok);
       tc::fence_after();
-      // warpgroup g finishes the rows r = g mod 2, of both O^T.  One that had no tile left its columns as they were.
-      const bool whole = w.j0 == 0 && w.j1 == w.n, both = n > 1;
-      float o[2][NR];
+      const Walk now = w;
+      more = w.next();
+      if (more) load_q();                         // the next row's q, on its way while this one is finished
+      if (tid < NR) {
+        float mx = s_lm[0][tid], sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t c[TERMS][NR];
+        for (int v = 1; v < 8; ++v) mx = fmaxf(mx, s_lm[v][tid]);
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) tc::Tmem<NR>::ld(tm_o + k * S::NP + term * NR, c[term]);
-        tc::wait_ld();
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float v = __uint_as_float(c[TERMS - 1][r]);
-#pragma unroll
-          for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[term][r]));
-          o[k][r] = v;
-        }
-      }
-      tc::fence_before();
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        if (r >= R || (r & 1) != g) continue;
-        float mx = s_lm[0][r], sum = 0.0f;
-#pragma unroll
-        for (int v = 1; v < 8; ++v) mx = fmaxf(mx, s_lm[v][r]);
-#pragma unroll
-        for (int v = 0; v < 8; ++v) sum += s_l[v][r] * ex2(s_lm[v][r] - mx);
-        // O^T is relative to m - HEAD: bring both to the denominator's reference
-        float x = 0.0f;
+        for (int v = 0; v < 8; ++v) sum = fmaf(s_l[v][tid], ex2(s_lm[v][tid] - mx), sum);
+        s_sum[tid] = sum;
+        s_ref[tid] = mx;
+        // O^T is relative to m - HEAD: both come to the denominator's reference.  A warpgroup that had no tile left its
+        // columns as they were.
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-          if ((both || k == (int)(i0 & 1)) && s_m[k][r] != -INFINITY) x = fmaf(o[k][r], exp2f(s_m[k][r] - HEAD - mx), x);
+          s_f[k][tid] = (n == 1 && k != (int)(i0 & 1)) || s_m[k][tid] == -INFINITY ? 0.0f : exp2f(s_m[k][tid] - HEAD - mx);
+      }
+      uint32_t c[2][TERMS][NR];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) tc::Tmem<NR>::ld(tm_o + k * S::NP + term * NR, c[k][term]);
+      }
+      tc::wait_ld();
+      tc::fence_before();
+      tc::named_sync(3, 2 * GROUP);
+      const bool whole = now.j0 == 0 && now.j1 == now.n;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (r >= R || (r & 1) != g) continue;     // warpgroup g finishes the rows r = g mod 2
+        float x = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float v = __uint_as_float(c[k][TERMS - 1][r]);
+#pragma unroll
+          for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][r]));
+          if (s_f[k][r] != 0.0f) x = fmaf(v, s_f[k][r], x);
+        }
+        const float sum = s_sum[r];
         if (bad) x = __uint_as_float(0x7FFFFFFFu);
-        const int tt = r / a.G, hq = h * a.G + r - tt * a.G;
         if (whole) {
-          T* op = reinterpret_cast<T*>(a.out) + w.b * a.ob + hq * a.oh + tt * a.ot;
+          const int tt = late ? r / a.G : 0;
+          T* op = reinterpret_cast<T*>(a.out) + now.b * a.ob + (int64_t)(h * a.G + r - tt * a.G) * a.oh + tt * a.ot;
           from_f32(bad ? x : sum == 0.0f ? 0.0f : x / sum, op + t);
         } else {
-          float* part = a.part + (((int64_t)blockIdx.x + w.bh) * R + r) * PART;
+          float* part = a.part + (((int64_t)blockIdx.x + now.bh) * R + r) * PART;
           part[t] = x;
-          if (t == 0) part[D] = mx, part[D + 1] = sum;
+          if (t == 0) part[D] = s_ref[r], part[D + 1] = sum;
         }
       }
-      tc::named_sync(3, 2 * GROUP);               // the shared denominators and scales are read
       i0 += n;
     }
   }
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (warp == 9) tc::tmem_free(tm, S::TMEM);
+  if (warp == 9) tc::tmem_free(s_tmem, S::TMEM);
   if (tid == 0 && s_gave_up) atomicAdd(a.timeouts, 1ull);
 }
 
