@@ -156,6 +156,8 @@ struct Walk {
   int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
   __device__ Walk(const Args& a_, const Place& p, int count)
       : a(a_), per(items_per_bh(a_)), item(p.item), tile(p.tile), left(count) {}
+  // accumulators of 128 rows that the item needs
+  __device__ int halves() const { return rows_of(a) - it * ROWS > ROWS / 2 ? 2 : 1; }
   __device__ bool next() {
     if (left <= 0) return false;
     bh = item / per;

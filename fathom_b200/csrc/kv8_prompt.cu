@@ -128,20 +128,24 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
     while (w.next()) {
+      if (w.halves() <= h2) {                      // no row in this half
+        vt += w.j1 - w.j0;
+        continue;
+      }
       const int total = rows_of(a), row = w.it * ROWS + h2 * HALF + r;
+      const bool idle = row - lane >= total;       // no row in this warp: it only keeps the barriers going
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
       // the row's query as e4m3 terms of its own scale: this thread's 64 dims
-      float rs;
-      {
+      float rs = 0.0f;
+      if (!idle) {
         const T* qp = reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt + 64 * ch;
-        uint4 v[8];
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          v[i] = *reinterpret_cast<const uint4*>(qp + 8 * i);
-          const T* e = reinterpret_cast<const T*>(&v[i]);
+          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * i);
+          const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
           for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f32(e[j])) & 0x7FFFFFFFu);
         }
@@ -149,28 +153,26 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         tc::named_sync(pair_bar, 64);
         top = max(top, __float_as_uint(*s_other));
         const int e2 = kv8_exponent(top);
-        const float inv = pow2i(-e2);
+        const float inv = top < 0x7F800000u ? pow2i(-e2) : __uint_as_float(0x7FFFFFFFu);   // a row with inf or NaN is NaN
         rs = pow2i(e2) * QSCALE;
+#pragma unroll 1                                   // run once a piece: small code over fast code
+        for (int c = 0; c < 8; ++c) {              // 8 dims a time, read again from the caches
+          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * c);
+          const T* e = reinterpret_cast<const T*>(&v);
+          float2 x[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x[16];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const T* e = reinterpret_cast<const T*>(&v[2 * c + i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[8 * i + j] = to_f32(e[j]) * inv;
-          }
+          for (int j = 0; j < 4; ++j) x[j] = make_float2(to_f32(e[2 * j]) * inv, to_f32(e[2 * j + 1]) * inv);
 #pragma unroll
           for (int term = 0; term < QT; ++term) {
             uint32_t code[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              code[i] = kv8_encode2(x[4 * i], x[4 * i + 1]) | kv8_encode2(x[4 * i + 2], x[4 * i + 3]) << 16;
-              const float2 lo = kv8_decode2(code[i]), hi = kv8_decode2(code[i] >> 16);
-              x[4 * i] -= lo.x, x[4 * i + 1] -= lo.y, x[4 * i + 2] -= hi.x, x[4 * i + 3] -= hi.y;
+            for (int j = 0; j < 4; ++j) {
+              code[j] = __nv_cvt_float2_to_fp8x2(x[j], __NV_SATFINITE, __NV_E4M3);
+              const float2 d = kv8_decode2(code[j]);
+              x[j] = make_float2(x[j].x - d.x, x[j].y - d.y);
             }
-            *reinterpret_cast<uint4*>(sq + term * HALF * D + (((4 * ch + c) ^ (r & 7)) << 4)) =
-                make_uint4(code[0], code[1], code[2], code[3]);
+            *reinterpret_cast<uint2*>(sq + term * HALF * D + (((4 * ch + (c >> 1)) ^ (r & 7)) << 4) + (c & 1) * 8) =
+                make_uint2(code[0] | code[1] << 16, code[2] | code[3] << 16);
           }
         }
       }
@@ -194,6 +196,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         ++phase;
         __syncwarp();
         tc::fence_after();
+        if (idle) {                                // weights of rows that no one reads may be anything
+          if (lane == 0) tc::mbar_arrive(p_full(h2));
+          continue;
+        }
         int see = BLK;                             // tokens of the block that this row sees
         const bool masked = (j + 1) * TILE > all_see;
         if (masked) {
@@ -278,6 +284,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       }
       ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);      // the piece's last product
       ++phase;
+      if (idle) continue;
+      __syncwarp();
       *s_mine = l;
       tc::named_sync(pair_bar, 64);
       l += *s_other;
@@ -409,11 +417,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       // ---- products (the whole warp: elect_one)
       constexpr uint32_t id_s = tc::instr(TILE, false, false), id_o = tc::instr(D, false, true);
       const uint32_t tmu = tc::uniform(tm);
-      uint32_t i = 0, pn = 0, seg = 0;             // tiles done, weight tiles done, pieces begun
+      uint32_t i = 0;                              // tiles done
+      uint32_t pn[2] = {0, 0}, seg[2] = {0, 0};    // by half: weight tiles done, pieces begun
       uint32_t ks = 0, vs = 0;                     // stages of the next key tile, of the next value tile
       bool ok = true;
-      // S_h of the next key tile, which is spent when h is 1
-      auto scores = [&](int h) {
+      // S_h of the next key tile, which is spent with the last half
+      auto scores = [&](int h, bool spent) {
         const uint64_t dk = tc::operand(sbase + S::K + tc::uniform(ks) * KBYTES);
         if (tc::elect_one()) {
 #pragma unroll
@@ -423,54 +432,55 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
               tc::mma_fp8(tmu + h * 128, tc::operand(sbase + S::Q + (h * QT + term) * HALF * D) + kk * 2, dk + kk * 2, id_s,
                           term > 0 || kk > 0);
           }
-          if (h == 1) tc::mma_commit(bar + 8 * (KSTAGES + ks));
+          if (spent) tc::mma_commit(bar + 8 * (KSTAGES + ks));
           tc::mma_commit(s_full(h));
         }
         __syncwarp();
-        if (h == 1) ks = ks + 1 == KSTAGES ? 0 : ks + 1;
+        if (spent) ks = ks + 1 == KSTAGES ? 0 : ks + 1;
       };
       // O_h of the next value tile; the piece's last is announced as scores are
-      auto values = [&](int h, bool accumulate, bool last) {
+      auto values = [&](int h, bool spent, bool accumulate, bool last) {
         const uint64_t dv = tc::operand(sbase + S::V + tc::uniform(vs) * VBYTES, TILE * 128);
         if (tc::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < TILE / 16; ++kk)   // 16 tokens a step: 8 columns of weights, 2 groups of 8 value rows
             tc::mma_f16_ts(tmu + 256 + h * 128, tmu + h * 128 + kk / 2 * 32 + kk % 2 * 8, dv + kk * (16 * 128 / 16), id_o,
                            accumulate || kk > 0);
-          if (h == 1) tc::mma_commit(bar2 + 8 * (VSTAGES + vs));
+          if (spent) tc::mma_commit(bar2 + 8 * (VSTAGES + vs));
           if (last) tc::mma_commit(s_full(h));
         }
         __syncwarp();
-        if (h == 1) vs = vs + 1 == VSTAGES ? 0 : vs + 1;
+        if (spent) vs = vs + 1 == VSTAGES ? 0 : vs + 1;
       };
       while (ok && w.next()) {
         const int n = w.j1 - w.j0;
-        for (int h = 0; h < 2; ++h) ok = ok && tc::mbar_wait(q_full(h), seg & 1, gave_up);
-        ++seg;
+        const bool two = w.halves() == 2;
+        ok = tc::mbar_wait(q_full(0), seg[0]++ & 1, gave_up);
+        if (two) ok = ok && tc::mbar_wait(q_full(1), seg[1]++ & 1, gave_up);
         ok = ok && tc::mbar_wait(k_full(i), (i / KSTAGES) & 1, gave_up);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc::fence_after();
-        scores(0);
-        scores(1);
+        scores(0, !two);
+        if (two) scores(1, true);
         for (int j = 1; j <= n; ++j) {
           const uint32_t v = i + j - 1;
           const bool last = j == n;
           ok = last || tc::mbar_wait(k_full(i + j), ((i + j) / KSTAGES) & 1, gave_up);
           ok = ok && tc::mbar_wait(v_full(v), (v / VSTAGES) & 1, gave_up);
-          ok = ok && tc::mbar_wait(p_full(0), pn & 1, gave_up);
+          ok = ok && tc::mbar_wait(p_full(0), pn[0]++ & 1, gave_up);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc::fence_after();
-          values(0, j > 1, last);
-          if (!last) scores(0);
-          ok = tc::mbar_wait(p_full(1), pn & 1, gave_up);
+          values(0, !two, j > 1, last);
+          if (!last) scores(0, !two);
+          if (!two) continue;
+          ok = tc::mbar_wait(p_full(1), pn[1]++ & 1, gave_up);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc::fence_after();
-          values(1, j > 1, last);
-          if (!last) scores(1);
-          ++pn;
+          values(1, true, j > 1, last);
+          if (!last) scores(1, true);
         }
         i += n;
       }
