@@ -24,6 +24,9 @@ struct Args {
   int64_t T;
   float* part;                    // workspace: partial results
   unsigned long long* timeouts;   // counts waits that gave up
+  // Set by plan_shares (kv8_line.cuh) where every row bh is one item of the same length: tiles per CTA, and the
+  // distance of two items in the line.  0: the device cuts the line.
+  int share, stride;
 };
 
 // Tokens of sequence b that exist.
@@ -52,10 +55,10 @@ int sm_count();
 // kv8_token.cu: up to TOKEN_ROWS query rows (G * T) per KV head.
 constexpr int TOKEN_ROWS = 16;
 size_t token_workspace(int64_t BH, int64_t R);
-int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
+int token_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st);
 // kv8_prompt.cu: any number of query rows, 256 at a time.
 size_t prompt_workspace();
-int prompt_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st);
+int prompt_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st);
 
 }  // namespace kv8
 }  // namespace fathom

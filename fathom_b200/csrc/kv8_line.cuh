@@ -2,9 +2,11 @@
 //
 // An item is up to 256 query rows (token-major pairs of token and head) of one cache row bh; its tiles are the 128-token
 // stretches up to the last key that any of its rows sees.  Items follow each other by bh, then by row; CTA c of C
-// takes tiles [c * share, (c + 1) * share) of the line, share = ceil(tiles / C), whatever the lengths are.
+// takes tiles [c * share, (c + 1) * share) of the line, share = ceil(tiles / C), whatever the lengths are.  Where every
+// bh is one item of the same length, items may lie further apart than their tiles, so that no CTA has pieces of two.
 #pragma once
 #include "kv8_attn.cuh"
+#include "tc.cuh"
 
 #include <atomic>
 
@@ -109,39 +111,35 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int d) {
 }
 
 // One warp: where this CTA's share begins, and how many tiles it has (0 or less: none).  A token's latency counts on
-// this: the common forms, one item per bh, equal lengths or up to 32 sequences, take one pass.
+// this: the common forms, a plan or up to 32 sequences of one item per bh, take one pass.
 __device__ inline Place my_share(const Args& a, int* count) {
   const int lane = threadIdx.x & 31;
   Place p{0, 0};
-  if (items_per_bh(a) == 1 && (!a.end_dev || a.B <= 32)) {
-    int64_t total, x = 0, mine = 0;
-    int nt = 0;
-    if (a.end_dev) {
-      nt = lane < a.B ? tiles_of(a, seq_end(a, lane), 0) : 0;
-      x = mine = (int64_t)nt * a.Hkv;
+  if (a.share) {
+    const int64_t at = (int64_t)a.share * blockIdx.x, items = (int64_t)a.B * a.Hkv;
+    p.item = (int)quotient(at, a.stride);
+    p.tile = (int)(at - (int64_t)p.item * a.stride);
+    const int nt = tiles_of(a, seq_end(a, 0), 0);
+    *count = (int)min((int64_t)a.share, a.stride > nt ? (int64_t)nt - p.tile : items * nt - at);
+    return p;
+  }
+  if (items_per_bh(a) == 1 && a.B <= 32) {       // (ragged: equal lengths have a plan)
+    const int nt = lane < a.B ? tiles_of(a, seq_end(a, lane), 0) : 0;
+    const int64_t mine = (int64_t)nt * a.Hkv;
+    int64_t x = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      total = __shfl_sync(0xffffffffu, x, 31);
-    } else {
-      nt = tiles_of(a, seq_end(a, 0), 0);
-      total = (int64_t)nt * a.Hkv * a.B;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    const int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
+    const int64_t total = __shfl_sync(0xffffffffu, x, 31), share = quotient(total + gridDim.x - 1, gridDim.x);
     int64_t at = share * blockIdx.x;
     *count = (int)min(share, total - at);
     if (*count <= 0) return p;
-    int b = 0;
-    if (a.end_dev) {
-      const unsigned hit = __ballot_sync(0xffffffffu, x > at);     // the first sequence that ends past `at`
-      b = __ffs(hit) - 1;
-      at -= __shfl_sync(0xffffffffu, x - mine, b);
-      nt = __shfl_sync(0xffffffffu, nt, b);
-    }
-    const int bh = (int)quotient(at, nt);
-    return Place{b * a.Hkv + bh, (int)(at - (int64_t)bh * nt)};
+    const int b = __ffs(__ballot_sync(0xffffffffu, x > at)) - 1;     // the first sequence that ends past `at`
+    at -= __shfl_sync(0xffffffffu, x - mine, b);
+    const int n = __shfl_sync(0xffffffffu, nt, b), bh = (int)quotient(at, n);
+    return Place{b * a.Hkv + bh, (int)(at - (int64_t)bh * n)};
   }
   const int64_t total = line(a, -1, &p), share = quotient(total + gridDim.x - 1, gridDim.x), first = share * blockIdx.x;
   *count = (int)min(share, total - first);
@@ -149,13 +147,14 @@ __device__ inline Place my_share(const Args& a, int* count) {
   return p;
 }
 
-// A share as its pieces of items, the same walk in every role.
+// A share as its pieces of items, the same walk in every role; made by a converged warp and uniform as the compiler sees
+// it, so that loops over it are.
 struct Walk {
   const Args& a;
   int per, item, tile, left;
   int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
   __device__ Walk(const Args& a_, const Place& p, int count)
-      : a(a_), per(items_per_bh(a_)), item(p.item), tile(p.tile), left(count) {}
+      : a(a_), per(items_per_bh(a_)), item(tc::uniform(p.item)), tile(tc::uniform(p.tile)), left(tc::uniform(max(count, 0))) {}
   // accumulators of 128 rows that the item needs
   __device__ int halves() const { return rows_of(a) - it * ROWS > ROWS / 2 ? 2 : 1; }
   __device__ bool next() {
@@ -173,6 +172,24 @@ struct Walk {
     return true;
   }
 };
+
+// Where every bh is one item of the same length (known here): cuts the line for at most `most` CTAs and returns their
+// number; else leaves it to the device and returns `most`.  Either the items follow each other, and a CTA may have
+// pieces of two, or each has k CTAs of its own; beginning and ending a piece takes as long as `piece` tiles.
+inline int plan_shares(Args& a, int most, int piece) {
+  if (a.end_dev || a.G * a.T > ROWS) return most;
+  const int64_t items = (int64_t)a.B * a.Hkv, nt = a.end > TILE ? cdiv(a.end, TILE) : 1;
+  if (items > most) {
+    a.share = (int)cdiv(items * nt, most);
+    a.stride = (int)nt;
+    return (int)cdiv(items * nt, a.share);
+  }
+  const int64_t k = most / items < nt ? most / items : nt, own = cdiv(nt, k), dense = cdiv(items * nt, most);
+  const bool apart = own <= dense + piece;
+  a.share = (int)(apart ? own : dense);
+  a.stride = (int)(apart ? own * k : nt);
+  return (int)cdiv(items * a.stride, a.share);
+}
 
 // Lets `kernel` use `smem` bytes of dynamic shared memory on the current device; done: one bit per device that has been told.
 template <typename K> int allow_smem(K kernel, int smem, std::atomic<uint64_t>& done) {

@@ -21,9 +21,7 @@
 //
 // Work: the tiles of all (bh, 256 rows) items in a line, cut into equal contiguous shares, one per CTA; an item cut
 // by a share's end leaves parts in the workspace, which a second kernel joins in a fixed order.
-#include "kv8.cuh"
 #include "kv8_line.cuh"
-#include "tc.cuh"
 
 namespace fathom {
 namespace kv8 {
@@ -39,6 +37,7 @@ constexpr float HEAD = 8.0f;                 // weights at the reference are 2^8
 // registers per thread of the softmax, value and other warps: together no more than the 768 * 80 of the launch
 constexpr int REG_LAUNCH = 80, REG_SOFT = 88, REG_VALUE = 64, REG_OTHER = 64;
 static_assert(4 * REG_SOFT + REG_VALUE + REG_OTHER <= 6 * REG_LAUNCH, "register split");
+constexpr int PIECE = 4;                     // tiles (~1.7 us each) that beginning and ending a piece takes
 constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
 
 template <int QT> struct Shape {
@@ -83,7 +82,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
   __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];         // tokens whose value holds a NaN (tiles whose mask differs by row)
-  __shared__ float s_pair[2][2][HALF];             // what the two threads of a row tell each other
+  __shared__ int s_ev[VSTAGES];                    // log2 of the largest value scale of the stage's sequence
+  __shared__ float s_rs[2][HALF];                  // scale of a row's scores: 2^e log2(e) / sqrt(128)
+  __shared__ float s_pair[2 * SOFT];               // by thread: what the two threads of a row (tid, tid ^ HALF) tell each other
   const uint32_t bar = tc::smem_u32(bars);
   auto k_full = [&](uint32_t i) { return bar + 8 * (i % KSTAGES); };
   auto k_free = [&](uint32_t i) { return bar + 8 * (KSTAGES + i % KSTAGES); };
@@ -123,8 +124,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     const int pair_bar = 1 + h2 * 4 + (warp & 3);  // the two warps of 32 rows
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tm_s = tm + h2 * 128 + 64 * ch + my, tm_o = tm + 256 + h2 * 128 + 64 * ch + my;
-    uint8_t* sq = smem + S::Q + h2 * QT * HALF * D + r * D;
-    float *s_mine = &s_pair[h2][ch][r], *s_other = &s_pair[h2][ch ^ 1][r];
     uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
     while (w.next()) {
@@ -133,46 +132,46 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         continue;
       }
       const int total = rows_of(a), row = w.it * ROWS + h2 * HALF + r;
-      const bool idle = row - lane >= total;       // no row in this warp: it only keeps the barriers going
+      // no row in this warp: it only keeps the barriers going (uniform as the compiler sees it, or the loop below loses 4%)
+      const bool idle = w.it * ROWS + h2 * HALF + (warp & 3) * 32 >= total;
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
-      // the row's query as e4m3 terms of its own scale: this thread's 64 dims
-      float rs = 0.0f;
-      if (!idle) {
-        const T* qp = reinterpret_cast<const T*>(a.q) + w.b * a.qb + hq * a.qh + tt * a.qt + 64 * ch;
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * i);
-          const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(to_f32(e[j])) & 0x7FFFFFFFu);
-        }
-        *s_mine = __uint_as_float(top);
-        tc::named_sync(pair_bar, 64);
-        top = max(top, __float_as_uint(*s_other));
-        const int e2 = kv8_exponent(top);
-        const float inv = top < 0x7F800000u ? pow2i(-e2) : __uint_as_float(0x7FFFFFFFu);   // a row with inf or NaN is NaN
-        rs = pow2i(e2) * QSCALE;
+      // the half's queries as e4m3 terms of their own scales: a warp takes every eighth row, 4 rows at a time, a lane 4 dims
+      const int first = w.it * ROWS + h2 * HALF, rows = min(HALF, total - first);
 #pragma unroll 1                                   // run once a piece: small code over fast code
-        for (int c = 0; c < 8; ++c) {              // 8 dims a time, read again from the caches
-          const uint4 v = *reinterpret_cast<const uint4*>(qp + 8 * c);
-          const T* e = reinterpret_cast<const T*>(&v);
-          float2 x[4];
+      for (int r0 = warp & 7; r0 < rows; r0 += 32) {
+        uint2 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = make_float2(to_f32(e[2 * j]) * inv, to_f32(e[2 * j + 1]) * inv);
+        for (int i = 0; i < 4; ++i) {
+          const int rw = first + min(r0 + 8 * i, rows - 1), tk = rw / a.G;
+          v[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(a.q) + w.b * a.qb +
+                                                 (int64_t)((w.bh % a.Hkv) * a.G + rw - tk * a.G) * a.qh + tk * a.qt + 4 * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rl = r0 + 8 * i;
+          if (rl >= rows) break;
+          const T* e = reinterpret_cast<const T*>(&v[i]);
+          float2 x[2] = {make_float2(to_f32(e[0]), to_f32(e[1])), make_float2(to_f32(e[2]), to_f32(e[3]))};
+          uint32_t top = __float_as_uint(fmaxf(fmaxf(fabsf(x[0].x), fabsf(x[0].y)), fmaxf(fabsf(x[1].x), fabsf(x[1].y))));
+          top = __reduce_max_sync(0xffffffffu, top);
+          const int e2 = kv8_exponent(top);
+          const float inv = top < 0x7F800000u ? pow2i(-e2) : __uint_as_float(0x7FFFFFFFu);   // a row with an infinity is NaN
+          if (lane == 0) s_rs[h2][rl] = pow2i(e2) * QSCALE;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) x[k] = make_float2(x[k].x * inv, x[k].y * inv);
 #pragma unroll
           for (int term = 0; term < QT; ++term) {
-            uint32_t code[4];
+            uint32_t code[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              code[j] = __nv_cvt_float2_to_fp8x2(x[j], __NV_SATFINITE, __NV_E4M3);
-              const float2 d = kv8_decode2(code[j]);
-              x[j] = make_float2(x[j].x - d.x, x[j].y - d.y);
+            for (int k = 0; k < 2; ++k) {
+              code[k] = __nv_cvt_float2_to_fp8x2(x[k], __NV_SATFINITE, __NV_E4M3);
+              const float2 d = kv8_decode2(code[k]);
+              x[k] = make_float2(x[k].x - d.x, x[k].y - d.y);
             }
-            *reinterpret_cast<uint2*>(sq + term * HALF * D + (((4 * ch + (c >> 1)) ^ (r & 7)) << 4) + (c & 1) * 8) =
-                make_uint2(code[0] | code[1] << 16, code[2] | code[3] << 16);
+            *reinterpret_cast<uint32_t*>(smem + S::Q + (h2 * QT + term) * HALF * D + rl * D +
+                                         (((lane >> 2) ^ (rl & 7)) << 4) + (lane & 3) * 4) = code[0] | code[1] << 16;
           }
         }
       }
@@ -180,26 +179,35 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       tc::fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(q_full(h2));
+      tc::named_sync(9 + h2, SOFT);                // the scales are there
+      const float rs = s_rs[h2][r];
       // keys that every row of the CTA sees need no mask
       const int all_see = seen(a, w.end, w.it * ROWS);
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
-      const int ev = largest_ev(sc, w.end);
+      if (idle) {                                  // weights of rows that no one reads may be anything
+        for (int j = w.j0; j <= w.j1; ++j) {
+          ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);
+          ++phase;
+          __syncwarp();
+          if (j < w.j1 && lane == 0) tc::mbar_arrive(p_full(h2));
+        }
+        vt += w.j1 - w.j0;
+        continue;
+      }
+      ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
+      const int ev = s_ev[vt % VSTAGES];           // log2 of the sequence's largest value scale: comes with the first values
       float m = -INFINITY, l = 0.0f;               // m is the same in both threads of a row, l is this thread's share
       for (int j = w.j0; j < w.j1; ++j, ++vt) {
         const int blk = j * (TILE / BLK) + ch;
         const float2 s2 = blk < a.cap / BLK ? sc[blk] : make_float2(0.0f, 0.0f);
         // above 0, so that a masked score stays -inf; void blocks may hold anything, NaN too
         const float cs = fmaxf(s2.x * rs, 1e-37f);
-        const int evb = weight_ev(s2.y, ev);
-        const float es = (float)evb;
         ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);
         ++phase;
         __syncwarp();
         tc::fence_after();
-        if (idle) {                                // weights of rows that no one reads may be anything
-          if (lane == 0) tc::mbar_arrive(p_full(h2));
-          continue;
-        }
+        const int evb = weight_ev(s2.y, ev);
+        const float es = (float)evb;
         int see = BLK;                             // tokens of the block that this row sees
         const bool masked = (j + 1) * TILE > all_see;
         if (masked) {
@@ -229,9 +237,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         }
         float top = fmaf(fmaxf(t0, t1), cs, es);
         if (tc::named_or(pair_bar, 64, top > m + SLACK)) {        // also the first time: m = -inf
-          *s_mine = top;
+          s_pair[tid] = top;
           tc::named_sync(pair_bar, 64);
-          top = fmaxf(top, *s_other);
+          top = fmaxf(top, s_pair[tid ^ HALF]);
           tc::named_sync(pair_bar, 64);
           const bool up = top > m + SLACK;
           const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
@@ -284,11 +292,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       }
       ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);      // the piece's last product
       ++phase;
-      if (idle) continue;
       __syncwarp();
-      *s_mine = l;
+      s_pair[tid] = l;
       tc::named_sync(pair_bar, 64);
-      l += *s_other;
+      l += s_pair[tid ^ HALF];
       tc::fence_after();
       const bool whole = w.j0 == 0 && w.j1 == w.n;
       const float vscale = pow2i(ev);              // the denominator is relative to the largest scale
@@ -350,6 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         ok = ok && tc::mbar_wait(v_free(i), ((i / VSTAGES) & 1) ^ 1, gave_up);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        if (t == 0) s_ev[i % VSTAGES] = ev;
         uint8_t* vb = smem + S::V + (i % VSTAGES) * VBYTES + (u >> 2) * (TILE * 128);
         const bool differs = (j + 1) * TILE > all_see;
 #pragma unroll
@@ -506,17 +514,24 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args
   __shared__ Place s_place;
   __shared__ int64_t s_total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = items_per_bh(a);
-  if (warp == 0) {
+  if (!a.share && warp == 0) {
     Place p{0, 0};
-    const int64_t total = line(a, -1, &p), share = (total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
+    const int64_t total = line(a, -1, &p), cut = quotient(total + ctas - 1, ctas) * (blockIdx.x + 1);
     if (cut < total) line(a, cut, &p);
     if (lane == 0) s_place = p, s_total = total;
   }
   __syncthreads();
-  const Place p = s_place;
-  const int64_t share = (s_total + ctas - 1) / ctas, cut = share * (blockIdx.x + 1);
+  Place p = s_place;
+  int64_t share = a.share, cut = share * (blockIdx.x + 1), length = (int64_t)a.B * a.Hkv * a.stride;
+  if (a.share) {
+    p.item = (int)quotient(cut, a.stride);
+    p.tile = (int)(cut - (int64_t)p.item * a.stride);
+    if (p.tile >= tiles_of(a, seq_end(a, 0), 0)) p.tile = 0;        // between two items
+  } else {
+    length = s_total, share = quotient(length + ctas - 1, ctas), cut = share * (blockIdx.x + 1);
+  }
   tc::wait_dependency();                           // the parts are written; and nothing ends before they are
-  if (cut >= s_total || p.tile == 0 || p.tile > share) return;    // no item is cut here, or an earlier cut joins it
+  if (cut >= length || p.tile == 0 || p.tile > share) return;    // no item is cut here, or an earlier cut joins it
   const int bh = p.item / per, it = p.item % per, b = bh / a.Hkv, total = rows_of(a);
   const int64_t first = cut - p.tile;              // the item's first tile in the line
   const int c0 = blockIdx.x, c1 = (int)((first + tiles_of(a, seq_end(a, b), it) - 1) / share);
@@ -548,7 +563,7 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
   const int r = allow_smem(prompt_kernel<T, QT>, S::SMEM, told);
   if (r != FATHOM_OK) return r;
   prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (ctas == 1) return check_launch("kv8_attend");
+  if (ctas == 1 || (a.share && a.share == a.stride)) return check_launch("kv8_attend");   // no item is cut
   const int rows = a.G * a.T < ROWS ? (int)(a.G * a.T) : ROWS;
   return launch_join(prompt_join_kernel<T>, dim3(ctas - 1, (rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, a, ctas, st);
 }
@@ -557,8 +572,8 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
 
 size_t prompt_workspace() { return (size_t)sm_count() * 2 * ROWS * PART * sizeof(float); }
 
-int prompt_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st) {
-  const int ctas = sm_count();
+int prompt_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st) {
+  const int ctas = plan_shares(a, sm_count(), PIECE);
   return dtype == FATHOM_DTYPE_BF16 ? launch<__nv_bfloat16, 2>(map, a, ctas, st) : launch<__half, 3>(map, a, ctas, st);
 }
 

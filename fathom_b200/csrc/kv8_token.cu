@@ -21,7 +21,6 @@
 //
 // A row's parts in different CTAs (kv8_line.cuh) are joined by a second kernel in a fixed order.
 #include "kv8_line.cuh"
-#include "tc.cuh"
 
 namespace fathom {
 namespace kv8 {
@@ -34,6 +33,8 @@ constexpr int STAGE_BYTES = 2 * TILE * D;        // key tile, value tile
 constexpr int STAGES = 6;
 constexpr float SLACK = 6.0f;                    // a tile may exceed the reference by 2^6
 constexpr float HEAD = 2.0f;                     // weights at the reference are 4: 2^(HEAD + SLACK) = 256 <= 448
+constexpr int PIECE = 6;                         // tiles (~0.4 us each) that beginning and ending a piece takes: ~2.5 us
+constexpr int SHORT = 8;                         // tiles that take less than the second kernel (~4 us)
 constexpr int MAX_CTAS = 512;                    // shares that the join kernel has room for
 
 constexpr int up16(int n) { return (n + 15) / 16 * 16; }
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
         for (int r = 0; r < NR; ++r) above = above || s[r] + lv > m[r] + SLACK;
         if (tc::named_or(1 + g, GROUP, above)) {
-          bad = tc::named_or(1 + g, GROUP, !ok);
+          bad = tc::uniform(tc::named_or(1 + g, GROUP, !ok));
           // some row outgrew its reference: the tile's largest becomes every row's
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
         if (t == 0) s_m[g][r] = m[r];
       }
       tc::fence_before();
-      bad = tc::named_or(3, 2 * GROUP, !ok);
+      bad = tc::uniform(tc::named_or(3, 2 * GROUP, !ok));
       tc::fence_after();
       const Walk now = w;
       more = w.next();
@@ -477,28 +478,25 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   const int R = rows_of(a), tid = threadIdx.x, lane = tid & 31;
   const int bh = blockIdx.x / R, r = blockIdx.x % R, b = bh / a.Hkv, h = bh % a.Hkv;
   const int nt = tiles_of(a, seq_end(a, b), 0);
-  if (tid < 32) {
+  if (a.end_dev && tid < 32) {
     // tiles of the sequences before b, and of all
     int64_t before = 0, total = 0;
-    if (!a.end_dev) {
-      before = (int64_t)nt * a.Hkv * b, total = (int64_t)nt * a.Hkv * a.B;
-    } else {
-      for (int j = tid; j < a.B; j += 32) {
-        const int64_t x = (int64_t)tiles_of(a, seq_end(a, j), 0) * a.Hkv;
-        total += x;
-        if (j < b) before += x;
-      }
+    for (int j = tid; j < a.B; j += 32) {
+      const int64_t x = (int64_t)tiles_of(a, seq_end(a, j), 0) * a.Hkv;
+      total += x;
+      if (j < b) before += x;
+    }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-      }
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     if (tid == 0) s_before = before, s_total = total;
   }
   __syncthreads();
-  const int64_t share = (s_total + ctas - 1) / ctas, first = s_before + (int64_t)h * nt;
-  const int c0 = (int)(first / share), n = (int)((first + nt - 1) / share) - c0 + 1;
+  const int64_t share = a.share ? a.share : quotient(s_total + ctas - 1, ctas);
+  const int64_t first = a.share ? (int64_t)bh * a.stride : s_before + (int64_t)h * nt;
+  const int c0 = (int)quotient(first, (int)share), n = (int)quotient(first + nt - 1, (int)share) - c0 + 1;
   tc::wait_dependency();                          // the parts are written; and nothing ends before they are
   if (n == 1) return;
   const float* part = a.part + ((int64_t)(c0 + bh) * R + r) * PART;
@@ -526,9 +524,6 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
 
-// Short rows of a known length have a CTA each: up to 8 tiles, ~0.5 us apiece, take less than the second kernel.
-bool whole_rows(const Args& a) { return !a.end_dev && a.end <= 8 * TILE; }
-
 template <typename T, int NR, int QT>
 int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   using S = Shape<NR, QT>;
@@ -537,7 +532,7 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   const int r = allow_smem(token_kernel<T, NR, QT>, S::SMEM, told);
   if (r != FATHOM_OK) return r;
   token_kernel<T, NR, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (whole_rows(a)) return check_launch("kv8_attend");      // nothing to join
+  if (a.share && a.share == a.stride) return check_launch("kv8_attend");     // every row whole: nothing to join
   return launch_join(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, a, ctas, st);
 }
 
@@ -549,21 +544,24 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   return launch<T, 16, QT>(map, a, ctas, st);
 }
 
-int token_launch(const CUtensorMap& map, const Args& a, int dtype, int ctas, cudaStream_t st) {
-  return dtype == FATHOM_DTYPE_BF16 ? launch_rows<__nv_bfloat16, 2>(map, a, ctas, st)
-                                    : launch_rows<__half, 3>(map, a, ctas, st);
-}
-
 }  // namespace
 
 size_t token_workspace(int64_t BH, int64_t R) { return (size_t)((sm_count() + BH) * R * PART * sizeof(float)); }
 
-int token_attend(const CUtensorMap& map, const Args& a, int dtype, cudaStream_t st) {
+int token_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st) {
   // one CTA per SM, but no more than there can be tiles
-  if (whole_rows(a)) return token_launch(map, a, dtype, a.B * a.Hkv, st);
-  const int64_t per = cdiv(a.end_dev ? a.cap : a.end, TILE), most = (int64_t)a.B * a.Hkv * (per > 1 ? per : 1);
+  const int64_t per = cdiv(a.end_dev ? a.cap : a.end, TILE), items = (int64_t)a.B * a.Hkv, tiles = items * (per > 1 ? per : 1);
   const int64_t sms = sm_count() < MAX_CTAS ? sm_count() : MAX_CTAS;
-  return token_launch(map, a, dtype, (int)(most < sms ? most : sms), st);
+  int ctas = (int)(tiles < sms ? tiles : sms);
+  if (!a.end_dev && per <= SHORT) {
+    // each row whole in one CTA
+    a.share = a.stride = (int)(per > 1 ? per : 1);
+    ctas = (int)items;
+  } else {
+    ctas = plan_shares(a, ctas, PIECE);
+  }
+  return dtype == FATHOM_DTYPE_BF16 ? launch_rows<__nv_bfloat16, 2>(map, a, ctas, st)
+                                    : launch_rows<__half, 3>(map, a, ctas, st);
 }
 
 }  // namespace kv8

@@ -58,7 +58,7 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 // A value that is the same in the whole warp, as the compiler can see.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 
 // ---- proxies -------------------------------------------------------------------------------------
 // Orders this thread's shared-memory writes before later reads by the tensor cores and TMA.
