@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 namespace fathom {
 namespace kv8 {
 
@@ -48,6 +50,18 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Lets `kernel` use `smem` bytes of dynamic shared memory on the current device; done: one bit per device that has been told.
+template <typename K> int allow_smem(K kernel, int smem, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return FATHOM_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return FATHOM_OK;
 }
 
 int sm_count();

@@ -8,8 +8,6 @@
 #include "kv8_attn.cuh"
 #include "tc.cuh"
 
-#include <atomic>
-
 namespace fathom {
 namespace kv8 {
 
@@ -189,18 +187,6 @@ inline int plan_shares(Args& a, int most, int piece) {
   a.share = (int)(apart ? own : dense);
   a.stride = (int)(apart ? own * k : nt);
   return (int)cdiv(items * a.stride, a.share);
-}
-
-// Lets `kernel` use `smem` bytes of dynamic shared memory on the current device; done: one bit per device that has been told.
-template <typename K> int allow_smem(K kernel, int smem, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (e == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return FATHOM_OK;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
-  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return FATHOM_OK;
 }
 
 // Launches the kernel that joins the parts of cut items; it may start while the kernel before still runs, and waits for it.

@@ -1,0 +1,349 @@
+// Attention over listed rows of the 8-bit cache (layout in kv8.cuh), one list per query head.
+//
+// Bound by the rows' bytes, 256 at random addresses per pick, and for one sequence by latency.  A warp takes 16 picks at a
+// time; their rows come into shared memory by 16-byte asynchronous copies, STAGES - 1 chunks ahead, so ~100 KB are on
+// their way per SM whatever the warps wait for.  With one query row per list a product has nothing to share, but
+// dequantising and multiplying on the fp32 pipes took ~290 instructions per 4 picks; as fragments of 16-bit matrix
+// instructions (an e4m3 is exact in f16) it is ~190 per 16:
+//
+//   scores   [16 picks x 8] = K [16 x 128] q^T          columns: q as a sum of three f16 terms (33 bits)
+//   output^T [128 dims x 8] += V^T [128 x 16 picks] p   columns: the weights as two f16 terms (22 bits)
+//
+// The order of dims within a score, and of picks within a sum, is free, so a lane's fragments are 16-byte pieces of rows as
+// they lie: K piece j and j + 4 of picks g and g + 8, V piece g of picks 2j, 2j + 1, 2j + 8, 2j + 9 (lane = 4 g + j).
+// Softmax state per warp, in fp32 as in kv8_token.cu: references of s + log2(value scale) for the output and of s for
+// the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their states are joined in warp
+// order in the first CTA's shared memory.
+#include "kv8_attn.cuh"
+
+#include <cooperative_groups.h>
+
+namespace fathom {
+namespace kv8 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int PW = 4;                    // warps per CTA
+constexpr int CHUNK = 16;                // picks per step of a warp
+constexpr int STAGES = 3;
+constexpr int CTAS_PER_SM = 4;           // 4 x 52 KB of shared memory, 4 x 128 threads of 128 registers
+constexpr float SLACK = 6.0f;            // a chunk may exceed the reference by 2^6
+constexpr float HEAD = 8.0f;             // weights at the reference are 2^8: f16 from 2^-24 to 2^15
+
+struct PicksArgs {
+  const int64_t* idx;        // [BH*G][k]
+  const int32_t* slot;       // [BH*G][k] row of `rows` that holds the pick, -1: none; NULL: the pick itself
+  int64_t k;
+  const uint8_t* rows;       // [BH][row_cap][256]
+  int64_t row_cap;
+  const float* scales;
+  int64_t cap, end;
+  const int64_t* end_dev;
+  int Hkv, G;
+};
+
+struct alignas(16) Stage {
+  uint8_t row[CHUNK][KV8_ROW];           // 16-byte pieces permuted within each half (piece_of)
+  float2 scale[CHUNK];
+  int valid[CHUNK];
+};
+
+// Where piece c (0..7) of a row's key or value half lies, so that the 8 lanes of a shared-memory phase meet 8 banks groups:
+// keys are read as 2 rows x 4 pieces, values as 4 even or odd rows x 2 pieces.
+__device__ __forceinline__ int piece_of(int row, int which, int c) {
+  return which ? c ^ (row & 7) : c ^ ((row & 1) << 2 | (row >> 1 & 3));
+}
+
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {     // zeros where there is no row
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t half2_of(uint32_t codes) {       // two codes in the low 16 bits
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), __NV_E4M3);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+__device__ __forceinline__ float element(const void* p, int dtype, int64_t i) {
+  if (dtype == FATHOM_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == FATHOM_DTYPE_BF16) return to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return to_f32(reinterpret_cast<const __half*>(p)[i]);
+}
+
+template <int CS>
+__global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a,
+                                                                   void* __restrict__ out) {
+  constexpr int NW = PW * CS;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ float s_m[NW], s_lm[NW], s_l[NW];         // the cluster's first CTA: every warp's state
+  __shared__ __align__(16) float s_acc[NW][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
+  Stage* st = reinterpret_cast<Stage*>(smem_raw) + warp * STAGES;
+  const unsigned crank = CS == 1 ? 0u : cg::this_cluster().block_rank();
+  if constexpr (CS > 1) cg::this_cluster().barrier_arrive();     // waited for before the first store into another CTA
+  const int64_t bhg = blockIdx.x / CS;
+  const int bh = (int)(bhg / a.G), gw = (int)crank * PW + warp;
+  int64_t end = a.end_dev ? a.end_dev[bh / a.Hkv] : a.end;
+  if (end > a.cap) end = a.cap;
+  const uint8_t* base = a.rows + (int64_t)bh * a.row_cap * KV8_ROW;
+  const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)bh * (a.cap / BLK);
+  const int64_t chunks = (a.k + CHUNK - 1) / CHUNK;
+  const int n = chunks > gw ? (int)((chunks - gw + NW - 1) / NW) : 0;      // this warp's: gw, gw + NW, ..
+
+  // lanes 0..15: the chunk's picks and the rows that hold them
+  auto pick = [&](int i, int64_t& tok, int& row) {
+    const int64_t p = ((int64_t)i * NW + gw) * CHUNK + lane;
+    tok = -1;
+    row = -1;
+    if (i < n && lane < CHUNK && p < a.k) {
+      tok = a.idx[bhg * a.k + p];
+      if (tok >= 0 && tok < end) row = a.slot ? a.slot[bhg * a.k + p] : (int)tok;
+    }
+  };
+  auto bring = [&](int i, int64_t tok, int row) {
+    Stage& s = st[i % STAGES];
+    if (i < n) {
+      if (lane < CHUNK) {
+        s.valid[lane] = row;
+        if (row >= 0) copy8(&s.scale[lane], sc + tok / BLK);
+      }
+#pragma unroll
+      for (int u = 0; u < CHUNK / 2; ++u) {
+        const int r = 2 * u + (lane >> 4), c = lane & 15;
+        const int from = __shfl_sync(0xffffffffu, row, r);
+        copy16(&s.row[r][(c & 8) * 16 + piece_of(r, c >> 3, c & 7) * 16], base + (int64_t)max(from, 0) * KV8_ROW + c * 16, from >= 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+  int64_t tok;
+  int row;
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    pick(i, tok, row);
+    bring(i, tok, row);
+  }
+  pick(STAGES - 1, tok, row);
+
+  // q: this lane's dims, 16 j .. and 64 + 16 j .., of term g (0, 1, 2; zeros for the others)
+  uint32_t qf[16];
+  float rs;
+  {
+    float x[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      x[i] = element(q, dtype, bhg * D + (i < 16 ? 16 * j + i : 48 + 16 * j + i));
+      top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int e = kv8_exponent(top);
+    const float inv = top < 0x7F800000u ? pow2i(-e) : __uint_as_float(0x7FFFFFFFu);   // a row with inf or NaN is NaN
+    rs = pow2i(e) * QSCALE;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float2 y = make_float2(x[2 * i] * inv, x[2 * i + 1] * inv);
+      __half2 h = __floats2half2_rn(y.x, y.y);
+      for (int t = 0; t < g && t < 2; ++t) {           // what the terms before left
+        const float2 f = __half22float2(h);
+        y = make_float2(y.x - f.x, y.y - f.y);
+        h = __floats2half2_rn(y.x, y.y);
+      }
+      qf[i] = g < 3 ? bits(h) : 0u;
+    }
+  }
+
+  float acc[8][4];                                     // dims 16 g + 2 t and + 1; columns 2 j, 2 j + 1
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
+  float m = -INFINITY, lm = -1e30f, l = 0.0f;          // m is the warp's; l is of picks g and g + 8 of its chunks
+  for (int i = 0; i < n; ++i) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();                                      // chunk i is there; chunk i - 1 has been read
+    bring(i + STAGES - 1, tok, row);
+    pick(i + STAGES, tok, row);
+    const Stage& s = st[i % STAGES];
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(&s.row[g][piece_of(g, 0, j + 4 * h) * 16]);
+      const uint4 hi = *reinterpret_cast<const uint4*>(&s.row[g + 8][piece_of(g + 8, 0, j + 4 * h) * 16]);
+      const uint32_t x[4] = {lo.x, lo.y, lo.z, lo.w}, y[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        mma(c, half2_of(x[w]), half2_of(y[w]), half2_of(x[w] >> 16), half2_of(y[w] >> 16), qf[8 * h + 2 * w], qf[8 * h + 2 * w + 1]);
+    }
+    // scores of picks g and g + 8: the sum of their columns, 2 of them in each lane of a quad
+    float v[2] = {c[0] + c[1], c[2] + c[3]}, lv[2], w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
+      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
+      const int r = g + 8 * e;
+      const bool there = s.valid[r] >= 0;
+      const float2 ks = there ? s.scale[r] : make_float2(0.0f, 1.0f);
+      v[e] = there ? v[e] * (ks.x * rs) : -INFINITY;
+      lv[e] = (float)((int)(__float_as_uint(ks.y) >> 23) - 127);
+    }
+    float top = fmaxf(v[0] + lv[0], v[1] + lv[1]);
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top > m + SLACK) {                             // the same in every lane; also the first time: m = -inf
+      const float f = m == -INFINITY ? 0.0f : ex2(m - top);
+      m = top;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][e] *= f;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w[e] = m == -INFINITY && !(v[e] != v[e]) ? 0.0f : ex2(v[e] + (lv[e] - m + HEAD));
+      const float d = v[e] - lm, p = ex2(-fabsf(d));
+      l = d > 0.0f ? fmaf(l, p, 1.0f) : l + p;
+      lm = fmaxf(lm, v[e]);
+    }
+    // weights of picks 2 j, 2 j + 1 and 2 j + 8, 2 j + 9 as term g
+    uint32_t b[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = __shfl_sync(0xffffffffu, w[e], 8 * j), y = __shfl_sync(0xffffffffu, w[e], 8 * j + 4);
+      const __half2 hi = __floats2half2_rn(x, y);
+      const float2 f = __half22float2(hi);
+      b[e] = g == 0 ? bits(hi) : g == 1 ? bits(__floats2half2_rn(x - f.x, y - f.y)) : 0u;
+    }
+    uint32_t x[4][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = 2 * j + (e & 1) + (e & 2) * 4;
+      const uint4 y = *reinterpret_cast<const uint4*>(&s.row[r][D + piece_of(r, 1, g) * 16]);
+      x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                    // bytes 4 u + 2 h and + 1 of two picks side by side
+        const uint32_t s01 = __byte_perm(x[0][u], x[1][u], h ? 0x7362 : 0x5140);
+        const uint32_t s89 = __byte_perm(x[2][u], x[3][u], h ? 0x7362 : 0x5140);
+        mma(acc[2 * u + h], half2_of(s01), half2_of(s01 >> 16), half2_of(s89), half2_of(s89 >> 16), b[0], b[1]);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+  // the warp's state: picks are spread over g
+  const float all = fmaxf(fmaxf(lm, __shfl_xor_sync(0xffffffffu, lm, 4)), -1e30f);
+  float ref = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, 8));
+  ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, 16));
+  l *= ex2(lm - ref);
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  float *dm = s_m, *dlm = s_lm, *dl = s_l, *da = &s_acc[0][0];
+  if constexpr (CS > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_wait();
+    dm = cluster.map_shared_rank(s_m, 0);
+    dlm = cluster.map_shared_rank(s_lm, 0);
+    dl = cluster.map_shared_rank(s_l, 0);
+    da = cluster.map_shared_rank(&s_acc[0][0], 0);
+  }
+  if (lane == 0) dm[gw] = m, dlm[gw] = ref, dl[gw] = l;
+  if (j == 0) {                                        // columns 0 and 1: the two terms' sums
+    float4* dst = reinterpret_cast<float4*>(da + gw * D + 16 * g);
+#pragma unroll
+    for (int t = 0; t < 8; t += 2)
+      dst[t / 2] = make_float4(acc[t][0] + acc[t][1], acc[t][2] + acc[t][3], acc[t + 1][0] + acc[t + 1][1],
+                               acc[t + 1][2] + acc[t + 1][3]);
+  }
+  if constexpr (CS == 1) __syncthreads();
+  else cg::this_cluster().sync();
+  if (crank != 0) return;
+  float M = -1e30f, L = 0.0f, O = 0.0f;
+#pragma unroll 8
+  for (int v = 0; v < NW; ++v) M = fmaxf(M, s_lm[v]);
+#pragma unroll 8
+  for (int v = 0; v < NW; ++v) {
+    L = fmaf(s_l[v], ex2(s_lm[v] - M), L);
+    if (s_m[v] != -INFINITY) O = fmaf(s_acc[v][threadIdx.x], exp2f(s_m[v] - HEAD - M), O);
+  }
+  const float o = L == 0.0f ? 0.0f : O / L;
+  const int64_t at = bhg * D + threadIdx.x;
+  if (dtype == FATHOM_DTYPE_F32) from_f32(o, reinterpret_cast<float*>(out) + at);
+  else if (dtype == FATHOM_DTYPE_BF16) from_f32(o, reinterpret_cast<__nv_bfloat16*>(out) + at);
+  else from_f32(o, reinterpret_cast<__half*>(out) + at);
+}
+
+template <int CS> int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, void* out, cudaStream_t st) {
+  constexpr int smem = PW * STAGES * (int)sizeof(Stage);
+  static std::atomic<uint64_t> told{0};
+  const int r = allow_smem(picks_kernel<CS>, smem, told, "kv8_attend_picks");
+  if (r != FATHOM_OK) return r;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(heads * CS));
+  cfg.blockDim = dim3(PW * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CS;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CS > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, picks_kernel<CS>, q, dtype, a, out);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend_picks: launch: %s", cudaGetErrorString(e));
+  return check_launch("kv8_attend_picks");
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace kv8
+}  // namespace fathom
+
+using namespace fathom;
+using namespace fathom::kv8;
+
+extern "C" size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k) {
+  if (B <= 0 || Hkv <= 0 || G <= 0 || k <= 0) return 0;
+  return 256;
+}
+
+extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int64_t Hkv, int G, const int64_t* idx,
+                                       int64_t k, const uint8_t* rows, const float* scales, int64_t cap, int64_t end,
+                                       const int64_t* end_dev, void* out, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  FATHOM_REQUIRE(q && idx && rows && scales && out && workspace, FATHOM_ERR_NULL, "kv8_attend_picks: NULL pointer");
+  FATHOM_REQUIRE(dtype >= FATHOM_DTYPE_F32 && dtype <= FATHOM_DTYPE_F16, FATHOM_ERR_UNSUPPORTED,
+                 "kv8_attend_picks: queries must be fp32, bf16 or fp16");
+  FATHOM_REQUIRE(B >= 1 && Hkv >= 1 && B <= 65535 && Hkv <= 65535 && B * Hkv <= 65535 && G >= 1 && G <= 65535 &&
+                     B * Hkv * G <= INT32_MAX / 8 && k >= 1 && k <= INT32_MAX && cap >= BLK && cap % BLK == 0 &&
+                     cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE, "kv8_attend_picks: bad shape");
+  FATHOM_REQUIRE(end_dev || (end >= 0 && end <= cap), FATHOM_ERR_SHAPE,
+                 "kv8_attend_picks: end %lld is outside the cache's %lld", (long long)end, (long long)cap);
+  FATHOM_REQUIRE(aligned16(rows) && aligned16(q) && aligned16(out), FATHOM_ERR_SHAPE,
+                 "kv8_attend_picks: rows, q and out must be 16-byte aligned");
+  FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_picks_workspace_bytes(B, Hkv, G, k), FATHOM_ERR_WORKSPACE,
+                 "kv8_attend_picks: workspace too small");
+  const PicksArgs a{idx, nullptr, k, rows, cap, scales, cap, end, end_dev, (int)Hkv, G};
+  const int64_t heads = B * Hkv * G, slots = (int64_t)CTAS_PER_SM * sm_count(), chunks = cdiv(k, CHUNK);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  // as many CTAs per head as fit the GPU at once and have a chunk for every warp
+  if (heads * 8 <= slots && chunks > 4 * PW) return launch_picks<8>(q, dtype, a, heads, out, st);
+  if (heads * 4 <= slots && chunks > 2 * PW) return launch_picks<4>(q, dtype, a, heads, out, st);
+  if (heads * 2 <= slots && chunks > PW) return launch_picks<2>(q, dtype, a, heads, out, st);
+  return launch_picks<1>(q, dtype, a, heads, out, st);
+}

@@ -560,7 +560,7 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
   using S = Shape<QT>;
   static_assert(S::SMEM <= 226 * 1024, "shared memory");
   static std::atomic<uint64_t> told{0};
-  const int r = allow_smem(prompt_kernel<T, QT>, S::SMEM, told);
+  const int r = allow_smem(prompt_kernel<T, QT>, S::SMEM, told, "kv8_attend");
   if (r != FATHOM_OK) return r;
   prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
   if (ctas == 1 || (a.share && a.share == a.stride)) return check_launch("kv8_attend");   // no item is cut

@@ -529,7 +529,7 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   using S = Shape<NR, QT>;
   static_assert(S::SMEM <= 224 * 1024, "shared memory");
   static std::atomic<uint64_t> told{0};
-  const int r = allow_smem(token_kernel<T, NR, QT>, S::SMEM, told);
+  const int r = allow_smem(token_kernel<T, NR, QT>, S::SMEM, told, "kv8_attend");
   if (r != FATHOM_OK) return r;
   token_kernel<T, NR, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
   if (a.share && a.share == a.stride) return check_launch("kv8_attend");     // every row whole: nothing to join
