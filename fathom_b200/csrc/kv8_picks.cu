@@ -18,16 +18,18 @@
 
 #include <cooperative_groups.h>
 
+#include <stddef.h>
+
 namespace fathom {
 namespace kv8 {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int PW = 4;                    // warps per CTA
 constexpr int CHUNK = 16;                // picks per step of a warp
-constexpr int STAGES = 3;
-constexpr int CTAS_PER_SM = 4;           // 4 x 52 KB of shared memory, 4 x 128 threads of 128 registers
+constexpr int STAGES = 2;                // chunks in shared memory: being used, and on its way
+constexpr int WARPS_PER_SM = 16;         // 16 x 2 x 4.3 KB of shared memory, 16 x 32 threads of 128 registers
+constexpr int MAX_CS = 8, MAX_PW = 4;    // CTAs of a cluster, warps of a CTA
 constexpr float SLACK = 6.0f;            // a chunk may exceed the reference by 2^6
 constexpr float HEAD = 8.0f;             // weights at the reference are 2^8: f16 from 2^-24 to 2^15
 
@@ -43,25 +45,22 @@ struct PicksArgs {
   int Hkv, G;
 };
 
-struct alignas(16) Stage {
+struct alignas(128) Stage {              // halves of rows 128-byte aligned: pieces are permuted by XOR on addresses
   uint8_t row[CHUNK][KV8_ROW];           // 16-byte pieces permuted within each half (piece_of)
   float2 scale[CHUNK];
   int valid[CHUNK];
 };
 
-// Where piece c (0..7) of a row's key or value half lies, so that the 8 lanes of a shared-memory phase meet 8 banks groups:
-// keys are read as 2 rows x 4 pieces, values as 4 even or odd rows x 2 pieces.
-__device__ __forceinline__ int piece_of(int row, int which, int c) {
-  return which ? c ^ (row & 7) : c ^ ((row & 1) << 2 | (row >> 1 & 3));
-}
+// Piece c (0..7) of a row's key or value half lies at c ^ permuted(row), so that the 8 lanes of a shared-memory phase meet
+// 8 different bank groups: keys are read as rows 2p, 2p + 1 x 4 pieces, values as 4 even or odd rows x 2 pieces.
+__device__ __forceinline__ int permuted(int row) { return ((row >> 1 & 3) ^ (row & 1) << 1) << 1; }
 
-__device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {     // zeros where there is no row
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
-               "r"(there ? 16 : 0)
-               : "memory");
+// dst: shared-memory addresses; zeros where there is no row.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -76,78 +75,94 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t codes) {       // two code
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
-__device__ __forceinline__ float element(const void* p, int dtype, int64_t i) {
-  if (dtype == FATHOM_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == FATHOM_DTYPE_BF16) return to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return to_f32(reinterpret_cast<const __half*>(p)[i]);
+// 16 consecutive elements of q, 16-byte aligned.
+__device__ __forceinline__ void load16(const void* p, int dtype, int64_t i, float* x) {
+  if (dtype == FATHOM_DTYPE_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<float4*>(x + 4 * e) = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[e];
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint4 v = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i)[e];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float2 f = dtype == FATHOM_DTYPE_BF16
+                           ? make_float2(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u))
+                           : __half22float2(*reinterpret_cast<const __half2*>(&w[u]));
+      x[8 * e + 2 * u] = f.x, x[8 * e + 2 * u + 1] = f.y;
+    }
+  }
 }
 
-template <int CS>
-__global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a,
+__global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW) picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a,
                                                                    void* __restrict__ out) {
-  constexpr int NW = PW * CS;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ float s_m[NW], s_lm[NW], s_l[NW];         // the cluster's first CTA: every warp's state
-  __shared__ __align__(16) float s_acc[NW][D];
+  const int PW = blockDim.x >> 5, NW = PW * (int)gridDim.y;      // one cluster of gridDim.y CTAs per (batch, query head)
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  constexpr int MAX_NW = MAX_PW * MAX_CS;
+  __shared__ float s_m[MAX_NW], s_lm[MAX_NW], s_l[MAX_NW];       // the cluster's first CTA: every warp's state
+  float(*const s_acc)[D] = reinterpret_cast<float(*)[D]>(smem_raw + PW * STAGES * sizeof(Stage));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-  Stage* st = reinterpret_cast<Stage*>(smem_raw) + warp * STAGES;
-  const unsigned crank = CS == 1 ? 0u : cg::this_cluster().block_rank();
-  if constexpr (CS > 1) cg::this_cluster().barrier_arrive();     // waited for before the first store into another CTA
-  const int64_t bhg = blockIdx.x / CS;
-  const int bh = (int)(bhg / a.G), gw = (int)crank * PW + warp;
+  Stage* const st = reinterpret_cast<Stage*>(smem_raw) + warp * STAGES;
+  const unsigned crank = blockIdx.y;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();                            // waited for before the first store into another CTA
+  const int64_t bhg = blockIdx.x;
+  const int bh = (int)bhg / a.G, gw = (int)crank * PW + warp;
   int64_t end = a.end_dev ? a.end_dev[bh / a.Hkv] : a.end;
   if (end > a.cap) end = a.cap;
-  const uint8_t* base = a.rows + (int64_t)bh * a.row_cap * KV8_ROW;
   const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)bh * (a.cap / BLK);
-  const int64_t chunks = (a.k + CHUNK - 1) / CHUNK;
-  const int n = chunks > gw ? (int)((chunks - gw + NW - 1) / NW) : 0;      // this warp's: gw, gw + NW, ..
+  const int k = (int)a.k, chunks = (k + CHUNK - 1) / CHUNK;
+  const int n = chunks > gw ? (chunks - gw + NW - 1) / NW : 0;   // this warp's chunks: gw, gw + NW, ..
 
-  // lanes 0..15: the chunk's picks and the rows that hold them
-  auto pick = [&](int i, int64_t& tok, int& row) {
-    const int64_t p = ((int64_t)i * NW + gw) * CHUNK + lane;
-    tok = -1;
-    row = -1;
-    if (i < n && lane < CHUNK && p < a.k) {
-      tok = a.idx[bhg * a.k + p];
-      if (tok >= 0 && tok < end) row = a.slot ? a.slot[bhg * a.k + p] : (int)tok;
+  // lanes 0..15: the next chunk's picks and the rows that hold them (-1: none)
+  int next = lane < CHUNK ? gw * CHUNK + lane : k;
+  auto pick = [&](int& tok, int& row) {
+    tok = row = -1;
+    if (next < k) {
+      const int64_t t = a.idx[bhg * k + next];
+      if (t >= 0 && t < end) tok = (int)t, row = a.slot ? a.slot[bhg * k + next] : tok;
+      next += NW * CHUNK;
     }
   };
-  auto bring = [&](int i, int64_t tok, int row) {
-    Stage& s = st[i % STAGES];
-    if (i < n) {
-      if (lane < CHUNK) {
-        s.valid[lane] = row;
-        if (row >= 0) copy8(&s.scale[lane], sc + tok / BLK);
-      }
+  // copies of a chunk into stage s: a lane has piece lane & 15 of rows 2 u + (lane >> 4)
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(st);
+  const uint32_t lane_at = (lane >> 4) * KV8_ROW + (lane & 8) * 16 + ((lane & 7) ^ permuted(lane >> 4)) * 16;
+  const uint8_t* const from = a.rows + (int64_t)bh * a.row_cap * KV8_ROW + (lane & 15) * 16;
+  auto bring = [&](int s, int tok, int row) {
+    const uint32_t at = ring + s * (uint32_t)sizeof(Stage);
+    if (lane < CHUNK) {
+      st[s].valid[lane] = row;
+      if (row >= 0) copy8(at + (uint32_t)offsetof(Stage, scale) + lane * 8, sc + tok / BLK);
+    }
 #pragma unroll
-      for (int u = 0; u < CHUNK / 2; ++u) {
-        const int r = 2 * u + (lane >> 4), c = lane & 15;
-        const int from = __shfl_sync(0xffffffffu, row, r);
-        copy16(&s.row[r][(c & 8) * 16 + piece_of(r, c >> 3, c & 7) * 16], base + (int64_t)max(from, 0) * KV8_ROW + c * 16, from >= 0);
-      }
+    for (int u = 0; u < CHUNK / 2; ++u) {
+      const int r = __shfl_sync(0xffffffffu, row, 2 * u + (lane >> 4));
+      copy16((at + lane_at + u * 2 * KV8_ROW) ^ ((u & 3) << 5), from + (int64_t)max(r, 0) * KV8_ROW, r >= 0);
     }
-    asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-  int64_t tok;
-  int row;
+  auto commit = []() { asm volatile("cp.async.commit_group;\n" ::: "memory"); };
+  int tok, row;
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
-    pick(i, tok, row);
-    bring(i, tok, row);
+    pick(tok, row);
+    if (i < n) bring(i, tok, row);
+    commit();
   }
-  pick(STAGES - 1, tok, row);
+  pick(tok, row);
 
   // q: this lane's dims, 16 j .. and 64 + 16 j .., of term g (0, 1, 2; zeros for the others)
   uint32_t qf[16];
   float rs;
   {
     float x[32];
+    load16(q, dtype, bhg * D + 16 * j, x);
+    load16(q, dtype, bhg * D + 64 + 16 * j, x + 16);
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      x[i] = element(q, dtype, bhg * D + (i < 16 ? 16 * j + i : 48 + 16 * j + i));
-      top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    }
+    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = __reduce_max_sync(0xffffffffu, top);
     const int e = kv8_exponent(top);
     const float inv = top < 0x7F800000u ? pow2i(-e) : __uint_as_float(0x7FFFFFFFu);   // a row with inf or NaN is NaN
@@ -155,38 +170,59 @@ __global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void*
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float2 y = make_float2(x[2 * i] * inv, x[2 * i + 1] * inv);
-      __half2 h = __floats2half2_rn(y.x, y.y);
-      for (int t = 0; t < g && t < 2; ++t) {           // what the terms before left
-        const float2 f = __half22float2(h);
-        y = make_float2(y.x - f.x, y.y - f.y);
-        h = __floats2half2_rn(y.x, y.y);
+      __half2 h[3];
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        h[t] = __floats2half2_rn(y.x, y.y);
+        const float2 f = __half22float2(h[t]);
+        y = make_float2(y.x - f.x, y.y - f.y);         // what the terms so far leave
       }
-      qf[i] = g < 3 ? bits(h) : 0u;
+      qf[i] = g == 0 ? bits(h[0]) : g == 1 ? bits(h[1]) : g == 2 ? bits(h[2]) : 0u;
     }
   }
 
+  // this lane's pieces within a stage: of keys g and g + 8 (permuted alike), of values 2 j + (e & 1) + 4 (e & 2)
+  const int key_at = g * KV8_ROW + (j ^ permuted(g)) * 16;
+  int value_at[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) value_at[e] = (2 * j + e) * KV8_ROW + D + (g ^ permuted(2 * j + e)) * 16;
   float acc[8][4];                                     // dims 16 g + 2 t and + 1; columns 2 j, 2 j + 1
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
   float m = -INFINITY, lm = -1e30f, l = 0.0f;          // m is the warp's; l is of picks g and g + 8 of its chunks
+  int here = 0;                                        // stage of chunk i
   for (int i = 0; i < n; ++i) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                      // chunk i is there; chunk i - 1 has been read
-    bring(i + STAGES - 1, tok, row);
-    pick(i + STAGES, tok, row);
-    const Stage& s = st[i % STAGES];
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (i + STAGES - 1 < n) bring(here == 0 ? STAGES - 1 : here - 1, tok, row);
+    commit();
+    pick(tok, row);
+    const Stage& s = st[here];
+    const uint8_t* const bytes = &s.row[0][0];
+    here = here + 1 == STAGES ? 0 : here + 1;
+    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains of products
+    const uint4 k0 = *reinterpret_cast<const uint4*>(bytes + key_at), k1 = *reinterpret_cast<const uint4*>(bytes + (key_at ^ 64));
+    const uint4 k8 = *reinterpret_cast<const uint4*>(bytes + 8 * KV8_ROW + key_at),
+                k9 = *reinterpret_cast<const uint4*>(bytes + 8 * KV8_ROW + (key_at ^ 64));
+    uint32_t x[4][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(&s.row[g][piece_of(g, 0, j + 4 * h) * 16]);
-      const uint4 hi = *reinterpret_cast<const uint4*>(&s.row[g + 8][piece_of(g + 8, 0, j + 4 * h) * 16]);
-      const uint32_t x[4] = {lo.x, lo.y, lo.z, lo.w}, y[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        mma(c, half2_of(x[w]), half2_of(y[w]), half2_of(x[w] >> 16), half2_of(y[w] >> 16), qf[8 * h + 2 * w], qf[8 * h + 2 * w + 1]);
+    for (int e = 0; e < 4; ++e) {
+      const uint4 y = *reinterpret_cast<const uint4*>(bytes + (e >> 1) * 8 * KV8_ROW + value_at[e & 1]);
+      x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
     }
+    {
+      const uint32_t lo[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w}, hi[8] = {k8.x, k8.y, k8.z, k8.w, k9.x, k9.y, k9.z, k9.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        mma(c, half2_of(lo[w]), half2_of(hi[w]), half2_of(lo[w] >> 16), half2_of(hi[w] >> 16), qf[2 * w], qf[2 * w + 1]);
+        mma(c2, half2_of(lo[w + 4]), half2_of(hi[w + 4]), half2_of(lo[w + 4] >> 16), half2_of(hi[w + 4] >> 16), qf[8 + 2 * w],
+            qf[9 + 2 * w]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] += c2[e];
     // scores of picks g and g + 8: the sum of their columns, 2 of them in each lane of a quad
     float v[2] = {c[0] + c[1], c[2] + c[3]}, lv[2], w[2];
 #pragma unroll
@@ -226,13 +262,6 @@ __global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void*
       const float2 f = __half22float2(hi);
       b[e] = g == 0 ? bits(hi) : g == 1 ? bits(__floats2half2_rn(x - f.x, y - f.y)) : 0u;
     }
-    uint32_t x[4][4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = 2 * j + (e & 1) + (e & 2) * 4;
-      const uint4 y = *reinterpret_cast<const uint4*>(&s.row[r][D + piece_of(r, 1, g) * 16]);
-      x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
-    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
@@ -245,21 +274,15 @@ __global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void*
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
   // the warp's state: picks are spread over g
-  const float all = fmaxf(fmaxf(lm, __shfl_xor_sync(0xffffffffu, lm, 4)), -1e30f);
-  float ref = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, 8));
-  ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, 16));
+  float ref = lm;
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
   l *= ex2(lm - ref);
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  float *dm = s_m, *dlm = s_lm, *dl = s_l, *da = &s_acc[0][0];
-  if constexpr (CS > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.barrier_wait();
-    dm = cluster.map_shared_rank(s_m, 0);
-    dlm = cluster.map_shared_rank(s_lm, 0);
-    dl = cluster.map_shared_rank(s_l, 0);
-    da = cluster.map_shared_rank(&s_acc[0][0], 0);
-  }
+  cluster.barrier_wait();
+  float *dm = cluster.map_shared_rank(s_m, 0), *dlm = cluster.map_shared_rank(s_lm, 0);
+  float *dl = cluster.map_shared_rank(s_l, 0), *da = cluster.map_shared_rank(&s_acc[0][0], 0);
   if (lane == 0) dm[gw] = m, dlm[gw] = ref, dl[gw] = l;
   if (j == 0) {                                        // columns 0 and 1: the two terms' sums
     float4* dst = reinterpret_cast<float4*>(da + gw * D + 16 * g);
@@ -268,42 +291,48 @@ __global__ void __launch_bounds__(PW * 32, CTAS_PER_SM) picks_kernel(const void*
       dst[t / 2] = make_float4(acc[t][0] + acc[t][1], acc[t][2] + acc[t][3], acc[t + 1][0] + acc[t + 1][1],
                                acc[t + 1][2] + acc[t + 1][3]);
   }
-  if constexpr (CS == 1) __syncthreads();
-  else cg::this_cluster().sync();
+  cluster.sync();
   if (crank != 0) return;
-  float M = -1e30f, L = 0.0f, O = 0.0f;
+  // lane = warp state: its factor, then every thread a dim or more
+  float M = lane < NW ? s_lm[lane] : -1e30f;
+  M = warp_max(M);
+  const float L = warp_sum(lane < NW ? s_l[lane] * ex2(s_lm[lane] - M) : 0.0f);
+  const float mine = lane < NW && s_m[lane] != -INFINITY ? exp2f(s_m[lane] - HEAD - M) : 0.0f;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float O = 0.0f;
 #pragma unroll 8
-  for (int v = 0; v < NW; ++v) M = fmaxf(M, s_lm[v]);
-#pragma unroll 8
-  for (int v = 0; v < NW; ++v) {
-    L = fmaf(s_l[v], ex2(s_lm[v] - M), L);
-    if (s_m[v] != -INFINITY) O = fmaf(s_acc[v][threadIdx.x], exp2f(s_m[v] - HEAD - M), O);
+    for (int v = 0; v < NW; ++v) {
+      const float f = __shfl_sync(0xffffffffu, mine, v);
+      if (f != 0.0f) O = fmaf(s_acc[v][d], f, O);
+    }
+    const float o = O * inv;
+    const int64_t at = bhg * D + d;
+    if (dtype == FATHOM_DTYPE_F32) from_f32(o, reinterpret_cast<float*>(out) + at);
+    else if (dtype == FATHOM_DTYPE_BF16) from_f32(o, reinterpret_cast<__nv_bfloat16*>(out) + at);
+    else from_f32(o, reinterpret_cast<__half*>(out) + at);
   }
-  const float o = L == 0.0f ? 0.0f : O / L;
-  const int64_t at = bhg * D + threadIdx.x;
-  if (dtype == FATHOM_DTYPE_F32) from_f32(o, reinterpret_cast<float*>(out) + at);
-  else if (dtype == FATHOM_DTYPE_BF16) from_f32(o, reinterpret_cast<__nv_bfloat16*>(out) + at);
-  else from_f32(o, reinterpret_cast<__half*>(out) + at);
 }
 
-template <int CS> int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, void* out, cudaStream_t st) {
-  constexpr int smem = PW * STAGES * (int)sizeof(Stage);
+int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, int pw, int cs, void* out, cudaStream_t st) {
+  const int smem = pw * STAGES * (int)sizeof(Stage) + pw * cs * D * (int)sizeof(float);
+  constexpr int most = MAX_PW * STAGES * (int)sizeof(Stage) + MAX_PW * MAX_CS * D * (int)sizeof(float);
   static std::atomic<uint64_t> told{0};
-  const int r = allow_smem(picks_kernel<CS>, smem, told, "kv8_attend_picks");
+  const int r = allow_smem(picks_kernel, most, told, "kv8_attend_picks");
   if (r != FATHOM_OK) return r;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(heads * CS));
-  cfg.blockDim = dim3(PW * 32);
+  cfg.gridDim = dim3((unsigned)heads, (unsigned)cs);
+  cfg.blockDim = dim3((unsigned)pw * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CS;
-  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = (unsigned)cs;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = CS > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, picks_kernel<CS>, q, dtype, a, out);
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, picks_kernel, q, dtype, a, out);
   if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend_picks: launch: %s", cudaGetErrorString(e));
   return check_launch("kv8_attend_picks");
 }
@@ -330,7 +359,7 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
   FATHOM_REQUIRE(dtype >= FATHOM_DTYPE_F32 && dtype <= FATHOM_DTYPE_F16, FATHOM_ERR_UNSUPPORTED,
                  "kv8_attend_picks: queries must be fp32, bf16 or fp16");
   FATHOM_REQUIRE(B >= 1 && Hkv >= 1 && B <= 65535 && Hkv <= 65535 && B * Hkv <= 65535 && G >= 1 && G <= 65535 &&
-                     B * Hkv * G <= INT32_MAX / 8 && k >= 1 && k <= INT32_MAX && cap >= BLK && cap % BLK == 0 &&
+                     B * Hkv * G <= INT32_MAX / 8 && k >= 1 && k <= 1 << 30 && cap >= BLK && cap % BLK == 0 &&
                      cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE, "kv8_attend_picks: bad shape");
   FATHOM_REQUIRE(end_dev || (end >= 0 && end <= cap), FATHOM_ERR_SHAPE,
                  "kv8_attend_picks: end %lld is outside the cache's %lld", (long long)end, (long long)cap);
@@ -339,11 +368,12 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
   FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_picks_workspace_bytes(B, Hkv, G, k), FATHOM_ERR_WORKSPACE,
                  "kv8_attend_picks: workspace too small");
   const PicksArgs a{idx, nullptr, k, rows, cap, scales, cap, end, end_dev, (int)Hkv, G};
-  const int64_t heads = B * Hkv * G, slots = (int64_t)CTAS_PER_SM * sm_count(), chunks = cdiv(k, CHUNK);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // as many CTAs per head as fit the GPU at once and have a chunk for every warp
-  if (heads * 8 <= slots && chunks > 4 * PW) return launch_picks<8>(q, dtype, a, heads, out, st);
-  if (heads * 4 <= slots && chunks > 2 * PW) return launch_picks<4>(q, dtype, a, heads, out, st);
-  if (heads * 2 <= slots && chunks > PW) return launch_picks<2>(q, dtype, a, heads, out, st);
-  return launch_picks<1>(q, dtype, a, heads, out, st);
+  // as many warps per head as the GPU holds at once, 32 at most, and no more than there are chunks; in CTAs of 2 (in
+  // whose number a wave is filled best) or of 4
+  const int64_t heads = B * Hkv * G, chunks = cdiv(k, CHUNK);
+  int64_t warps = (int64_t)WARPS_PER_SM * sm_count() / heads;
+  if (warps > chunks) warps = chunks;
+  const int pw = warps > 2 * MAX_CS ? 4 : warps > 1 ? 2 : 1;
+  const int64_t cs = warps / pw < 1 ? 1 : warps / pw > MAX_CS ? MAX_CS : warps / pw;
+  return launch_picks(q, dtype, a, heads, pw, (int)cs, out, reinterpret_cast<cudaStream_t>(stream));
 }
