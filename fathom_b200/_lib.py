@@ -67,8 +67,8 @@ SIGNATURES = {
     "fathom_kv8_attend_workspace_bytes": (SZ, [I64, I64, I32, I64]),
     "fathom_kv8_attend": (I32, [P, I32, I64, I64, I32, I64, I64, I64, I64, P, P, I64, I64, P, P, I64, I64, I64, P, SZ,
                                 P]),
-    "fathom_kv8_attend_picks_workspace_bytes": (SZ, [I64, I64, I32, I64]),
-    "fathom_kv8_attend_picks": (I32, [P, I32, I64, I64, I32, P, I64, P, P, I64, I64, P, P, P, SZ, P]),
+    "fathom_kv8_attend_picks_workspace_bytes": (SZ, [I64, I64, I32, I64, I32]),
+    "fathom_kv8_attend_picks": (I32, [P, I32, I64, I64, I32, P, I64, P, I32, P, I64, I64, P, P, P, SZ, P]),
     "fathom_host_alloc_mapped": (I32, [SZ, ctypes.POINTER(P), ctypes.POINTER(P)]),
     "fathom_host_alloc_mapped_ex": (I32, [SZ, I32, ctypes.POINTER(P), ctypes.POINTER(P)]),
     "fathom_host_free": (I32, [P]),

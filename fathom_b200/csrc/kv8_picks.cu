@@ -14,6 +14,7 @@
 // Softmax state per warp, in fp32 as in kv8_token.cu: references of s + log2(value scale) for the output and of s for
 // the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their states are joined in warp
 // order in the first CTA's shared memory.
+#include "dedupe.cuh"
 #include "kv8_attn.cuh"
 
 #include <cooperative_groups.h>
@@ -337,6 +338,52 @@ int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, in
   return check_launch("kv8_attend_picks");
 }
 
+// Rows in host memory: each distinct row of a KV head once over the host link into the workspace, in ascending order.
+// 16 lanes x 16 bytes per row, 4 rows in flight per lane.
+constexpr int GT = 256, GROWS = GT / 16 * 4;
+__global__ void __launch_bounds__(GT) gather_kernel(const int32_t* __restrict__ ucount, const int64_t* __restrict__ uniq,
+                                                    int64_t M, const uint4* __restrict__ rows, int64_t cap,
+                                                    uint4* __restrict__ stage) {
+  constexpr int LPR = KV8_ROW / 16, RPP = GT / LPR, PASSES = GROWS / RPP;
+  const int64_t bh = blockIdx.y, U = ucount[bh], r0 = (int64_t)blockIdx.x * GROWS;
+  if (r0 >= U) return;
+  const int c = threadIdx.x % LPR;
+  uint4 v[PASSES];
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int64_t r = r0 + p * RPP + threadIdx.x / LPR;
+    if (r < U) v[p] = rows[(bh * cap + uniq[bh * M + r]) * LPR + c];
+  }
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const int64_t r = r0 + p * RPP + threadIdx.x / LPR;
+    if (r < U) stage[(bh * M + r) * LPR + c] = v[p];
+  }
+}
+
+struct StageWs {
+  int32_t* slot;       // [BH][M] pick -> row of the stage (-1: none)
+  int64_t* uniq;       // [BH][M] distinct picks, ascending
+  int32_t* ucount;     // [BH]
+  uint8_t* rows;       // [BH][M][256]
+};
+size_t stage_bytes(int64_t BH, int64_t M) {
+  return align256(BH * M * sizeof(int32_t)) + align256(BH * M * sizeof(int64_t)) + align256(BH * sizeof(int32_t)) +
+         (size_t)(BH * M) * KV8_ROW;
+}
+StageWs carve(void* base, int64_t BH, int64_t M) {
+  char* p = static_cast<char*>(base);
+  StageWs w;
+  w.slot = reinterpret_cast<int32_t*>(p);
+  p += align256(BH * M * sizeof(int32_t));
+  w.uniq = reinterpret_cast<int64_t*>(p);
+  p += align256(BH * M * sizeof(int64_t));
+  w.ucount = reinterpret_cast<int32_t*>(p);
+  p += align256(BH * sizeof(int32_t));
+  w.rows = reinterpret_cast<uint8_t*>(p);
+  return w;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
@@ -346,13 +393,13 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 using namespace fathom;
 using namespace fathom::kv8;
 
-extern "C" size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k) {
+extern "C" size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k, int host_rows) {
   if (B <= 0 || Hkv <= 0 || G <= 0 || k <= 0) return 0;
-  return 256;
+  return host_rows && G * k <= MAX_M ? stage_bytes(B * Hkv, G * k) : 256;
 }
 
 extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int64_t Hkv, int G, const int64_t* idx,
-                                       int64_t k, const uint8_t* rows, const float* scales, int64_t cap, int64_t end,
+                                       int64_t k, const uint8_t* rows, int host_rows, const float* scales, int64_t cap, int64_t end,
                                        const int64_t* end_dev, void* out, void* workspace, size_t workspace_bytes,
                                        void* stream) {
   FATHOM_REQUIRE(q && idx && rows && scales && out && workspace, FATHOM_ERR_NULL, "kv8_attend_picks: NULL pointer");
@@ -365,9 +412,23 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
                  "kv8_attend_picks: end %lld is outside the cache's %lld", (long long)end, (long long)cap);
   FATHOM_REQUIRE(aligned16(rows) && aligned16(q) && aligned16(out), FATHOM_ERR_SHAPE,
                  "kv8_attend_picks: rows, q and out must be 16-byte aligned");
-  FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_picks_workspace_bytes(B, Hkv, G, k), FATHOM_ERR_WORKSPACE,
-                 "kv8_attend_picks: workspace too small");
-  const PicksArgs a{idx, nullptr, k, rows, cap, scales, cap, end, end_dev, (int)Hkv, G};
+  FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_picks_workspace_bytes(B, Hkv, G, k, host_rows) &&
+                     (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, FATHOM_ERR_WORKSPACE,
+                 "kv8_attend_picks: workspace needs %zu bytes, 256-byte aligned",
+                 fathom_kv8_attend_picks_workspace_bytes(B, Hkv, G, k, host_rows));
+  PicksArgs a{idx, nullptr, k, rows, cap, scales, cap, end, end_dev, (int)Hkv, G};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t BH = B * Hkv, M = G * k;
+  if (host_rows && M <= MAX_M) {             // longer lists read their rows in place, over the link, once per pick
+    const StageWs w = carve(workspace, BH, M);
+    int r = launch_dedupe(idx, BH, M, 0, cap, cap, w.slot, w.uniq, w.ucount, st);
+    if (r != FATHOM_OK) return r;
+    gather_kernel<<<dim3((unsigned)cdiv(M, GROWS), (unsigned)BH), GT, 0, st>>>(
+        w.ucount, w.uniq, M, reinterpret_cast<const uint4*>(rows), cap, reinterpret_cast<uint4*>(w.rows));
+    r = check_launch("kv8_attend_picks (dedupe, gather)");
+    if (r != FATHOM_OK) return r;
+    a.slot = w.slot, a.rows = w.rows, a.row_cap = M;
+  }
   // as many warps per head as the GPU holds at once, 32 at most, and no more than there are chunks; in CTAs of 2 (in
   // whose number a wave is filled best) or of 4
   const int64_t heads = B * Hkv * G, chunks = cdiv(k, CHUNK);
@@ -375,5 +436,5 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
   if (warps > chunks) warps = chunks;
   const int pw = warps > 2 * MAX_CS ? 4 : warps > 1 ? 2 : 1;
   const int64_t cs = warps / pw < 1 ? 1 : warps / pw > MAX_CS ? MAX_CS : warps / pw;
-  return launch_picks(q, dtype, a, heads, pw, (int)cs, out, reinterpret_cast<cudaStream_t>(stream));
+  return launch_picks(q, dtype, a, heads, pw, (int)cs, out, st);
 }

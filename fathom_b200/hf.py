@@ -17,6 +17,11 @@ Life cycle of a sequence batch:
             appended); the local window [m - local, m) appended (it reaches into the recent
             buffer); exact attention over the picks, host rows fetched once per KV head (:163-244)
 
+With kv="e4m3" the K/V rows are an 8-bit cache (fathom_b200.kv8) from the first prefill chunk on: each chunk is
+written to it and attends to it, the index is built from the keys read back, a generated token is appended to it,
+and the picks are read from it (half the bytes per row, in HBM or over the host link).  A context of at most k
+tokens then needs no index: with rows in HBM its decode steps attend to every key.
+
 With klt=True the index is the KLT-rotated store (planesK, for models without QK-norm): the basis
 comes from the session's own prefill keys, the plan from the rotated gains.
 
@@ -30,6 +35,7 @@ import torch
 import torch.nn.functional as F
 
 from . import bitplane as bp, klt as klt_mod
+from .kv8 import KVCache8
 from .offload import HostPlaneStore, MappedBuffer, decode_attention
 
 SKIP = 16        # tokens left out of the key statistics (4 * SINK, scripts/sketch.py:44-46)
@@ -37,11 +43,11 @@ SKIP = 16        # tokens left out of the key statistics (4 * SINK, scripts/sket
 
 class _Layer:
     __slots__ = ("Kdev", "Vdev", "len", "n", "rows", "K_src", "V_src", "store", "var", "Krec", "Vrec", "nrec",
-                 "owned")
+                 "owned", "kv8")
 
     def __init__(self):
         self.Kdev = self.Vdev = self.rows = self.K_src = self.V_src = self.store = self.var = None
-        self.Krec = self.Vrec = None
+        self.Krec = self.Vrec = self.kv8 = None
         self.len = self.n = self.nrec = 0
         self.owned = []
 
@@ -54,6 +60,7 @@ class OffloadedDecoder:
     budget          scan budget: a number, or a per-layer sequence / {layer: budget} (per-layer budgets)
     index, rows     "host" (pinned mapped host memory, zero-copy) or "hbm" for the bit-plane index and
                     for the K/V rows
+    kv              "bf16", or "e4m3" for K/V rows in 8 bits (KVCache8)
     max_new         capacity of the recent-token buffer (generated tokens)
     klt             KLT-rotated index (planesK) instead of the plain one
     graphs          replay one CUDA graph of the whole model step per generated token once the local
@@ -64,7 +71,7 @@ class OffloadedDecoder:
     """
 
     def __init__(self, model, k=580, sink=4, local=64, budget=48.0, index="host", rows="host", max_new=64,
-                 klt=False, prefill_chunk=2048, graphs=False):
+                 klt=False, prefill_chunk=2048, graphs=False, kv="bf16"):
         cfg = model.config
         self.model = model
         self.Hq = cfg.num_attention_heads
@@ -76,7 +83,9 @@ class OffloadedDecoder:
         self.k, self.sink, self.local = k, sink, local
         if index not in ("host", "hbm") or rows not in ("host", "hbm"):
             raise ValueError("OffloadedDecoder: index and rows must be 'host' or 'hbm'")
-        self.index, self.rows, self.max_new, self.klt = index, rows, max_new, klt
+        if kv not in ("bf16", "e4m3"):
+            raise ValueError("OffloadedDecoder: kv must be 'bf16' or 'e4m3'")
+        self.index, self.rows, self.max_new, self.klt, self.kv = index, rows, max_new, klt, kv
         self.prefill_chunk = prefill_chunk
         self.attn = [layer.self_attn for layer in model.model.layers]
         nL = len(self.attn)
@@ -138,8 +147,11 @@ class OffloadedDecoder:
         dev = input_ids.device
         self._reset(B)
         for c in self.cache:
-            c.Kdev = torch.empty(B, self.Hkv, n, self.D, dtype=torch.bfloat16, device=dev)
-            c.Vdev = torch.empty_like(c.Kdev)
+            if self.kv == "e4m3":
+                c.kv8 = KVCache8(B, self.Hkv, n + self.max_new, dev)
+            else:
+                c.Kdev = torch.empty(B, self.Hkv, n, self.D, dtype=torch.bfloat16, device=dev)
+                c.Vdev = torch.empty_like(c.Kdev)
             c.len = 0
         self.mode = "prefill"
         logits = None
@@ -154,6 +166,10 @@ class OffloadedDecoder:
     def _prefill_attn(self, L, q, k, v):
         c = self.cache[L]
         m0, Tq = c.len, q.shape[2]
+        if c.kv8 is not None:
+            c.kv8.write(k, v, m0)
+            c.len = m0 + Tq
+            return c.kv8.attend(q, c.len)
         c.Kdev[:, :, m0:m0 + Tq] = k
         c.Vdev[:, :, m0:m0 + Tq] = v
         c.len = m = m0 + Tq
@@ -170,6 +186,10 @@ class OffloadedDecoder:
             self._reset(K.shape[0])
         c = self.cache[L]
         c.Kdev, c.Vdev, c.len = K, V, K.shape[2]
+        if self.kv == "e4m3" and rows_of is None:
+            c.kv8 = KVCache8(self.B, self.Hkv, c.len + self.max_new, K.device)
+            c.kv8.write(K, V)
+            c.Kdev = c.Vdev = None
         if offload:
             self._offload_layer(L, rows_of)
             if L == len(self.cache) - 1:
@@ -187,10 +207,14 @@ class OffloadedDecoder:
         BH = B * Hkv
         c = self.cache[L]
         n = c.len
-        if n < self.k + 1:
+        dense = self.kv == "e4m3" and self.rows == "hbm" and n <= self.k and rows_of is None
+        if n < self.k + 1 and not dense:
             raise ValueError(f"OffloadedDecoder: prefill of {n} tokens is shorter than k = {self.k}")
         if L > 0 and n != self.cache[0].n:
             raise ValueError("OffloadedDecoder: every layer needs the same prefill length")
+        if self.kv == "e4m3":
+            self._offload_layer8(L, rows_of, dense)
+            return
         K = c.Kdev[:, :, :n].reshape(BH, n, D).to(torch.bfloat16)
         V = None if rows_of is not None else c.Vdev[:, :, :n].reshape(BH, n, D).to(torch.bfloat16)
         dev = K.device
@@ -220,9 +244,39 @@ class OffloadedDecoder:
         c.n, c.nrec = n, 0
         c.Kdev = c.Vdev = None
 
+    def _offload_layer8(self, L, rows_of, dense):
+        """As _offload_layer over an 8-bit cache: the index sees the keys that attention will."""
+        c = self.cache[L]
+        n, BH = c.len, self.B * self.Hkv
+        if rows_of is not None:
+            src = self.cache[rows_of]
+            if not (0 <= rows_of < L) or src.kv8 is None or src.n != n:
+                raise ValueError(f"OffloadedDecoder: rows_of={rows_of} must name an offloaded earlier layer")
+            c.kv8, K = src.kv8, c.Kdev.to(torch.bfloat16)
+        elif not dense:
+            K = c.kv8.read(0, n)[0]
+        if not dense:
+            K = K.reshape(BH, n, self.D)
+            basis = klt_mod.klt_basis(K) if self.klt else None
+            if self.index == "host":
+                c.store = HostPlaneStore(K, torch.float32 if self.klt else torch.float16, basis=basis)
+                c.owned.append(c.store)
+            else:
+                c.store = klt_mod.KLTPlaneStore(K, basis) if self.klt else bp.PlaneStore(K)
+            c.var = None if self.klt else K[:, SKIP:].float().var(1)
+        if self.rows == "host" and rows_of is None:
+            dev8 = c.kv8
+            c.kv8 = KVCache8(self.B, self.Hkv, dev8.cap, dev8.device, host=True)
+            c.kv8.rows.copy_(dev8.rows)
+            c.kv8.scales.copy_(dev8.scales)
+            c.owned.append(c.kv8)
+        c.n, c.nrec = n, 0
+        c.Kdev = c.Vdev = None
+
     def _finish_offload(self):
         BH, n = self.B * self.Hkv, self.cache[0].n
-        dev = self.cache[0].Krec.device
+        c0 = self.cache[0]
+        dev = c0.kv8.device if c0.kv8 is not None else c0.Krec.device
         self._scores = torch.empty(BH, self.G, n, dtype=torch.float32, device=dev)
         self._idx = torch.empty(BH, self.G, self.k, dtype=torch.int64, device=dev)
         self._arange_local = torch.arange(self.local, dtype=torch.int64, device=dev)
@@ -247,7 +301,7 @@ class OffloadedDecoder:
             for o in c.owned:
                 o.free()
             c.owned = []
-            c.store = c.rows = c.K_src = c.V_src = None
+            c.store = c.rows = c.K_src = c.V_src = c.kv8 = None
         self.mode = "idle"
 
     # ---------------------------------------------------------------- decode
@@ -314,7 +368,15 @@ class OffloadedDecoder:
         sink, local = self.sink, self.local
         kk = self.k - sink - local
         n = c.n
-        if self._graph_mode:                     # slot and window base are device inputs; nrec moves outside
+        if c.kv8 is not None:                    # the new token goes where the sequence ends
+            pos = self._pos_s.view(-1) if self._graph_mode else n + c.nrec
+            c.kv8.write(k, v, pos)
+            if not self._graph_mode:
+                c.nrec += 1
+            m = n + c.nrec + (1 if self._graph_mode else 0)
+            if c.store is None:                  # at most k tokens of prefill: every key
+                return c.kv8.attend(q, pos + 1)
+        elif self._graph_mode:                   # slot and window base are device inputs; nrec moves outside
             c.Krec.index_copy_(1, self._slot_s, k.reshape(BH, 1, D))
             c.Vrec.index_copy_(1, self._slot_s, v.reshape(BH, 1, D))
             m = n + c.nrec + 1
@@ -341,6 +403,8 @@ class OffloadedDecoder:
         # the local window [m - local, m): one add into the strided tail of the index rows
         torch.add(self._arange_local.expand(BH, G, local), self._wbase_s if self._graph_mode else m - local,
                   out=idx[..., kk + sink:])
+        if c.kv8 is not None:
+            return c.kv8.attend_picks(q.reshape(BH, G, D), idx).view(B, Hq, 1, D)
         out = decode_attention(qf, idx, c.K_src, c.V_src, n, n, c.Krec, c.Vrec, self.max_new,
                                out_dtype=torch.bfloat16)
         return out.view(B, Hq, 1, D)

@@ -16,6 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib, ptr, require_cuda
+from .offload import MappedBuffer
 
 BLK, D = 64, 128
 
@@ -36,11 +37,13 @@ class KVCache8:
 
     rows    uint8 [B * Hkv, cap, 2, 128]: e4m3 codes of each token's key (0) and value (1)
     scales  fp32 [B * Hkv, cap / 64, 2]: powers of two; value = code * scale
-    Either both may be given (contiguous, of these shapes) or they are made, zeroed, on `device`.  Tokens past
-    the last written one are void: no call reads them.  Which tokens a sequence has is the caller's to
-    know: a write says where it begins, a read or an attention where it ends."""
+    Either both may be given (contiguous, of these shapes) or they are made on `device`; host=True puts the rows
+    into pinned mapped host memory (the scales stay on the device; free() or garbage collection releases
+    the rows): written and read over the host link, attended to over picks only.  Tokens past the last written
+    one are void: no call reads them.  Which tokens a sequence has is the caller's to know: a write says where it
+    begins, a read or an attention where it ends."""
 
-    def __init__(self, B, Hkv, cap, device="cuda", rows=None, scales=None):
+    def __init__(self, B, Hkv, cap, device="cuda", rows=None, scales=None, host=False):
         if B < 1 or Hkv < 1 or cap < 1:
             raise ValueError(f"KVCache8: B, Hkv and cap must be positive (got {B}, {Hkv}, {cap})")
         self.B, self.Hkv, self.BH = B, Hkv, B * Hkv
@@ -48,8 +51,16 @@ class KVCache8:
         self.cap = self.nblk * BLK
         if (rows is None) != (scales is None):
             raise ValueError("KVCache8: rows and scales come together")
+        if host and rows is not None:
+            raise ValueError("KVCache8: host=True makes the rows itself")
+        self.host, self._buf = host, None
         if rows is None:
-            rows = torch.zeros(self.BH, self.cap, 2, D, dtype=torch.uint8, device=device)
+            if host:
+                self._buf = MappedBuffer((self.BH, self.cap, 2, D), torch.uint8,
+                                         None if torch.device(device).index is None else device)
+                rows, device = self._buf.dev, self._buf.dev.device
+            else:
+                rows = torch.zeros(self.BH, self.cap, 2, D, dtype=torch.uint8, device=device)
             scales = torch.zeros(self.BH, self.nblk, 2, dtype=torch.float32, device=device)
         require_cuda(rows, scales)
         if rows.dtype != torch.uint8 or tuple(rows.shape) != (self.BH, self.cap, 2, D) or not rows.is_contiguous():
@@ -62,6 +73,13 @@ class KVCache8:
 
     def nbytes(self):
         return self.rows.numel() + self.scales.numel() * 4
+
+    def free(self):
+        """Release rows in host memory (device tensors go with their last reference)."""
+        if self._buf is not None:
+            self.rows = None
+            self._buf.free()
+            self._buf = None
 
     def _stream(self):
         return torch._C._cuda_getCurrentRawStream(self.device.index)
@@ -127,6 +145,8 @@ class KVCache8:
         [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
         that sees no key gives 0.  Returns [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
         self._check_on("KVCache8.attend", q)
+        if self.host:
+            raise ValueError("KVCache8.attend: the rows are in host memory (attend_picks reads those)")
         if q.dim() != 4 or q.shape[0] != self.B or q.shape[1] < 1 or q.shape[1] % self.Hkv or q.shape[3] != D:
             raise ValueError(f"KVCache8.attend: q must be [{self.B}, a multiple of {self.Hkv}, T, {D}] "
                              f"(got {tuple(q.shape)})")
@@ -153,7 +173,8 @@ class KVCache8:
         """Attention over listed tokens, as decode_attention over bf16 rows: q [BH, G, 128] (fp32, bf16 or fp16),
         idx [BH, G, k] int64.  Picks outside [0, end) are ignored (end: an int, int64 [B] on the device, or None
         for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  fp32
-        arithmetic; returns [BH, G, 128] in q's dtype."""
+        arithmetic; returns [BH, G, 128] in q's dtype.  Of rows in host memory each distinct one of a KV head is
+        fetched once."""
         self._check_on("KVCache8.attend_picks", q, idx)
         if q.dim() != 3 or q.shape[0] != self.BH or q.shape[1] < 1 or q.shape[2] != D:
             raise ValueError(f"KVCache8.attend_picks: q must be [{self.BH}, G, {D}] (got {tuple(q.shape)})")
@@ -173,10 +194,11 @@ class KVCache8:
         if q.data_ptr() % 16:
             q = q.clone()
         out = torch.empty(BH, G, D, dtype=q.dtype, device=self.device)
-        ws, nws = self._workspace((G, k, "picks"), lib().fathom_kv8_attend_picks_workspace_bytes, G, k)
-        check(lib().fathom_kv8_attend_picks(ptr(q), _lib.DTYPE_CODE[q.dtype], self.B, self.Hkv, G, ptr(idx), k,
-                                            ptr(self.rows), ptr(self.scales), self.cap, num, ptr(dev), ptr(out),
-                                            ptr(ws), nws, self._stream()), "KVCache8.attend_picks")
+        ws, nws = self._workspace((G, k, "picks"), lib().fathom_kv8_attend_picks_workspace_bytes, G, k, int(self.host))
+        check(lib().fathom_kv8_attend_picks(q.data_ptr(), _lib.DTYPE_CODE[q.dtype], self.B, self.Hkv, G, idx.data_ptr(), k,
+                                            self.rows.data_ptr(), int(self.host), self.scales.data_ptr(), self.cap, num,
+                                            ptr(dev), out.data_ptr(), ws.data_ptr(), nws, self._stream()),
+              "KVCache8.attend_picks")
         return out
 
 

@@ -344,13 +344,15 @@ int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, i
                       int64_t o_stride_t, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Workspace bytes of fathom_kv8_attend_picks. */
-size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k);
+size_t fathom_kv8_attend_picks_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t k, int host_rows);
 
 /* The same over listed tokens: q, out [B*Hkv][G][128] (fp32, bf16 or fp16), idx [B*Hkv][G][k] int64 token indices.
- * A pick outside [0, end) is ignored, one listed twice counts twice; no pick left gives 0. */
+ * A pick outside [0, end) is ignored, one listed twice counts twice; no pick left gives 0.  host_rows != 0: rows
+ * is a mapped host alias (the scales stay in device memory); each distinct row of a KV head is then fetched once over the
+ * link into the workspace where G*k <= 16384, and rows are read in place otherwise. */
 int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int64_t Hkv, int G, const int64_t* idx, int64_t k,
-                            const uint8_t* rows, const float* scales, int64_t cap, int64_t end, const int64_t* end_dev,
-                            void* out, void* workspace, size_t workspace_bytes, void* stream);
+                            const uint8_t* rows, int host_rows, const float* scales, int64_t cap, int64_t end,
+                            const int64_t* end_dev, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- host memory */
 

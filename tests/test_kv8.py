@@ -60,13 +60,15 @@ def test_c_entries_refuse_bad_arguments():
     assert attend(nb=0) == _lib.FATHOM_ERR_WORKSPACE
     assert b"workspace" in L.fathom_last_error()
 
-    def picks(q=p, dtype=1, B=1, H=1, G=4, idx=p, k=10, cap=128, end=100, nb=1 << 40):
-        return L.fathom_kv8_attend_picks(q, dtype, B, H, G, idx, k, p, p, cap, end, None, p, p, nb, None)
+    def picks(q=p, dtype=1, B=1, H=1, G=4, idx=p, k=10, cap=128, end=100, nb=1 << 40, host=0):
+        return L.fathom_kv8_attend_picks(q, dtype, B, H, G, idx, k, p, host, p, cap, end, None, p, p, nb, None)
 
     assert picks(q=None) == picks(idx=None) == _lib.FATHOM_ERR_NULL
     assert picks(dtype=5) == _lib.FATHOM_ERR_UNSUPPORTED
     assert picks(k=0) == picks(end=129) == picks(G=0) == picks(B=70000) == picks(q=odd) == _lib.FATHOM_ERR_SHAPE
-    assert picks(nb=0) == _lib.FATHOM_ERR_WORKSPACE
+    assert picks(nb=0) == picks(nb=1000, host=1) == _lib.FATHOM_ERR_WORKSPACE
+    assert L.fathom_kv8_attend_picks_workspace_bytes(1, 8, 4, 580, 1) >= 8 * 4 * 580 * 256
+    assert L.fathom_kv8_attend_picks_workspace_bytes(1, 8, 4, 580, 0) == 256
 
 
 def test_python_layer_refuses_cpu_tensors_and_bad_sizes():

@@ -330,6 +330,31 @@ def test_picks_outside_are_ignored():
         assert not out[0, 0].any() and not out[1, 1].any() and not out[2, 2].any()
 
 
+@pytest.mark.parametrize("G,k", [(4, 580), (1, 1), (8, 64), (7, 3000)])       # 7 * 3000 > 16384: read in place
+def test_picks_from_host_rows_equal_device_rows(G, k):
+    from fathom_b200.kv8 import KVCache8
+    B, H, n = 2, 2, 5000
+    K, V = _kv(B, H, n + 3, torch.bfloat16, 30)
+    dev, host = KVCache8(B, H, n + 50), KVCache8(B, H, n + 50, host=True)
+    g = torch.Generator().manual_seed(k)
+    idx = torch.randint(-5, n + 60, (B * H, G, k), generator=g).cuda()
+    idx[:, :, : k // 3] = idx[:, :1, : k // 3]                  # shared picks across the group
+    q = torch.randn(B * H, G, 128, generator=g).cuda()
+    ends = torch.tensor([n + 3, 100], device="cuda")
+    for c in (dev, host):
+        c.write(K[:, :, :n], V[:, :, :n])
+        for t in range(3):                                      # and token by token, over the link
+            c.write(K[:, :, n + t:n + t + 1], V[:, :, n + t:n + t + 1], n + t)
+    for end in (n + 3, ends):
+        assert torch.equal(host.attend_picks(q, idx, end), dev.attend_picks(q, idx, end))
+    for x, y in zip(host.read(0, n + 3), dev.read(0, n + 3)):
+        assert torch.equal(x, y)
+    with pytest.raises(ValueError, match="host"):
+        host.attend(q[:, :, None].bfloat16().view(B, H * G, 1, 128), n)
+    torch.cuda.synchronize()
+    host.free()
+
+
 def test_python_layer_refuses():
     from fathom_b200.kv8 import KVCache8
     c = KVCache8(2, 2, 100)
