@@ -67,7 +67,7 @@ template <typename K> int allow_smem(K kernel, int smem, std::atomic<uint64_t>& 
 int sm_count();
 
 // kv8_token.cu: up to TOKEN_ROWS query rows (G * T) per KV head.
-constexpr int TOKEN_ROWS = 16;
+constexpr int TOKEN_ROWS = 32;
 size_t token_workspace(int64_t BH, int64_t R);
 int token_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st);
 // kv8_prompt.cu: any number of query rows, 256 at a time.

@@ -14,7 +14,7 @@
 // cores work for the other.  A third warpgroup turns value tiles into f16.  The key scale multiplies the score and
 // the value scale 2^ev, a constant of each 64-token half of a tile, enters the weight's exponent, so a row sees its own
 // range whatever other blocks hold.  Softmax, thread = row: m, the reference of s + ev, follows the row's maximum
-// only when that exceeds it by 2^7 (then O is rescaled); weights are 2^(s + ev - m + 8), at most 2^15 in f16, rounded to
+// only when that exceeds it by 2^12 (then O is rescaled; at 2^7 that cost 3%); weights are 2^(s + ev - m + 3), at most 2^15 in f16, rounded to
 // 11 bits; sums in fp32, the denominator taking each half's sum times 2^(largest ev - ev).  Blocks whose
 // scale is below 2^-40 of the sequence's largest count as 2^-40 there and have the rest multiplied into their
 // f16 values, which keeps the denominator in range.
@@ -32,8 +32,8 @@ constexpr int KSTAGES = 3, VSTAGES = 2;
 constexpr int KBYTES = TILE * D, VBYTES = 2 * TILE * D;
 constexpr int SOFT = 256;                    // softmax threads of a half: two per row, one for each 64-token block of a tile
 constexpr int THREADS = 2 * SOFT + 256;      // warps 0-7, 8-15: softmax; 16-19: values; 20: products; 21: key loads
-constexpr float SLACK = 7.0f;                // a row may exceed its reference by 2^7
-constexpr float HEAD = 8.0f;                 // weights at the reference are 2^8
+constexpr float SLACK = 12.0f;               // a row may exceed its reference by 2^12
+constexpr float HEAD = 3.0f;                 // weights at the reference are 2^3
 // registers per thread of the softmax, value and other warps: together no more than the 768 * 80 of the launch
 constexpr int REG_LAUNCH = 80, REG_SOFT = 88, REG_VALUE = 64, REG_OTHER = 64;
 static_assert(4 * REG_SOFT + REG_VALUE + REG_OTHER <= 6 * REG_LAUNCH, "register split");

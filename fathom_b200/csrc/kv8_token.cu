@@ -16,8 +16,9 @@
 // Softmax, thread = token: with m the running reference of a row's (score + log2 of the value scale), a weight is
 // 2^(s + log2 vs - m); m moves only when a tile exceeds it by 2^6 (then O^T in tensor memory is rescaled), which
 // leaves e4m3's range room on both sides.  The denominator is kept per thread in fp32 with a reference of its
-// own, because the value scale must not enter it.  Two warpgroups take the even and the odd tiles, each with
-// its own references and its own O^T: one tile's chain of steps is longer than its bytes take.
+// own, because the value scale must not enter it.  One tile's chain of steps is longer than its bytes take, so there are
+// two softmax warpgroups: up to 16 rows they take the even and the odd tiles, each with its own references and its own
+// O^T; up to 32 rows (SPLIT) each takes 16 rows of every tile.
 //
 // A row's parts in different CTAs (kv8_line.cuh) are joined by a second kernel in a fixed order.
 #include "kv8_line.cuh"
@@ -30,7 +31,6 @@ constexpr int TERMS = 3;                         // e4m3 terms of a weight
 constexpr int GROUP = 128;                       // threads of a softmax warpgroup
 constexpr int THREADS = 2 * GROUP + 64;          // warps 0-3, 4-7: softmax; 8: loads; 9: products
 constexpr int STAGE_BYTES = 2 * TILE * D;        // key tile, value tile
-constexpr int STAGES = 6;
 constexpr float SLACK = 6.0f;                    // a tile may exceed the reference by 2^6
 constexpr float HEAD = 2.0f;                     // weights at the reference are 4: 2^(HEAD + SLACK) = 256 <= 448
 constexpr int PIECE = 6;                         // tiles (~0.4 us each) that beginning and ending a piece takes: ~2.5 us
@@ -39,11 +39,14 @@ constexpr int MAX_CTAS = 512;                    // shares that the join kernel 
 
 constexpr int up16(int n) { return (n + 15) / 16 * 16; }
 
-template <int NR, int QT> struct Shape {
-  static constexpr int NQ = up16(NR * QT), NP = up16(NR * TERMS);
-  static constexpr int COLS = 2 * NQ + 2 * NP;   // S^T and O^T of even and odd tiles
-  static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : 256;
+// NR: rows of a softmax thread; SPLIT: the two warpgroups have NR rows each.
+template <int NR, int QT, bool SPLIT> struct Shape {
+  static constexpr int RT = SPLIT ? 2 * NR : NR;
+  static constexpr int NQ = up16(RT * QT), NP = up16(RT * TERMS);
+  static constexpr int COLS = 2 * NQ + (SPLIT ? 1 : 2) * NP;     // S^T of even and odd tiles, then O^T
+  static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static_assert(COLS <= TMEM, "tensor memory");
+  static constexpr int STAGES = SPLIT ? 5 : 6;
   // byte offsets in dynamic shared memory (1024-byte aligned operands first)
   static constexpr int Q = STAGES * STAGE_BYTES, P = Q + (NQ * D + 1023) / 1024 * 1024, END = P + 2 * NP * TILE;
   static constexpr int SMEM = END + 1024;        // room to align
@@ -67,20 +70,21 @@ template <typename T> __device__ __forceinline__ void unpack4(uint2 v, float (&x
   for (int i = 0; i < 4; ++i) x[i] = to_f32(e[i]);
 }
 
-template <typename T, int NR, int QT>
+template <typename T, int NR, int QT, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant__ CUtensorMap map,
                                                           const __grid_constant__ Args a) {
-  using S = Shape<NR, QT>;
+  using S = Shape<NR, QT, SPLIT>;
+  constexpr int STAGES = S::STAGES, RT = S::RT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t sbase = tc::smem_u32(smem);
   __shared__ __align__(8) uint64_t bars[2 * STAGES + 10];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
-  __shared__ float s_rs[NR];                     // scale of a row's scores: 2^e log2(e) / sqrt(128)
+  __shared__ float s_rs[RT];                     // scale of a row's scores: 2^e log2(e) / sqrt(128)
   __shared__ float s_top[2][4][NR];              // a tile's largest s + log2 vs, by warpgroup and warp
   // at a row's end: references; denominators by warp; then the denominator, its reference, and what brings O^T there
-  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[NR], s_ref[NR], s_f[2][NR];
+  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[RT], s_ref[RT], s_f[2][RT];
   const uint32_t bar0 = tc::smem_u32(bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   auto empty = [&](uint32_t s) { return bar0 + 8 * (STAGES + s); };
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     if (lane == 0) {
       for (int s = 0; s < STAGES; ++s) tc::mbar_init(full(s), 1), tc::mbar_init(empty(s), 1);
       for (int k = 0; k < 2; ++k)
-        tc::mbar_init(s_full(k), 1), tc::mbar_init(s_free(k), 4), tc::mbar_init(p_full(k), 4), tc::mbar_init(p_free(k), 1);
+        tc::mbar_init(s_full(k), 1), tc::mbar_init(s_free(k), SPLIT ? 8 : 4), tc::mbar_init(p_full(k), SPLIT ? 8 : 4), tc::mbar_init(p_free(k), 1);
       tc::mbar_init(q_full, 8);
       tc::mbar_init(drain, 1);
       tc::fence_mbar_init();
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       if (tc::elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < TILE / 32; ++kk)    // 32 tokens a step: 4 groups of 8 value rows, 4 core matrices of weights
-          tc::mma_fp8(tmu + 2 * S::NQ + ku * S::NP, dv + kk * (32 * D / 16), dp + kk * (4 * 128 / 16), id_o, kk > 0 || accumulate);
+          tc::mma_fp8(tmu + 2 * S::NQ + (SPLIT ? 0 : ku * S::NP), dv + kk * (32 * D / 16), dp + kk * (4 * 128 / 16), id_o, kk > 0 || accumulate);
         tc::mma_commit(empty(vu));
         tc::mma_commit(p_free(ku));
       }
@@ -181,7 +185,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       const uint32_t i0 = i, n = w.j1 - w.j0;
       for (; i < i0 + n + 2 && ok; ++i) {
         if (i < i0 + n) scores(i);
-        if (ok && i >= i0 + 2) values(i - 2, i >= i0 + 4);
+        if (ok && i >= i0 + 2) values(i - 2, i >= i0 + (SPLIT ? 3 : 4));
       }
       i = i0 + n;
     }
@@ -191,11 +195,12 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       while (!tc::mbar_try(drain, 0) && tc::now_ns() - t0 < tc::WAIT_LIMIT_NS) {}
     }
   } else {
-    // ---- softmax: warpgroup g has the tiles i = g mod 2 of the share; thread = token of the tile; lane of tensor memory =
-    // token of S^T, dim of O^T
+    // ---- softmax: warpgroup g has the tiles i = g mod 2 of the share, or (SPLIT) rows g NR .. of every tile; thread = token
+    // of the tile; lane of tensor memory = token of S^T, dim of O^T
     const int R = rows_of(a), late = (int)a.T - 1, g = warp >> 2, t = tid & (GROUP - 1);
+    const int first = SPLIT ? g * NR : 0;         // this thread's rows: first + (0 .. NR - 1)
     // A warp brings every eighth row of q, a lane 4 dims of it; the share's first row ahead of everything else.
-    constexpr int QR = (NR + 7) / 8;
+    constexpr int QR = (RT + 7) / 8;
     uint2 qv[QR];
     auto q_at = [&](int r, int h) {               // rows are token-major: row = token * G + head
       const int tt = late ? r / a.G : 0;
@@ -220,10 +225,10 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     tc::launch_dependents();
     const uint32_t tm = s_tmem;
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tm_s = tm + g * S::NQ + my, tm_o = tm + 2 * S::NQ + my;
-    uint8_t* pb = smem + S::P + g * S::NP * TILE + t * 16;
+    const uint32_t tm_s = tm + first + my, tm_o = tm + 2 * S::NQ + first + my;
+    uint8_t* const pb = smem + S::P + t * 16;
     uint32_t i0 = 0;                              // the share's tiles before this row
-    bool ok = true, bad = false;                  // ok: this thread's waits; bad: some thread's gave up (uniform)
+    bool ok = true, bad = false;                  // ok: this thread's waits; bad: some thread's gave up
     while (more) {
       const int h = w.bh % a.Hkv, n = w.j1 - w.j0;
       // this row's queries as terms.  The products of the row before are complete (its O^T was read below), so its q
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
         for (int term = 0; term < QT; ++term) {
           const uint32_t code = kv8_encode2(x[0], x[1]) | kv8_encode2(x[2], x[3]) << 16;
-          const int c = term * NR + r;
+          const int c = term * RT + r;
           *reinterpret_cast<uint32_t*>(smem + S::Q + c * D + (((lane >> 2) ^ (c & 7)) << 4) + (lane & 3) * 4) = code;
           const float2 lo = kv8_decode2(code), hi = kv8_decode2(code >> 16);
           x[0] = (x[0] - lo.x) * 16.0f, x[1] = (x[1] - lo.y) * 16.0f;
@@ -259,39 +264,40 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       // a row's reference; its scale; this thread's denominator and that one's reference
       float m[NR], rs[NR], lm[NR], l[NR];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) m[r] = -INFINITY, lm[r] = -1e30f, l[r] = 0.0f, rs[r] = r < R ? s_rs[r] : 0.0f;
+      for (int r = 0; r < NR; ++r) m[r] = -INFINITY, lm[r] = -1e30f, l[r] = 0.0f, rs[r] = first + r < R ? s_rs[first + r] : 0.0f;
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       auto scale_of = [&](int tile) {
         const int tok = tile * TILE + t;
         return tok < w.end ? sc[tok / BLK] : make_float2(0.0f, 1.0f);
       };
-      const uint32_t mine = i0 + ((i0 ^ g) & 1);  // this warpgroup's first tile of the row
+      constexpr uint32_t STEP = SPLIT ? 1 : 2;
+      const uint32_t mine = SPLIT ? i0 : i0 + ((i0 ^ g) & 1);      // this warpgroup's first tile of the row
       float2 next_scale = scale_of(w.j0 + (int)(mine - i0));
       uint32_t i = mine;
-      for (; i < i0 + n && !bad; i += 2) {
+      for (; i < i0 + n; i += STEP) {             // to the end also when a wait gave up: barriers stay in step
         const int tile = w.j0 + (int)(i - i0), tok = tile * TILE + t;
-        const uint32_t use = i >> 1;              // uses of this warpgroup's buffers before
+        const uint32_t use = i >> 1, k = SPLIT ? i & 1 : g;        // uses of the buffers before; the buffers
         const float2 ks = next_scale;
-        next_scale = scale_of(tile + 2);          // read two tiles ahead
+        next_scale = scale_of(tile + STEP);       // read ahead
         const float lv = (float)((int)(__float_as_uint(ks.y) >> 23) - 127);      // log2 of the value scale
-        ok = ok && tc::mbar_wait(s_full(g), use & 1, gave_up);
+        ok = ok && tc::mbar_wait(s_full(k), use & 1, gave_up);
         __syncwarp();
         tc::fence_after();
         float s[NR];
         {
           uint32_t c[QT][NR];
 #pragma unroll
-          for (int term = 0; term < QT; ++term) tc::Tmem<NR>::ld(tm_s + term * NR, c[term]);
+          for (int term = 0; term < QT; ++term) tc::Tmem<NR>::ld(tm_s + k * S::NQ + term * RT, c[term]);
           tc::wait_ld();
           tc::fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(s_free(g));
+          if (lane == 0) tc::mbar_arrive(s_free(k));
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             float v = __uint_as_float(c[QT - 1][r]);
 #pragma unroll
             for (int term = QT - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[term][r]));
-            s[r] = r < R ? v * (ks.x * rs[r]) : -INFINITY;
+            s[r] = first + r < R ? v * (ks.x * rs[r]) : -INFINITY;
           }
         }
         // keys that a row does not see: past the end, or in the last T - 1 after its own
@@ -311,25 +317,25 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
               for (int e = 0; e < 4; ++e) nan_v = nan_v || __vcmpeq4(x[e] & 0x7F7F7F7Fu, 0x7F7F7F7Fu) != 0;
             }
           }
+          if (SPLIT) tc::named_sync(5, 2 * GROUP);             // both warpgroups have looked at the row
           if (void_row || nan_v) {
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) vrow[c] = make_uint4(0, 0, 0, 0);
           }
-          int room = w.end - tok - late, head = 0;        // seen by the queries whose token is above -room
+          int room = w.end - tok - late + first / a.G, head = first % a.G;        // seen by the queries whose token is above -room
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             if (room <= 0) s[r] = -INFINITY;
-            else if (nan_v && r < R) l[r] = __uint_as_float(0x7FFFFFFFu);
+            else if (nan_v && first + r < R) l[r] = __uint_as_float(0x7FFFFFFFu);
             if (++head == a.G) head = 0, ++room;
           }
           __syncwarp();
         }
-        ok = ok && tc::mbar_wait(p_free(g), (use & 1) ^ 1, gave_up);   // the product of this warpgroup's tile before
+        ok = ok && tc::mbar_wait(p_free(k), (use & 1) ^ 1, gave_up);   // the product that read this weight buffer
         bool above = !ok;
 #pragma unroll
         for (int r = 0; r < NR; ++r) above = above || s[r] + lv > m[r] + SLACK;
         if (tc::named_or(1 + g, GROUP, above)) {
-          bad = tc::uniform(tc::named_or(1 + g, GROUP, !ok));
           // some row outgrew its reference: the tile's largest becomes every row's
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
@@ -347,15 +353,18 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
           }
           tc::named_sync(1 + g, GROUP);
           if (i != mine) {
+            // O^T of the tiles before is complete
+            if (SPLIT) ok = ok && tc::mbar_wait(p_free(k ^ 1), ((i - 1) >> 1) & 1, gave_up);
+            __syncwarp();
             tc::fence_after();
 #pragma unroll
             for (int term = 0; term < TERMS; ++term) {
               uint32_t o[NR];
-              tc::Tmem<NR>::ld(tm_o + g * S::NP + term * NR, o);
+              tc::Tmem<NR>::ld(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
               tc::wait_ld();
 #pragma unroll
               for (int r = 0; r < NR; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * f[r]);
-              tc::Tmem<NR>::st(tm_o + g * S::NP + term * NR, o);
+              tc::Tmem<NR>::st(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
             }
             tc::wait_st();
           }
@@ -385,20 +394,22 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             y = __hmul2(__hsub2(y, *reinterpret_cast<const __half2*>(&c)), sixteen);
           }
         }
+        // columns term * RT + first + r; with NR = 16 a term's rows are a 16-byte piece of their own
+        constexpr int PIECES = SPLIT ? TERMS : S::NP / 16;
 #pragma unroll
-        for (int c = 0; c < S::NP / 16; ++c) {
+        for (int c = 0; c < PIECES; ++c) {
           uint32_t x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = 4 * c + e < TERMS * NR / 4 ? codes[4 * c + e < TERMS * NR / 4 ? 4 * c + e : 0] : 0;
-          *reinterpret_cast<uint4*>(pb + c * TILE * 16) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4*>(pb + k * S::NP * TILE + (SPLIT ? 2 * c + g : c) * TILE * 16) = make_uint4(x[0], x[1], x[2], x[3]);
         }
         tc::fence_async_smem();
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_full(g));
+        if (lane == 0) tc::mbar_arrive(p_full(k));
       }
       // the row's part (or whole): denominators over the threads, O^T out of tensor memory
-      if (i != mine) ok = ok && tc::mbar_wait(p_free(g), ((i - 2) >> 1) & 1, gave_up);
+      if (i != mine) ok = ok && tc::mbar_wait(p_free((i - STEP) & 1), ((i - STEP) >> 1) & 1, gave_up);
       __syncwarp();
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
@@ -413,39 +424,46 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       const Walk now = w;
       more = w.next();
       if (more) load_q();                         // the next row's q, on its way while this one is finished
-      if (tid < NR) {
-        float mx = s_lm[0][tid], sum = 0.0f;
+      if (tid < RT) {
+        // the warps that have the row, and its place among their rows
+        const int v0 = SPLIT ? tid / NR * 4 : 0, r = SPLIT ? tid % NR : tid;
+        constexpr int NV = SPLIT ? 4 : 8;
+        float mx = s_lm[v0][r], sum = 0.0f;
 #pragma unroll
-        for (int v = 1; v < 8; ++v) mx = fmaxf(mx, s_lm[v][tid]);
+        for (int v = 1; v < NV; ++v) mx = fmaxf(mx, s_lm[v0 + v][r]);
 #pragma unroll
-        for (int v = 0; v < 8; ++v) sum = fmaf(s_l[v][tid], ex2(s_lm[v][tid] - mx), sum);
+        for (int v = 0; v < NV; ++v) sum = fmaf(s_l[v0 + v][r], ex2(s_lm[v0 + v][r] - mx), sum);
         s_sum[tid] = sum;
         s_ref[tid] = mx;
         // O^T is relative to m - HEAD: both come to the denominator's reference.  A warpgroup that had no tile left its
         // columns as they were.
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          s_f[k][tid] = (n == 1 && k != (int)(i0 & 1)) || s_m[k][tid] == -INFINITY ? 0.0f : exp2f(s_m[k][tid] - HEAD - mx);
+        for (int k = 0; k < (SPLIT ? 1 : 2); ++k) {
+          const float m0 = s_m[SPLIT ? tid / NR : k][r];
+          s_f[k][tid] = (!SPLIT && n == 1 && k != (int)(i0 & 1)) || m0 == -INFINITY ? 0.0f : exp2f(m0 - HEAD - mx);
+        }
       }
-      uint32_t c[2][TERMS][NR];
+      constexpr int NO = SPLIT ? 1 : 2;           // accumulators that hold the row
+      uint32_t c[NO][TERMS][NR];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < NO; ++k) {
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) tc::Tmem<NR>::ld(tm_o + k * S::NP + term * NR, c[k][term]);
+        for (int term = 0; term < TERMS; ++term) tc::Tmem<NR>::ld(tm_o + k * S::NP + term * RT, c[k][term]);
       }
       tc::wait_ld();
       tc::fence_before();
       tc::named_sync(3, 2 * GROUP);
       const bool whole = now.j0 == 0 && now.j1 == now.n;
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        if (r >= R || (r & 1) != g) continue;     // warpgroup g finishes the rows r = g mod 2
+      for (int rr = 0; rr < NR; ++rr) {
+        const int r = first + rr;
+        if (r >= R || (!SPLIT && (r & 1) != g)) continue;      // warpgroup g finishes the rows r = g mod 2, or its own
         float x = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float v = __uint_as_float(c[k][TERMS - 1][r]);
+        for (int k = 0; k < NO; ++k) {
+          float v = __uint_as_float(c[k][TERMS - 1][rr]);
 #pragma unroll
-          for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][r]));
+          for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][rr]));
           if (s_f[k][r] != 0.0f) x = fmaf(v, s_f[k][r], x);
         }
         const float sum = s_sum[r];
@@ -524,14 +542,14 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
 
-template <typename T, int NR, int QT>
+template <typename T, int NR, int QT, bool SPLIT>
 int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
-  using S = Shape<NR, QT>;
+  using S = Shape<NR, QT, SPLIT>;
   static_assert(S::SMEM <= 224 * 1024, "shared memory");
   static std::atomic<uint64_t> told{0};
-  const int r = allow_smem(token_kernel<T, NR, QT>, S::SMEM, told, "kv8_attend");
+  const int r = allow_smem(token_kernel<T, NR, QT, SPLIT>, S::SMEM, told, "kv8_attend");
   if (r != FATHOM_OK) return r;
-  token_kernel<T, NR, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
+  token_kernel<T, NR, QT, SPLIT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
   if (a.share && a.share == a.stride) return check_launch("kv8_attend");     // every row whole: nothing to join
   return launch_join(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, a, ctas, st);
 }
@@ -539,9 +557,10 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
 template <typename T, int QT>
 int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   const int64_t R = a.G * a.T;
-  if (R <= 4) return launch<T, 4, QT>(map, a, ctas, st);
-  if (R <= 8) return launch<T, 8, QT>(map, a, ctas, st);
-  return launch<T, 16, QT>(map, a, ctas, st);
+  if (R <= 4) return launch<T, 4, QT, false>(map, a, ctas, st);
+  if (R <= 8) return launch<T, 8, QT, false>(map, a, ctas, st);
+  if (R <= 16) return launch<T, 16, QT, false>(map, a, ctas, st);
+  return launch<T, 16, QT, true>(map, a, ctas, st);
 }
 
 }  // namespace

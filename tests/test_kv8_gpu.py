@@ -174,7 +174,8 @@ def test_read_beyond_32_bit_offsets():
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("G,T,n", [(4, 1, 1), (4, 1, 63), (4, 1, 64), (1, 1, 65), (7, 1, 129), (8, 1, 700), (5, 1, 1111),
                                    (12, 1, 300), (33, 1, 200), (4, 2, 130), (4, 5, 387), (1, 33, 100), (7, 8, 250),
-                                   (4, 64, 64), (2, 130, 257), (3, 100, 40), (4, 70, 900), (1, 300, 300)])
+                                   (4, 64, 64), (2, 130, 257), (3, 100, 40), (4, 70, 900), (1, 300, 300),
+                                   (8, 4, 300), (1, 17, 64), (32, 1, 1500), (3, 10, 11), (5, 6, 129)])
 def test_attend_matches_the_oracle(dtype, G, T, n):
     B, H = 2, 2
     c, rows, scales = _filled(B, H, n, G * T + n, cap=n + 70)
@@ -186,7 +187,7 @@ def test_attend_matches_the_oracle(dtype, G, T, n):
     _close(out, ref, mag)
 
 
-@pytest.mark.parametrize("T", [1, 3, 40, 129])
+@pytest.mark.parametrize("T", [1, 3, 7, 40, 129])
 def test_attend_at_device_lengths(T):
     """Ragged lengths on the device: none, one, fewer than the queries, a block's edge, the whole cache, above it."""
     ends = [0, 1, 2, 64, 65, 191, 192, 500, 640, 10 ** 12, -3]
@@ -199,7 +200,7 @@ def test_attend_at_device_lengths(T):
     assert not out[0].any() and not out[-1].any()       # rows that see nothing
 
 
-@pytest.mark.parametrize("T", [1, 4, 80])
+@pytest.mark.parametrize("T", [1, 4, 6, 80])
 def test_attend_splits_a_long_context(T):
     n, G = 20011, 4
     c, rows, scales = _filled(1, 1, n, 11)
@@ -224,7 +225,7 @@ def test_attend_peaked_and_flat_weights():
     c = KVCache8(1, 2, n)
     c.write(K, V)
     for amp in (0.0, 1.0, 60.0):
-        for T in (1, 50):
+        for T in (1, 3, 6, 50):
             q = (amp * torch.randn(1, 2 * G, T, 128, generator=torch.Generator().manual_seed(13))).bfloat16()
             ref, mag = O.attend(_np(q), c.rows.cpu().numpy(), c.scales.cpu().numpy(), [n], 2)
             _close(c.attend(q.cuda(), n), ref, mag)
