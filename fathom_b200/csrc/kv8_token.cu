@@ -443,41 +443,47 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
           s_f[k][tid] = (!SPLIT && n == 1 && k != (int)(i0 & 1)) || m0 == -INFINITY ? 0.0f : exp2f(m0 - HEAD - mx);
         }
       }
-      constexpr int NO = SPLIT ? 1 : 2;           // accumulators that hold the row
-      uint32_t c[NO][TERMS][NR];
-#pragma unroll
-      for (int k = 0; k < NO; ++k) {
-#pragma unroll
-        for (int term = 0; term < TERMS; ++term) tc::Tmem<NR>::ld(tm_o + k * S::NP + term * RT, c[k][term]);
-      }
-      tc::wait_ld();
-      tc::fence_before();
       tc::named_sync(3, 2 * GROUP);
       const bool whole = now.j0 == 0 && now.j1 == now.n;
-#pragma unroll
-      for (int rr = 0; rr < NR; ++rr) {
-        const int r = first + rr;
-        if (r >= R || (!SPLIT && (r & 1) != g)) continue;      // warpgroup g finishes the rows r = g mod 2, or its own
-        float x = 0.0f;
+      // warpgroup g finishes its own rows, or of 4 rows r = g mod 2 (4 at a time: run once a row, small code is fast code)
+#pragma unroll 1
+      for (int r0 = 0; r0 < NR; r0 += 4) {
+        constexpr int NO = SPLIT ? 1 : 2;         // accumulators that hold the row
+        uint32_t c[NO][TERMS][4];
+        __syncwarp();
 #pragma unroll
         for (int k = 0; k < NO; ++k) {
-          float v = __uint_as_float(c[k][TERMS - 1][rr]);
 #pragma unroll
-          for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][rr]));
-          if (s_f[k][r] != 0.0f) x = fmaf(v, s_f[k][r], x);
+          for (int term = 0; term < TERMS; ++term) tc::Tmem<4>::ld(tm_o + k * S::NP + term * RT + r0, c[k][term]);
         }
-        const float sum = s_sum[r];
-        if (bad) x = __uint_as_float(0x7FFFFFFFu);
-        if (whole) {
-          const int tt = late ? r / a.G : 0;
-          T* op = reinterpret_cast<T*>(a.out) + now.b * a.ob + (int64_t)(h * a.G + r - tt * a.G) * a.oh + tt * a.ot;
-          from_f32(bad ? x : sum == 0.0f ? 0.0f : x / sum, op + t);
-        } else {
-          float* part = a.part + (((int64_t)blockIdx.x + now.bh) * R + r) * PART;
-          part[t] = x;
-          if (t == 0) part[D] = s_ref[r], part[D + 1] = sum;
+        tc::wait_ld();
+#pragma unroll
+        for (int rr = 0; rr < 4; ++rr) {
+          const int r = first + r0 + rr;
+          if (r >= R || (!SPLIT && (rr & 1) != g)) continue;
+          float x = 0.0f;
+#pragma unroll
+          for (int k = 0; k < NO; ++k) {
+            float v = __uint_as_float(c[k][TERMS - 1][rr]);
+#pragma unroll
+            for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][rr]));
+            if (s_f[k][r] != 0.0f) x = fmaf(v, s_f[k][r], x);
+          }
+          const float sum = s_sum[r];
+          if (bad) x = __uint_as_float(0x7FFFFFFFu);
+          if (whole) {
+            const int tt = late ? r / a.G : 0;
+            T* op = reinterpret_cast<T*>(a.out) + now.b * a.ob + (int64_t)(h * a.G + r - tt * a.G) * a.oh + tt * a.ot;
+            from_f32(bad ? x : sum == 0.0f ? 0.0f : x / sum, op + t);
+          } else {
+            float* part = a.part + (((int64_t)blockIdx.x + now.bh) * R + r) * PART;
+            part[t] = x;
+            if (t == 0) part[D] = s_ref[r], part[D + 1] = sum;
+          }
         }
       }
+      tc::fence_before();
+      tc::named_sync(3, 2 * GROUP);               // both warpgroups have read O^T: the next row may overwrite it
       i0 += n;
     }
   }
