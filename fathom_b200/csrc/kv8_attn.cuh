@@ -26,9 +26,10 @@ struct Args {
   int64_t T;
   float* part;                    // workspace: partial results
   unsigned long long* timeouts;   // counts waits that gave up
-  // Set by plan_shares (kv8_line.cuh) where every row bh is one item of the same length: tiles per CTA, and the
-  // distance of two items in the line.  0: the device cuts the line.
-  int share, stride;
+  // Set by plan_shares (kv8_line.cuh) where the lengths are known to the host: tiles per CTA, and the distance of two
+  // items in the line.  share = 0: the device cuts the line, into shares of at least `least` tiles.
+  int share, stride, least;
+  int ctas;                       // of the prompt kernel
 };
 
 // Tokens of sequence b that exist.

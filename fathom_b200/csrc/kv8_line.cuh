@@ -2,8 +2,8 @@
 //
 // An item is up to 256 query rows (token-major pairs of token and head) of one cache row bh; its tiles are the 128-token
 // stretches up to the last key that any of its rows sees.  Items follow each other by bh, then by row; CTA c of C
-// takes tiles [c * share, (c + 1) * share) of the line, share = ceil(tiles / C), whatever the lengths are.  Where every
-// bh is one item of the same length, items may lie further apart than their tiles, so that no CTA has pieces of two.
+// takes tiles [c * share, (c + 1) * share) of the line, share = ceil(tiles / C), whatever the lengths are.  Where
+// the host knows them, items may lie further apart than their tiles, so that no CTA has pieces of two.
 #pragma once
 #include "kv8_attn.cuh"
 #include "tc.cuh"
@@ -108,17 +108,25 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int d) {
   return n >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
 }
 
-// One warp: where this CTA's share begins, and how many tiles it has (0 or less: none).  A token's latency counts on
+// Tiles per CTA where the device cuts the line: at least `least`, or an item's where those are fewer.
+__device__ __forceinline__ int64_t share_of(const Args& a, int64_t total, int ctas) {
+  const int64_t share = quotient(total + ctas - 1, ctas);
+  return share >= a.least ? share : max(share, min((int64_t)a.least, quotient(total, a.B * a.Hkv * items_per_bh(a))));
+}
+
+// One warp: where this CTA's share begins, how many tiles it has (0 or less: none) and how many a CTA has at most.  A token's latency counts on
 // this: the common forms, a plan or up to 32 sequences of one item per bh, take one pass.
-__device__ inline Place my_share(const Args& a, int* count) {
+__device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
   const int lane = threadIdx.x & 31;
   Place p{0, 0};
   if (a.share) {
-    const int64_t at = (int64_t)a.share * blockIdx.x, items = (int64_t)a.B * a.Hkv;
+    const int64_t at = (int64_t)a.share * blockIdx.x;
+    *per_cta = a.share;
     p.item = (int)quotient(at, a.stride);
     p.tile = (int)(at - (int64_t)p.item * a.stride);
-    const int nt = tiles_of(a, seq_end(a, 0), 0);
-    *count = (int)min((int64_t)a.share, a.stride > nt ? (int64_t)nt - p.tile : items * nt - at);
+    const int nt = tiles_of(a, seq_end(a, 0), p.item % items_per_bh(a));
+    const bool apart = a.stride > nt || a.share == a.stride;       // no other item's tiles in this share
+    *count = (int)min((int64_t)a.share, apart ? (int64_t)nt - p.tile : (int64_t)a.B * a.Hkv * nt - at);
     return p;
   }
   if (items_per_bh(a) == 1 && a.B <= 32) {       // (ragged: equal lengths have a plan)
@@ -130,8 +138,9 @@ __device__ inline Place my_share(const Args& a, int* count) {
       const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    const int64_t total = __shfl_sync(0xffffffffu, x, 31), share = quotient(total + gridDim.x - 1, gridDim.x);
+    const int64_t total = __shfl_sync(0xffffffffu, x, 31), share = share_of(a, total, gridDim.x);
     int64_t at = share * blockIdx.x;
+    *per_cta = (int)share;
     *count = (int)min(share, total - at);
     if (*count <= 0) return p;
     const int b = __ffs(__ballot_sync(0xffffffffu, x > at)) - 1;     // the first sequence that ends past `at`
@@ -139,7 +148,8 @@ __device__ inline Place my_share(const Args& a, int* count) {
     const int n = __shfl_sync(0xffffffffu, nt, b), bh = (int)quotient(at, n);
     return Place{b * a.Hkv + bh, (int)(at - (int64_t)bh * n)};
   }
-  const int64_t total = line(a, -1, &p), share = quotient(total + gridDim.x - 1, gridDim.x), first = share * blockIdx.x;
+  const int64_t total = line(a, -1, &p), share = share_of(a, total, gridDim.x), first = share * blockIdx.x;
+  *per_cta = (int)share;
   *count = (int)min(share, total - first);
   if (*count > 0) line(a, first, &p);
   return p;
@@ -171,21 +181,25 @@ struct Walk {
   }
 };
 
-// Where every bh is one item of the same length (known here): cuts the line for at most `most` CTAs and returns their
-// number; else leaves it to the device and returns `most`.  Either the items follow each other, and a CTA may have
-// pieces of two, or each has k CTAs of its own; beginning and ending a piece takes as long as `piece` tiles.
-inline int plan_shares(Args& a, int most, int piece) {
-  if (a.end_dev || a.G * a.T > ROWS) return most;
-  const int64_t items = (int64_t)a.B * a.Hkv, nt = a.end > TILE ? cdiv(a.end, TILE) : 1;
-  if (items > most) {
-    a.share = (int)cdiv(items * nt, most);
-    a.stride = (int)nt;
-    return (int)cdiv(items * nt, a.share);
+// Cuts the line for at most `most` CTAs at a time and returns the grid.  Where the host knows the lengths:
+//  * items of at most `whole` tiles have a CTA each, and nothing is to be joined;
+//  * else, where every bh is one item, the items follow each other, and a CTA may have pieces of two, or each has k CTAs of
+//    its own: whichever takes the fewer tiles, beginning and ending a piece taking as long as `piece`.
+// All other lines are left to the device.  Shares have at least `least` tiles.
+inline int plan_shares(Args& a, int most, int piece, int whole, int least) {
+  a.least = least;
+  if (a.end_dev) return most;
+  const int64_t per = (a.G * a.T - 1) / ROWS + 1, items = (int64_t)a.B * a.Hkv * per, nt = a.end > TILE ? cdiv(a.end, TILE) : 1;
+  if (nt <= whole) {
+    a.share = a.stride = (int)nt;
+    return (int)items;
   }
-  const int64_t k = most / items < nt ? most / items : nt, own = cdiv(nt, k), dense = cdiv(items * nt, most);
-  const bool apart = own <= dense + piece;
-  a.share = (int)(apart ? own : dense);
-  a.stride = (int)(apart ? own * k : nt);
+  if (per > 1) return most;
+  const int64_t dense = cdiv(items * nt, most) > least ? cdiv(items * nt, most) : least;
+  const int64_t fit = most / items, k = fit < cdiv(nt, least) ? fit : cdiv(nt, least);
+  const bool apart = k >= 1 && cdiv(nt, k) <= dense + piece;
+  a.share = (int)(apart ? cdiv(nt, k) : dense);
+  a.stride = (int)(apart ? a.share * k : nt);
   return (int)cdiv(items * a.stride, a.share);
 }
 

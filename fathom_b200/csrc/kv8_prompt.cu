@@ -38,6 +38,8 @@ constexpr float HEAD = 3.0f;                 // weights at the reference are 2^3
 constexpr int REG_LAUNCH = 80, REG_SOFT = 88, REG_VALUE = 64, REG_OTHER = 64;
 static_assert(4 * REG_SOFT + REG_VALUE + REG_OTHER <= 6 * REG_LAUNCH, "register split");
 constexpr int PIECE = 4;                     // tiles (~1.7 us each) that beginning and ending a piece takes
+constexpr int LEAST = 4;                     // so shares are no shorter
+constexpr int WHOLE = 6;                     // tiles that take no longer than their halves and the second kernel
 constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
 
 template <int QT> struct Shape {
@@ -70,6 +72,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 template <int N> __device__ __forceinline__ void reg_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void reg_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
+// What a CTA's share left to join, after the parts (two slots per CTA): see prompt_join_kernel.
+__device__ __forceinline__ int4* cuts_of(const Args& a) { return reinterpret_cast<int4*>(a.part + 2 * (int64_t)a.ctas * ROWS * PART); }
 
 template <typename T, int QT>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constant__ CUtensorMap map,
@@ -108,8 +113,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     s_gave_up = 0;
   }
   if (warp == 20) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
-  int count;
-  const Place place = my_share(a, &count);
+  int count, share;
+  const Place place = my_share(a, &count, &share);
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -126,7 +131,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     const uint32_t tm_s = tm + h2 * 128 + 64 * ch + my, tm_o = tm + 256 + h2 * 128 + 64 * ch + my;
     uint32_t phase = 0, vt = 0;                    // completions of s_full seen; tiles seen
     bool ok = true;
+    int4 cut = make_int4(-1, 0, 0, 0);             // the item that this share begins and another ends
     while (w.next()) {
+      if (w.j0 == 0 && w.j1 < w.n) cut = make_int4(w.item - 1, w.n, w.j1, share);
       if (w.halves() <= h2) {                      // no row in this half
         vt += w.j1 - w.j0;
         continue;
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       __syncwarp();
       tc::fence_before();
     }
+    if (tid == 0 && (!a.share || a.share != a.stride)) cuts_of(a)[blockIdx.x] = cut;
   } else if (group == 4) {
     // ---- values: e4m3 rows from memory to f16, MN-major tiles of two 64-dim halves.  Thread = 16 dims of 8 tokens.
     reg_less<REG_VALUE>();
@@ -506,54 +514,47 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   if (tid == 0 && s_gave_up) atomicAdd(a.timeouts, 1ull);
 }
 
-// Joins the items that shares cut: block (c, rows) looks at the cut before share c + 1, and joins the item it
-// falls into if that is the item's first cut.  Warp = row, lane = 4 dims.
-constexpr int JOIN_WARPS = 8;
+// Joins the items that shares cut: block (c, ..) the one that share c begins and does not end.  Warp = row, lane = 4 dims.
+constexpr int JOIN_WARPS = 8, JOIN_BLOCKS = 16;    // blocks per cut
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args a, int ctas) {
-  __shared__ Place s_place;
-  __shared__ int64_t s_total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = items_per_bh(a);
-  if (!a.share && warp == 0) {
-    Place p{0, 0};
-    const int64_t total = line(a, -1, &p), cut = quotient(total + ctas - 1, ctas) * (blockIdx.x + 1);
-    if (cut < total) line(a, cut, &p);
-    if (lane == 0) s_place = p, s_total = total;
-  }
-  __syncthreads();
-  Place p = s_place;
-  int64_t share = a.share, cut = share * (blockIdx.x + 1), length = (int64_t)a.B * a.Hkv * a.stride;
-  if (a.share) {
-    p.item = (int)quotient(cut, a.stride);
-    p.tile = (int)(cut - (int64_t)p.item * a.stride);
-    if (p.tile >= tiles_of(a, seq_end(a, 0), 0)) p.tile = 0;        // between two items
-  } else {
-    length = s_total, share = quotient(length + ctas - 1, ctas), cut = share * (blockIdx.x + 1);
-  }
   tc::wait_dependency();                           // the parts are written; and nothing ends before they are
-  if (cut >= length || p.tile == 0 || p.tile > share) return;    // no item is cut here, or an earlier cut joins it
-  const int bh = p.item / per, it = p.item % per, b = bh / a.Hkv, total = rows_of(a);
-  const int64_t first = cut - p.tile;              // the item's first tile in the line
-  const int c0 = blockIdx.x, c1 = (int)((first + tiles_of(a, seq_end(a, b), it) - 1) / share);
-  const int r = blockIdx.y * JOIN_WARPS + warp, row = it * ROWS + r;
-  if (row >= total) return;
-  // parts: share c0 holds the item's first tiles (its second slot), the others begin with it (first slot)
-  auto part = [&](int c) { return a.part + ((2 * (int64_t)c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
-  float M = -INFINITY, L = 0.0f;
-  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int c = c0; c <= c1; ++c) M = fmaxf(M, part(c)[D]);
-  for (int c = c0; c <= c1; ++c) {
-    const float m = part(c)[D], e = m == -INFINITY ? 0.0f : exp2f(m - M);
-    const float4 o = *reinterpret_cast<const float4*>(part(c) + 4 * lane);
-    L = fmaf(part(c)[D + 1], e, L);
-    O.x = fmaf(o.x, e, O.x), O.y = fmaf(o.y, e, O.y), O.z = fmaf(o.z, e, O.z), O.w = fmaf(o.w, e, O.w);
+  const int4 cut = cuts_of(a)[blockIdx.x];         // item, its tiles, those in share c, tiles per share
+  if (cut.x < 0) return;
+  const int bh = cut.x / per, it = cut.x % per, b = bh / a.Hkv, total = rows_of(a);
+  const int c0 = blockIdx.x, c1 = c0 + (cut.y - cut.z + cut.w - 1) / cut.w;
+  for (int r = blockIdx.y * JOIN_WARPS + warp; r < ROWS; r += JOIN_BLOCKS * JOIN_WARPS) {
+    const int row = it * ROWS + r;
+    if (row >= total) return;
+    // parts: share c0 holds the item's first tiles (its second slot), the others begin with it (first slot)
+    auto part = [&](int c) { return a.part + ((2 * (int64_t)c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
+    // lane = part, 32 at a time, with a running reference
+    float M = -INFINITY, L = 0.0f;
+    float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = c0; c <= c1; c += 32) {
+      const int n = min(32, c1 - c + 1);
+      const float2 ml = lane < n ? *reinterpret_cast<const float2*>(part(c + lane) + D) : make_float2(-INFINITY, 0.0f);
+      const float top = fmaxf(M, warp_max(ml.x)), f = M == -INFINITY ? 0.0f : ex2(M - top);
+      const float e = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+      M = top;
+      L = fmaf(L, f, ml.y * e);
+      O = make_float4(O.x * f, O.y * f, O.z * f, O.w * f);
+#pragma unroll 8
+      for (int v = 0; v < n; ++v) {
+        const float4 o = *reinterpret_cast<const float4*>(part(c + v) + 4 * lane);
+        const float ev = __shfl_sync(0xffffffffu, e, v);
+        O.x = fmaf(o.x, ev, O.x), O.y = fmaf(o.y, ev, O.y), O.z = fmaf(o.z, ev, O.z), O.w = fmaf(o.w, ev, O.w);
+      }
+    }
+    L = warp_sum(L);
+    const float f = L == 0.0f ? 0.0f : 1.0f / L;
+    T y[4];
+    from_f32(O.x * f, &y[0]), from_f32(O.y * f, &y[1]), from_f32(O.z * f, &y[2]), from_f32(O.w * f, &y[3]);
+    const int tt = row / a.G, hq = (bh % a.Hkv) * a.G + row - tt * a.G;
+    T* op = reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + 4 * lane;
+    *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
   }
-  const float f = L == 0.0f ? 0.0f : 1.0f / L;
-  T y[4];
-  from_f32(O.x * f, &y[0]), from_f32(O.y * f, &y[1]), from_f32(O.z * f, &y[2]), from_f32(O.w * f, &y[3]);
-  const int hq = (bh % a.Hkv) * a.G + row % a.G;
-  T* op = reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + row / a.G * a.ot + 4 * lane;
-  *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);
 }
 
 template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
@@ -564,16 +565,15 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
   if (r != FATHOM_OK) return r;
   prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
   if (ctas == 1 || (a.share && a.share == a.stride)) return check_launch("kv8_attend");   // no item is cut
-  const int rows = a.G * a.T < ROWS ? (int)(a.G * a.T) : ROWS;
-  return launch_join(prompt_join_kernel<T>, dim3(ctas - 1, (rows + JOIN_WARPS - 1) / JOIN_WARPS), JOIN_WARPS * 32, a, ctas, st);
+  return launch_join(prompt_join_kernel<T>, dim3(ctas - 1, JOIN_BLOCKS), JOIN_WARPS * 32, a, ctas, st);
 }
 
 }  // namespace
 
-size_t prompt_workspace() { return (size_t)sm_count() * 2 * ROWS * PART * sizeof(float); }
+size_t prompt_workspace() { return (size_t)sm_count() * (2 * ROWS * PART * sizeof(float) + sizeof(int4)); }
 
 int prompt_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st) {
-  const int ctas = plan_shares(a, sm_count(), PIECE);
+  const int ctas = a.ctas = plan_shares(a, sm_count(), PIECE, WHOLE, LEAST);
   return dtype == FATHOM_DTYPE_BF16 ? launch<__nv_bfloat16, 2>(map, a, ctas, st) : launch<__half, 3>(map, a, ctas, st);
 }
 

@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
   const int tid = threadIdx.x, lane = tid & 31, warp = (int)tc::uniform(tid >> 5);
   volatile int* gave_up = &s_gave_up;
 
-  int count;
-  const Place place = my_share(a, &count);
+  int count, share;
+  const Place place = my_share(a, &count, &share);
   Walk w(a, place, count);
   if (warp == 8) {
     // ---- loads: the share's tiles in order, as stages come free.  They begin while the CTA still sets itself up.
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
     if (tid == 0) s_before = before, s_total = total;
   }
   __syncthreads();
-  const int64_t share = a.share ? a.share : quotient(s_total + ctas - 1, ctas);
+  const int64_t share = a.share ? a.share : share_of(a, s_total, ctas);
   const int64_t first = a.share ? (int64_t)bh * a.stride : s_before + (int64_t)h * nt;
   const int c0 = (int)quotient(first, (int)share), n = (int)quotient(first + nt - 1, (int)share) - c0 + 1;
   tc::wait_dependency();                          // the parts are written; and nothing ends before they are
@@ -577,14 +577,7 @@ int token_attend(const CUtensorMap& map, Args a, int dtype, cudaStream_t st) {
   // one CTA per SM, but no more than there can be tiles
   const int64_t per = cdiv(a.end_dev ? a.cap : a.end, TILE), items = (int64_t)a.B * a.Hkv, tiles = items * (per > 1 ? per : 1);
   const int64_t sms = sm_count() < MAX_CTAS ? sm_count() : MAX_CTAS;
-  int ctas = (int)(tiles < sms ? tiles : sms);
-  if (!a.end_dev && per <= SHORT) {
-    // each row whole in one CTA
-    a.share = a.stride = (int)(per > 1 ? per : 1);
-    ctas = (int)items;
-  } else {
-    ctas = plan_shares(a, ctas, PIECE);
-  }
+  const int ctas = plan_shares(a, (int)(tiles < sms ? tiles : sms), PIECE, SHORT, 1);
   return dtype == FATHOM_DTYPE_BF16 ? launch_rows<__nv_bfloat16, 2>(map, a, ctas, st)
                                     : launch_rows<__half, 3>(map, a, ctas, st);
 }
