@@ -29,6 +29,7 @@ struct Args {
   // Set by plan_shares (kv8_line.cuh) where the lengths are known to the host: tiles per CTA, and the distance of two
   // items in the line.  share = 0: the device cuts the line, into shares of at least `least` tiles.
   int share, stride, least;
+  int64_t tiles_bh;               // tiles of one row bh, where the host knows them; else 0
   int ctas;                       // of the prompt kernel
 };
 

@@ -74,7 +74,7 @@ __device__ inline int64_t line(const Args& a, int64_t at, Place* place) {
   int it = 0, b = 0;
   int64_t before = 0, total = 0, one = 0;
   if (!a.end_dev) {
-    one = bh_line(a, seq_end(a, 0), -1, &it, &before);
+    one = a.tiles_bh;
     total = one * a.Hkv * a.B;
     if (at < 0 || at >= total) return total;
     b = (int)(at / (one * a.Hkv));
@@ -95,7 +95,7 @@ __device__ inline int64_t line(const Args& a, int64_t at, Place* place) {
     if (!found) return total;
   }
   const int end = seq_end(a, b);
-  one = bh_line(a, end, -1, &it, &before);
+  if (a.end_dev) one = bh_line(a, end, -1, &it, &before);
   const int h = (int)(at / one);
   at -= h * one;
   bh_line(a, end, at, &it, &before);
@@ -189,7 +189,13 @@ struct Walk {
 inline int plan_shares(Args& a, int most, int piece, int whole, int least) {
   a.least = least;
   if (a.end_dev) return most;
-  const int64_t per = (a.G * a.T - 1) / ROWS + 1, items = (int64_t)a.B * a.Hkv * per, nt = a.end > TILE ? cdiv(a.end, TILE) : 1;
+  const int64_t per = (a.G * a.T - 1) / ROWS + 1;
+  for (int64_t it = 0; it < per; ++it) {
+    const int64_t rows = a.G * a.T, last = ((it + 1) * ROWS < rows ? (it + 1) * ROWS : rows) - 1;
+    const int64_t see = a.end - (a.T - 1) + last / a.G;            // as tiles_of
+    a.tiles_bh += see > TILE ? cdiv(see, TILE) : 1;
+  }
+  const int64_t items = (int64_t)a.B * a.Hkv * per, nt = a.end > TILE ? cdiv(a.end, TILE) : 1;   // of the longest
   if (nt <= whole) {
     a.share = a.stride = (int)nt;
     return (int)items;

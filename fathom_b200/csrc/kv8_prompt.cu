@@ -144,44 +144,55 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
-      // the half's queries as e4m3 terms of their own scales: a warp takes every eighth row, 4 rows at a time, a lane 4 dims
-      const int first = w.it * ROWS + h2 * HALF, rows = min(HALF, total - first);
+      // the half's queries as e4m3 terms of their own scales: 16 lanes per row, a lane 8 dims; a warp takes rows 2 (warp mod 8)
+      // and the next of every 16, 8 at a time.  What a term leaves of 11 bits is exact in f16.
+      const int first = w.it * ROWS + h2 * HALF, rows = min(HALF, total - first), piece = lane & 15;
+      const T* const qb = reinterpret_cast<const T*>(a.q) + w.b * a.qb + (int64_t)(w.bh % a.Hkv) * a.G * a.qh + 8 * piece;
+      const int tk0 = first / a.G, head0 = first - tk0 * a.G;
+      const float per_head = 1.0f / (float)a.G;
 #pragma unroll 1                                   // run once a piece: small code over fast code
-      for (int r0 = warp & 7; r0 < rows; r0 += 32) {
-        uint2 v[4];
+      for (int r0 = 2 * (warp & 7) + (lane >> 4); r0 - (lane >> 4) < rows; r0 += 64) {
+        uint4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int rw = first + min(r0 + 8 * i, rows - 1), tk = rw / a.G;
-          v[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(a.q) + w.b * a.qb +
-                                                 (int64_t)((w.bh % a.Hkv) * a.G + rw - tk * a.G) * a.qh + tk * a.qt + 4 * lane);
+          const int x = head0 + min(r0 + 16 * i, rows - 1), tk = (int)(((float)x + 0.5f) * per_head);   // x / G, x < 128 + G
+          v[i] = *reinterpret_cast<const uint4*>(qb + (int64_t)(x - tk * a.G) * a.qh + (tk0 + tk) * a.qt);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int rl = r0 + 8 * i;
-          if (rl >= rows) break;
+          const int rl = r0 + 16 * i;
           const T* e = reinterpret_cast<const T*>(&v[i]);
-          float2 x[2] = {make_float2(to_f32(e[0]), to_f32(e[1])), make_float2(to_f32(e[2]), to_f32(e[3]))};
-          uint32_t top = __float_as_uint(fmaxf(fmaxf(fabsf(x[0].x), fabsf(x[0].y)), fmaxf(fabsf(x[1].x), fabsf(x[1].y))));
-          top = __reduce_max_sync(0xffffffffu, top);
-          const int e2 = kv8_exponent(top);
-          const float inv = top < 0x7F800000u ? pow2i(-e2) : __uint_as_float(0x7FFFFFFFu);   // a row with an infinity is NaN
-          if (lane == 0) s_rs[h2][rl] = pow2i(e2) * QSCALE;
+          float2 x[4];
+          float most = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) x[k] = make_float2(x[k].x * inv, x[k].y * inv);
+          for (int k = 0; k < 4; ++k) {
+            x[k] = make_float2(to_f32(e[2 * k]), to_f32(e[2 * k + 1]));
+            most = max3(most, fabsf(x[k].x), fabsf(x[k].y));
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const int e2 = kv8_exponent(__float_as_uint(most));
+          const float inv = most < INFINITY ? pow2i(-e2) : __uint_as_float(0x7FFFFFFFu);   // a row with an infinity is NaN
+          if (rl >= rows) continue;
+          if (piece == 0) s_rs[h2][rl] = pow2i(e2) * QSCALE;
+          __half2 y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = __floats2half2_rn(x[k].x * inv, x[k].y * inv);
+          uint8_t* const at = smem + S::Q + h2 * QT * HALF * D + rl * D + (((piece >> 1) ^ (rl & 7)) << 4) + (piece & 1) * 8;
 #pragma unroll
           for (int term = 0; term < QT; ++term) {
-            uint32_t code[2];
+            uint32_t code[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              code[k] = __nv_cvt_float2_to_fp8x2(x[k], __NV_SATFINITE, __NV_E4M3);
-              const float2 d = kv8_decode2(code[k]);
-              x[k] = make_float2(x[k].x - d.x, x[k].y - d.y);
+            for (int k = 0; k < 4; ++k) {
+              code[k] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y[k]), __NV_SATFINITE, __NV_E4M3);
+              const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code[k], __NV_E4M3);
+              y[k] = __hsub2(y[k], *reinterpret_cast<const __half2*>(&d));
             }
-            *reinterpret_cast<uint32_t*>(smem + S::Q + (h2 * QT + term) * HALF * D + rl * D +
-                                         (((lane >> 2) ^ (rl & 7)) << 4) + (lane & 3) * 4) = code[0] | code[1] << 16;
+            *reinterpret_cast<uint2*>(at + term * HALF * D) = make_uint2(code[0] | code[1] << 16, code[2] | code[3] << 16);
           }
         }
       }
+      __syncwarp();
       tc::fence_async_smem();
       tc::fence_before();
       __syncwarp();
