@@ -97,11 +97,15 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
                      cap <= KV8_MAX_CAP, FATHOM_ERR_SHAPE, "kv8_attend: bad shape");
   FATHOM_REQUIRE(end_dev || (end >= 0 && end <= cap), FATHOM_ERR_SHAPE, "kv8_attend: end %lld is outside the cache's %lld",
                  (long long)end, (long long)cap);
+  FATHOM_REQUIRE((reinterpret_cast<uintptr_t>(scales) & 7) == 0, FATHOM_ERR_SHAPE,
+                 "kv8_attend: the scales must be 8-byte aligned");
   FATHOM_REQUIRE(aligned16(rows) && aligned16(q) && aligned16(out) && (q_stride_b | q_stride_h | q_stride_t) % 8 == 0 &&
                      (o_stride_b | o_stride_h | o_stride_t) % 8 == 0, FATHOM_ERR_SHAPE,
                  "kv8_attend: rows, q and out (with their strides) must be 16-byte aligned");
-  FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_workspace_bytes(B, Hkv, G, T), FATHOM_ERR_WORKSPACE,
-                 "kv8_attend: workspace too small");
+  FATHOM_REQUIRE(workspace_bytes >= fathom_kv8_attend_workspace_bytes(B, Hkv, G, T) &&
+                     (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, FATHOM_ERR_WORKSPACE,
+                 "kv8_attend: workspace needs %zu bytes, 16-byte aligned",
+                 fathom_kv8_attend_workspace_bytes(B, Hkv, G, T));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   unsigned long long* timeouts = timeout_counter();
   if (!timeouts) return set_error(FATHOM_ERR_CUDA, "kv8_attend: no address of the wait counter");

@@ -114,8 +114,8 @@ __device__ __forceinline__ int64_t share_of(const Args& a, int64_t total, int ct
   return share >= a.least ? share : max(share, min((int64_t)a.least, quotient(total, a.B * a.Hkv * items_per_bh(a))));
 }
 
-// One warp: where this CTA's share begins, how many tiles it has (0 or less: none) and how many a CTA has at most.  A token's latency counts on
-// this: the common forms, a plan or up to 32 sequences of one item per bh, take one pass.
+// One warp: where this CTA's share begins, how many tiles it has (0 or less: none) and how many a CTA has at most.  A
+// token's latency counts on this: the common forms, a plan or up to 32 sequences of one item per bh, take one pass.
 __device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
   const int lane = threadIdx.x & 31;
   Place p{0, 0};
@@ -162,7 +162,8 @@ struct Walk {
   int per, item, tile, left;
   int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
   __device__ Walk(const Args& a_, const Place& p, int count)
-      : a(a_), per(items_per_bh(a_)), item(tc::uniform(p.item)), tile(tc::uniform(p.tile)), left(tc::uniform(max(count, 0))) {}
+      : a(a_), per(items_per_bh(a_)), item(tc::uniform(p.item)), tile(tc::uniform(p.tile)),
+        left(tc::uniform(max(count, 0))) {}
   // accumulators of 128 rows that the item needs
   __device__ int halves() const { return rows_of(a) - it * ROWS > ROWS / 2 ? 2 : 1; }
   __device__ bool next() {

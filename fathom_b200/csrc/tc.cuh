@@ -70,8 +70,12 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 __device__ __forceinline__ void wait_dependency() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
 // Barrier `id` among `n` threads: waiting, not waiting, and waiting with an OR of a predicate.
-__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ void named_arrive(int id, int n) { asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ void named_sync(int id, int n) {
+  asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(n) : "memory");
+}
+__device__ __forceinline__ void named_arrive(int id, int n) {
+  asm volatile("bar.arrive %0, %1;\n" ::"r"(id), "r"(n) : "memory");
+}
 __device__ __forceinline__ bool named_or(int id, int n, bool v) {
   uint32_t r;
   asm volatile("{ .reg .pred p, q; setp.ne.u32 p, %1, 0; bar.red.or.pred q, %2, %3, p; selp.u32 %0, 1, 0, q; }\n"

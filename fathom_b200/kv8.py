@@ -143,7 +143,8 @@ class KVCache8:
         """softmax(q K^T / sqrt(128)) V of q [B, Hq, T, 128] (bf16 or fp16, any strides; Hq a multiple of Hkv):
         the T queries of a sequence are its last T tokens, already written, and query t sees the keys
         [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
-        that sees no key gives 0.  Returns [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
+        that sees no key gives 0; a NaN in a key or value reaches the queries that see it and no others.  Returns
+        [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
         self._check_on("KVCache8.attend", q)
         if self.host:
             raise ValueError("KVCache8.attend: the rows are in host memory (attend_picks reads those)")

@@ -124,8 +124,8 @@ int fathom_scan(const float* q, int64_t BH, int G, int64_t n, int64_t sub, const
                 float* scores, void* stream);
 
 /* Diagnostic, no reference counterpart: the number of bounded device waits that gave up on the
- * current device since the last reset (the scan's bulk-copy mbarrier waits, 2 s each).  A wait
- * that gives up makes its tile's scores NaN; 0 in normal operation.  Synchronises the device.
+ * current device since the last reset (the scan's bulk-copy mbarrier waits and those of fathom_kv8_attend,
+ * 2 s each).  A wait that gives up makes its tile's scores, or its share's outputs, NaN; 0 in normal operation.  Synchronises the device.
  *   count may be NULL; reset != 0 zeroes the counter after reading it. */
 int fathom_wait_timeouts(unsigned long long* count, int reset);
 
@@ -337,7 +337,9 @@ size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t 
 
 /* out = softmax(q K^T / sqrt(128)) V over the cache, for q, out [B][Hkv*G][T][128] (bf16 or fp16; strides in
  * elements, last dimension contiguous): the T queries of a sequence are its last T tokens, query t sees
- * the keys [0, end - (T - 1 - t)).  A query that sees no key gives 0.  end above cap is read as cap. */
+ * the keys [0, end - (T - 1 - t)).  A query that sees no key gives 0.  end above cap is read as cap.  Scores and
+ * sums in fp32; queries enter the products to 2^-18 of a row's largest element (bf16) or to 12 bits (fp16); weights are kept to 11 bits or more.  A NaN or infinity of a query, a key or a value makes the queries that
+ * see it NaN (of a value: in its dim at least) and no others. */
 int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,
                       int64_t q_stride_h, int64_t q_stride_t, const uint8_t* rows, const float* scales, int64_t cap,
                       int64_t end, const int64_t* end_dev, void* out, int64_t o_stride_b, int64_t o_stride_h,

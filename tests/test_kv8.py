@@ -50,22 +50,24 @@ def test_c_entries_refuse_bad_arguments():
     assert read(dtype=9) == _lib.FATHOM_ERR_UNSUPPORTED
     assert read(n=129) == read(start=121) == read(start=-1) == read(cap=65) == read(K=odd) == _lib.FATHOM_ERR_SHAPE
 
-    def attend(q=p, dtype=1, B=1, H=1, G=4, T=1, cap=128, end=100, dev=None, ws=p, nb=1 << 40, strides=(512, 128, 128)):
-        return L.fathom_kv8_attend(q, dtype, B, H, G, T, *strides, p, p, cap, end, dev, p, 512, 128, 128, ws, nb, None)
+    def attend(q=p, dtype=1, B=1, H=1, G=4, T=1, cap=128, end=100, dev=None, ws=p, nb=1 << 40, strides=(512, 128, 128), sc=p):
+        return L.fathom_kv8_attend(q, dtype, B, H, G, T, *strides, p, sc, cap, end, dev, p, 512, 128, 128, ws, nb, None)
 
     assert attend(q=None) == attend(ws=None) == _lib.FATHOM_ERR_NULL
     assert attend(dtype=0) == _lib.FATHOM_ERR_UNSUPPORTED
     assert attend(end=129) == attend(end=-1) == attend(G=0) == attend(T=0) == attend(cap=70) == _lib.FATHOM_ERR_SHAPE
     assert attend(q=odd) == attend(strides=(512, 130, 128)) == _lib.FATHOM_ERR_SHAPE
-    assert attend(nb=0) == _lib.FATHOM_ERR_WORKSPACE
+    assert attend(sc=ctypes.c_void_p(260)) == attend(cap=2 ** 31) == _lib.FATHOM_ERR_SHAPE
+    assert attend(nb=0) == attend(ws=odd) == _lib.FATHOM_ERR_WORKSPACE
     assert b"workspace" in L.fathom_last_error()
 
-    def picks(q=p, dtype=1, B=1, H=1, G=4, idx=p, k=10, cap=128, end=100, nb=1 << 40, host=0):
-        return L.fathom_kv8_attend_picks(q, dtype, B, H, G, idx, k, p, host, p, cap, end, None, p, p, nb, None)
+    def picks(q=p, dtype=1, B=1, H=1, G=4, idx=p, k=10, cap=128, end=100, nb=1 << 40, host=0, sc=p):
+        return L.fathom_kv8_attend_picks(q, dtype, B, H, G, idx, k, p, host, sc, cap, end, None, p, p, nb, None)
 
     assert picks(q=None) == picks(idx=None) == _lib.FATHOM_ERR_NULL
     assert picks(dtype=5) == _lib.FATHOM_ERR_UNSUPPORTED
     assert picks(k=0) == picks(end=129) == picks(G=0) == picks(B=70000) == picks(q=odd) == _lib.FATHOM_ERR_SHAPE
+    assert picks(sc=ctypes.c_void_p(260)) == picks(k=2 ** 31) == _lib.FATHOM_ERR_SHAPE
     assert picks(nb=0) == picks(nb=1000, host=1) == _lib.FATHOM_ERR_WORKSPACE
     assert L.fathom_kv8_attend_picks_workspace_bytes(1, 8, 4, 580, 1) >= 8 * 4 * 580 * 256
     assert L.fathom_kv8_attend_picks_workspace_bytes(1, 8, 4, 580, 0) == 256
