@@ -54,6 +54,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float redux_max(float x) {      // over the warp; NaN if none is a number
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Lets `kernel` use `smem` bytes of dynamic shared memory on the current device; done: one bit per device that has been told.
 template <typename K> int allow_smem(K kernel, int smem, std::atomic<uint64_t>& done, const char* what) {
   int dev = 0;

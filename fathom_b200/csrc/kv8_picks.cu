@@ -1,23 +1,22 @@
 // Attention over listed rows of the 8-bit cache (layout in kv8.cuh), one list per query head.
 //
-// The floor is the rows' bytes, 256 at random addresses per pick, and for one sequence latency.  A warp takes 16 picks at
-// a time; their rows come into shared memory by 16-byte asynchronous copies while it works on the 16 before: 64 KB on
-// their way per SM.  With one query row per list a product has nothing to share, but
-// dequantising and multiplying on the fp32 pipes took ~290 instructions per 4 picks; as fragments of 16-bit matrix
-// instructions (an e4m3 is exact in f16) it is ~190 per 16:
+// The floor is the rows' bytes, 256 at random addresses per pick, and for one sequence latency.  A warp takes 32 picks at
+// a time; their rows come into shared memory by 16-byte asynchronous copies while it works on the 32 before.  With one query row per list a product has nothing to share, but the matrix instructions take e4m3 as
+// it lies in memory, so nothing is dequantised:
 //
-//   scores   [16 picks x 8] = K [16 x 128] q^T          columns: q as a sum of three f16 terms (33 bits)
-//   output^T [128 dims x 8] += V^T [128 x 16 picks] p   columns: the weights as two f16 terms (22 bits)
+//   scores   [32 picks x 8] = K [32 x 128] q^T          columns: q as a sum of six e4m3 terms, 16^-n apart (24 bits)
+//   output^T [128 dims x 8] += V^T [128 x 32 picks] p   columns: the weights as six such terms
 //
-// The order of dims within a score, and of picks within a sum, is free, so a lane's fragments are 16-byte pieces of rows as
-// they lie: K piece j and j + 4 of picks g and g + 8, V piece g of picks 2j, 2j + 1, 2j + 8, 2j + 9 (lane = 4 g + j).
-// Softmax state per warp, in fp32 as in kv8_token.cu: references of s + log2(value scale) for the output and of s for
-// the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their states are joined in warp
-// order in the first CTA's shared memory.
+// (m16n8k32 keeps 24 bits of a sum; measured with single large and small products.)  The order of dims within a score,
+// and of picks within a sum, is free, so a lane's fragments are 16-byte pieces of rows as they lie: lane 4 g + j has key
+// pieces j and j + 4 of picks g, g + 8, g + 16, g + 24, and value piece g of picks 4 j .. 4 j + 3 and 16 + 4 j .., whose
+// bytes it transposes 4 x 4.  Softmax, lane = pick, in fp32 as in kv8_token.cu: references of s + log2(value scale)
+// for the output and of s for the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their
+// states are joined in warp order in the first CTA's shared memory.
 //
-// Measured over 128k: 2116 picks for each of 224 heads 34 us, 3.6 TB/s of rows (58 us on the fp32 pipes); with the rows
-// in L2 it takes 29: the warps' own steps are the bound, and 16 warps per SM with 2 stages are better than 12 with 3.
-// 580 picks for 32 heads: 8.0 us with its launch.
+// Measured over 128k: 2116 picks for each of 224 heads 32.5 us, 3.7 TB/s of rows (34 with 16-bit matrix instructions on
+// rows turned to f16, 58 on the fp32 pipes); with the rows in L2 25.6.  580 picks for 32 heads: 5.6 us with its launch (8.0
+// with 16 picks per step).  Issuing the copies is the bound: 1,800 of the 3,200 cycles that a warp takes per 32 picks.
 #include "dedupe.cuh"
 #include "kv8_attn.cuh"
 
@@ -31,12 +30,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int CHUNK = 16;                // picks per step of a warp
+constexpr int CHUNK = 32;                // picks per step of a warp
 constexpr int STAGES = 2;                // chunks in shared memory: being used, and on its way
-constexpr int WARPS_PER_SM = 16;         // 16 x 2 x 4.3 KB of shared memory, 16 x 32 threads of 128 registers
+constexpr int WARPS_PER_SM = 9;          // 9 x 23 KB of shared memory: all are resident at once
 constexpr int MAX_CS = 8, MAX_PW = 4;    // CTAs of a cluster, warps of a CTA
+constexpr int TERMS = 6;                 // e4m3 terms of q and of the weights, 4 bits each
 constexpr float SLACK = 6.0f;            // a chunk may exceed the reference by 2^6
-constexpr float HEAD = 8.0f;             // weights at the reference are 2^8: f16 from 2^-24 to 2^15
+constexpr float HEAD = 2.0f;             // weights at the reference are 4: 2^(HEAD + SLACK) = 256 <= 448
 
 struct PicksArgs {
   const int64_t* idx;        // [BH*G][k]
@@ -51,14 +51,18 @@ struct PicksArgs {
 };
 
 struct alignas(128) Stage {              // halves of rows 128-byte aligned: pieces are permuted by XOR on addresses
-  uint8_t row[CHUNK][KV8_ROW];           // 16-byte pieces permuted within each half (piece_of)
+  uint8_t row[CHUNK][KV8_ROW];           // 16-byte pieces permuted within each half
   float2 scale[CHUNK];
   int valid[CHUNK];
 };
+struct alignas(128) Warp {
+  Stage stage[STAGES];
+  uint32_t weight[8][CHUNK / 4];         // term n of the chunk's weights; rows TERMS .. stay 0
+};
 
 // Piece c (0..7) of a row's key or value half lies at c ^ permuted(row), so that the 8 lanes of a shared-memory phase meet
-// 8 different bank groups: keys are read as rows 2p, 2p + 1 x 4 pieces, values as 4 even or odd rows x 2 pieces.
-__device__ __forceinline__ int permuted(int row) { return ((row >> 1 & 3) ^ (row & 1) << 1) << 1; }
+// 8 different bank groups: keys are read as rows 2p, 2p + 1 x 4 pieces, values as rows i, i + 4, i + 8, i + 12 x 2.
+__device__ __forceinline__ int permuted(int row) { return ((row >> 2 & 3) ^ (row & 1) << 1) << 1; }
 
 // dst: shared-memory addresses; zeros where there is no row.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -71,48 +75,55 @@ __device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t half2_of(uint32_t codes) {       // two codes in the low 16 bits
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xFFFFu), __NV_E4M3);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Bytes b of four words side by side: x[b] = (w0.b, w1.b, w2.b, w3.b).
+__device__ __forceinline__ void transpose4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&x)[4]) {
+  const uint32_t t0 = __byte_perm(w0, w1, 0x5140), t1 = __byte_perm(w0, w1, 0x7362);
+  const uint32_t t2 = __byte_perm(w2, w3, 0x5140), t3 = __byte_perm(w2, w3, 0x7362);
+  x[0] = __byte_perm(t0, t2, 0x5410), x[1] = __byte_perm(t0, t2, 0x7632);
+  x[2] = __byte_perm(t1, t3, 0x5410), x[3] = __byte_perm(t1, t3, 0x7632);
 }
-__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+// Two values to two codes; what they leave, times 16.
+__device__ __forceinline__ uint32_t next_term(float2& y) {
+  const uint32_t code = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+  const float2 d = kv8_decode2(code);
+  y = make_float2(fmaf(d.x, -16.0f, 16.0f * y.x), fmaf(d.y, -16.0f, 16.0f * y.y));
+  return code;
+}
 
-// 16 consecutive elements of q, 16-byte aligned.
-__device__ __forceinline__ void load16(const void* p, int dtype, int64_t i, float* x) {
+// 4 consecutive elements of q.
+__device__ __forceinline__ void load4(const void* p, int dtype, int64_t i, float (&x)[4]) {
   if (dtype == FATHOM_DTYPE_F32) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      *reinterpret_cast<float4*>(x + 4 * e) = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i)[e];
+    const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     return;
   }
+  const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
+  const uint32_t w[2] = {v.x, v.y};
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint4 v = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i)[e];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float2 f = dtype == FATHOM_DTYPE_BF16
-                           ? make_float2(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u))
-                           : __half22float2(*reinterpret_cast<const __half2*>(&w[u]));
-      x[8 * e + 2 * u] = f.x, x[8 * e + 2 * u + 1] = f.y;
-    }
+  for (int u = 0; u < 2; ++u) {
+    const float2 f = dtype == FATHOM_DTYPE_BF16
+                         ? make_float2(__uint_as_float(w[u] << 16), __uint_as_float(w[u] & 0xFFFF0000u))
+                         : __half22float2(*reinterpret_cast<const __half2*>(&w[u]));
+    x[2 * u] = f.x, x[2 * u + 1] = f.y;
   }
 }
 
 __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
-    picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a,
-                                                                   void* __restrict__ out) {
+    picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a, void* __restrict__ out) {
   const int PW = blockDim.x >> 5, NW = PW * (int)gridDim.y;      // one cluster of gridDim.y CTAs per (batch, query head)
   extern __shared__ __align__(128) uint8_t smem_raw[];
   constexpr int MAX_NW = MAX_PW * MAX_CS;
   __shared__ float s_m[MAX_NW], s_lm[MAX_NW], s_l[MAX_NW];       // the cluster's first CTA: every warp's state
-  float(*const s_acc)[D] = reinterpret_cast<float(*)[D]>(smem_raw + PW * STAGES * sizeof(Stage));
+  __shared__ __align__(16) uint32_t s_q[8][D / 4];               // term n of q; rows TERMS .. are 0
+  __shared__ float s_rs;
+  float(*const s_acc)[D] = reinterpret_cast<float(*)[D]>(smem_raw + PW * sizeof(Warp));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, j = lane & 3;
-  Stage* const st = reinterpret_cast<Stage*>(smem_raw) + warp * STAGES;
+  Warp& mine = reinterpret_cast<Warp*>(smem_raw)[warp];
+  Stage* const st = mine.stage;
   const unsigned crank = blockIdx.y;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();                            // waited for before the first store into another CTA
@@ -124,8 +135,8 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   const int k = (int)a.k, chunks = (k + CHUNK - 1) / CHUNK;
   const int n = chunks > gw ? (chunks - gw + NW - 1) / NW : 0;   // this warp's chunks: gw, gw + NW, ..
 
-  // lanes 0..15: the next chunk's picks and the rows that hold them (-1: none)
-  int next = lane < CHUNK ? gw * CHUNK + lane : k;
+  // lane: the next chunk's pick and the row that holds it (-1: none)
+  int next = gw * CHUNK + lane;
   auto pick = [&](int& tok, int& row) {
     tok = row = -1;
     if (next < k) {
@@ -140,14 +151,12 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   const uint8_t* const from = a.rows + (int64_t)bh * a.row_cap * KV8_ROW + (lane & 15) * 16;
   auto bring = [&](int s, int tok, int row) {
     const uint32_t at = ring + s * (uint32_t)sizeof(Stage);
-    if (lane < CHUNK) {
-      st[s].valid[lane] = row;
-      if (row >= 0) copy8(at + (uint32_t)offsetof(Stage, scale) + lane * 8, sc + tok / BLK);
-    }
+    st[s].valid[lane] = row;
+    if (row >= 0) copy8(at + (uint32_t)offsetof(Stage, scale) + lane * 8, sc + tok / BLK);
 #pragma unroll
     for (int u = 0; u < CHUNK / 2; ++u) {
       const int r = __shfl_sync(0xffffffffu, row, 2 * u + (lane >> 4));
-      copy16((at + lane_at + u * 2 * KV8_ROW) ^ ((u & 3) << 5), from + (int64_t)max(r, 0) * KV8_ROW, r >= 0);
+      copy16((at + lane_at + u * 2 * KV8_ROW) ^ ((u >> 1 & 3) << 5), from + (int64_t)max(r, 0) * KV8_ROW, r >= 0);
     }
   };
   auto commit = []() { asm volatile("cp.async.commit_group;\n" ::: "memory"); };
@@ -159,46 +168,48 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
     commit();
   }
   pick(tok, row);
+  if (lane < 2 * 8) mine.weight[TERMS + lane / 8][lane % 8] = 0;
 
-  // q: this lane's dims, 16 j .. and 64 + 16 j .., of term g (0, 1, 2; zeros for the others)
-  uint32_t qf[16];
-  float rs;
-  {
-    float x[32];
-    load16(q, dtype, bhg * D + 16 * j, x);
-    load16(q, dtype, bhg * D + 64 + 16 * j, x + 16);
+  // q as terms: one warp, a lane 4 dims; then term g of this lane's dims, 16 j .. and 64 + 16 j ..
+  if (warp == 0) {
+    float x[4];
+    load4(q, dtype, bhg * D + 4 * lane, x);
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
     top = __reduce_max_sync(0xffffffffu, top);
     const int e = kv8_exponent(top);
     const float inv = top < 0x7F800000u ? pow2i(-e) : __uint_as_float(0x7FFFFFFFu);   // a row with inf or NaN is NaN
-    rs = pow2i(e) * QSCALE;
+    float2 y0 = make_float2(x[0] * inv, x[1] * inv), y1 = make_float2(x[2] * inv, x[3] * inv);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float2 y = make_float2(x[2 * i] * inv, x[2 * i + 1] * inv);
-      __half2 h[3];
-#pragma unroll
-      for (int t = 0; t < 3; ++t) {
-        h[t] = __floats2half2_rn(y.x, y.y);
-        const float2 f = __half22float2(h[t]);
-        y = make_float2(y.x - f.x, y.y - f.y);         // what the terms so far leave
+    for (int t = 0; t < 8; ++t) {
+      uint32_t code = 0;
+      if (t < TERMS) {
+        code = next_term(y0);
+        code |= next_term(y1) << 16;
       }
-      qf[i] = g == 0 ? bits(h[0]) : g == 1 ? bits(h[1]) : g == 2 ? bits(h[2]) : 0u;
+      s_q[t][lane] = code;
     }
+    if (lane == 0) s_rs = pow2i(e) * QSCALE;
   }
+  __syncthreads();
+  const float rs = s_rs;
+  uint32_t qf[8];
+  *reinterpret_cast<uint4*>(qf) = *reinterpret_cast<const uint4*>(&s_q[g][4 * j]);
+  *reinterpret_cast<uint4*>(qf + 4) = *reinterpret_cast<const uint4*>(&s_q[g][16 + 4 * j]);
+  const float f0 = exp2f((float)(-8 * j)), f1 = f0 * 0.0625f;          // columns 2 j and 2 j + 1 are terms: 16^-(2 j), ..
 
-  // this lane's pieces within a stage: of keys g and g + 8 (permuted alike), of values 2 j + (e & 1) + 4 (e & 2)
-  const int key_at = g * KV8_ROW + (j ^ permuted(g)) * 16;
-  int value_at[2];
+  // this lane's pieces within a stage, of keys g (+ 8, 16, 24: the piece permuted alike for + 16) and of values 4 j + e
+  const int key_at = g * KV8_ROW + (j ^ permuted(g)) * 16, key8_at = (g + 8) * KV8_ROW + (j ^ permuted(g + 8)) * 16;
+  int value_at[4];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) value_at[e] = (2 * j + e) * KV8_ROW + D + (g ^ permuted(2 * j + e)) * 16;
-  float acc[8][4];                                     // dims 16 g + 2 t and + 1; columns 2 j, 2 j + 1
+  for (int e = 0; e < 4; ++e) value_at[e] = (4 * j + e) * KV8_ROW + D + (g ^ permuted(4 * j + e)) * 16;
+  float acc[8][4];                                     // dims 16 g + 2 t and + 1; terms 2 j, 2 j + 1
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.0f;
-  float m = -INFINITY, lm = -1e30f, l = 0.0f;          // m is the warp's; l is of picks g and g + 8 of its chunks
+  float m = -INFINITY, lm = -1e30f, l = 0.0f;          // m is the warp's; lm, l: of this lane's picks
   int here = 0;                                        // stage of chunk i
   for (int i = 0; i < n; ++i) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
@@ -209,44 +220,36 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
     const Stage& s = st[here];
     const uint8_t* const bytes = &s.row[0][0];
     here = here + 1 == STAGES ? 0 : here + 1;
-    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, c2[4] = {0.0f, 0.0f, 0.0f, 0.0f};      // two chains of products
-    const uint4 k0 = *reinterpret_cast<const uint4*>(bytes + key_at),
-                k1 = *reinterpret_cast<const uint4*>(bytes + (key_at ^ 64));
-    const uint4 k8 = *reinterpret_cast<const uint4*>(bytes + 8 * KV8_ROW + key_at),
-                k9 = *reinterpret_cast<const uint4*>(bytes + 8 * KV8_ROW + (key_at ^ 64));
-    uint32_t x[4][4];
+    float c[2][4];                                     // picks g, g + 8; g + 16, g + 24
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint4 y = *reinterpret_cast<const uint4*>(bytes + (e >> 1) * 8 * KV8_ROW + value_at[e & 1]);
-      x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* const at = bytes + h * 16 * KV8_ROW;
+      uint32_t lo[8], hi[8];
+      *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(at + key_at);
+      *reinterpret_cast<uint4*>(lo + 4) = *reinterpret_cast<const uint4*>(at + (key_at ^ 64));
+      *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(at + key8_at);
+      *reinterpret_cast<uint4*>(hi + 4) = *reinterpret_cast<const uint4*>(at + (key8_at ^ 64));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[h][e] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; w += 2) mma(c[h], lo[w], hi[w], lo[w + 1], hi[w + 1], qf[w], qf[w + 1]);
     }
+    // scores: the sums over a quad's columns, of pick g + 8 j in lane (g, j)
+    float v;
     {
-      const uint32_t lo[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
-      const uint32_t hi[8] = {k8.x, k8.y, k8.z, k8.w, k9.x, k9.y, k9.z, k9.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        mma(c, half2_of(lo[w]), half2_of(hi[w]), half2_of(lo[w] >> 16), half2_of(hi[w] >> 16), qf[2 * w], qf[2 * w + 1]);
-        mma(c2, half2_of(lo[w + 4]), half2_of(hi[w + 4]), half2_of(lo[w + 4] >> 16), half2_of(hi[w + 4] >> 16), qf[8 + 2 * w],
-            qf[9 + 2 * w]);
-      }
+      const float s0 = fmaf(c[0][1], f1, c[0][0] * f0), s1 = fmaf(c[0][3], f1, c[0][2] * f0);
+      const float s2 = fmaf(c[1][1], f1, c[1][0] * f0), s3 = fmaf(c[1][3], f1, c[1][2] * f0);
+      const bool odd = j & 1, high = j & 2;
+      const float x = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 1);
+      const float y = (odd ? s3 : s2) + __shfl_xor_sync(0xffffffffu, odd ? s2 : s3, 1);
+      v = (high ? y : x) + __shfl_xor_sync(0xffffffffu, high ? x : y, 2);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] += c2[e];
-    // scores of picks g and g + 8: the sum of their columns, 2 of them in each lane of a quad
-    float v[2] = {c[0] + c[1], c[2] + c[3]}, lv[2], w[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 1);
-      v[e] += __shfl_xor_sync(0xffffffffu, v[e], 2);
-      const int r = g + 8 * e;
-      const bool there = s.valid[r] >= 0;
-      const float2 ks = there ? s.scale[r] : make_float2(0.0f, 1.0f);
-      v[e] = there ? v[e] * (ks.x * rs) : -INFINITY;
-      lv[e] = (float)((int)(__float_as_uint(ks.y) >> 23) - 127);
-    }
-    float top = fmaxf(v[0] + lv[0], v[1] + lv[1]);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int mypick = g + 8 * j;
+    const bool there = s.valid[mypick] >= 0;
+    const float2 ks = there ? s.scale[mypick] : make_float2(0.0f, 1.0f);
+    v = there ? v * (ks.x * rs) : -INFINITY;
+    const float lv = (float)((int)(__float_as_uint(ks.y) >> 23) - 127);
+    const float top = redux_max(v + lv);
     if (top > m + SLACK) {                             // the same in every lane; also the first time: m = -inf
       const float f = m == -INFINITY ? 0.0f : ex2(m - top);
       m = top;
@@ -255,50 +258,52 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t][e] *= f;
     }
+    // this pick's weight as terms, and its part of the denominator
+    {
+      float2 y = make_float2(m == -INFINITY && !(v != v) ? 0.0f : ex2(v + (lv - m + HEAD)), 0.0f);
+      uint8_t* const at = reinterpret_cast<uint8_t*>(mine.weight) + mypick;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      w[e] = m == -INFINITY && !(v[e] != v[e]) ? 0.0f : ex2(v[e] + (lv[e] - m + HEAD));
-      const float d = v[e] - lm, p = ex2(-fabsf(d));
+      for (int t = 0; t < TERMS; ++t) at[t * CHUNK] = (uint8_t)next_term(y);
+      const float d = v - lm, p = ex2(-fabsf(d));
       l = d > 0.0f ? fmaf(l, p, 1.0f) : l + p;
-      lm = fmaxf(lm, v[e]);
+      lm = fmaxf(lm, v);
     }
-    // weights of picks 2 j, 2 j + 1 and 2 j + 8, 2 j + 9 as term g
-    uint32_t b[2];
+    uint32_t x[8][4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float x = __shfl_sync(0xffffffffu, w[e], 8 * j), y = __shfl_sync(0xffffffffu, w[e], 8 * j + 4);
-      const __half2 hi = __floats2half2_rn(x, y);
-      const float2 f = __half22float2(hi);
-      b[e] = g == 0 ? bits(hi) : g == 1 ? bits(__floats2half2_rn(x - f.x, y - f.y)) : 0u;
-    }
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<uint4*>(x[e]) = *reinterpret_cast<const uint4*>(bytes + (e >> 2) * 16 * KV8_ROW + value_at[e & 3]);
+    __syncwarp();
+    const uint32_t b0 = mine.weight[g][j], b1 = mine.weight[g][4 + j];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {                    // bytes 4 u + 2 h and + 1 of two picks side by side
-        const uint32_t s01 = __byte_perm(x[0][u], x[1][u], h ? 0x7362 : 0x5140);
-        const uint32_t s89 = __byte_perm(x[2][u], x[3][u], h ? 0x7362 : 0x5140);
-        mma(acc[2 * u + h], half2_of(s01), half2_of(s01 >> 16), half2_of(s89), half2_of(s89 >> 16), b[0], b[1]);
-      }
+    for (int u = 0; u < 4; ++u) {                      // bytes 4 u .. of the lane's 16 dims
+      uint32_t lo[4], hi[4];
+      transpose4(x[0][u], x[1][u], x[2][u], x[3][u], lo);
+      transpose4(x[4][u], x[5][u], x[6][u], x[7][u], hi);
+      mma(acc[2 * u], lo[0], lo[1], hi[0], hi[1], b0, b1);
+      mma(acc[2 * u + 1], lo[2], lo[3], hi[2], hi[3], b0, b1);
     }
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
-  // the warp's state: picks are spread over g
-  float ref = lm;
+  // the warp's state: picks are spread over its lanes, the terms of an output over the columns of a quad
+  const float ref = redux_max(lm);
+  l = warp_sum(l * ex2(lm - ref));
 #pragma unroll
-  for (int o = 4; o < 32; o <<= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
-  l *= ex2(lm - ref);
+  for (int t = 0; t < 8; ++t) {
 #pragma unroll
-  for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    for (int e = 0; e < 4; e += 2) {
+      float o = fmaf(acc[t][e + 1], f1, acc[t][e] * f0);
+      o += __shfl_xor_sync(0xffffffffu, o, 1);
+      acc[t][e] = o + __shfl_xor_sync(0xffffffffu, o, 2);
+    }
+  }
   cluster.barrier_wait();
   float *dm = cluster.map_shared_rank(s_m, 0), *dlm = cluster.map_shared_rank(s_lm, 0);
   float *dl = cluster.map_shared_rank(s_l, 0), *da = cluster.map_shared_rank(&s_acc[0][0], 0);
   if (lane == 0) dm[gw] = m, dlm[gw] = ref, dl[gw] = l;
-  if (j == 0) {                                        // columns 0 and 1: the two terms' sums
+  if (j == 0) {
     float4* dst = reinterpret_cast<float4*>(da + gw * D + 16 * g);
 #pragma unroll
-    for (int t = 0; t < 8; t += 2)
-      dst[t / 2] = make_float4(acc[t][0] + acc[t][1], acc[t][2] + acc[t][3], acc[t + 1][0] + acc[t + 1][1],
-                               acc[t + 1][2] + acc[t + 1][3]);
+    for (int t = 0; t < 8; t += 2) dst[t / 2] = make_float4(acc[t][0], acc[t][2], acc[t + 1][0], acc[t + 1][2]);
   }
   cluster.sync();
   if (crank != 0) return;
@@ -306,13 +311,13 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   float M = lane < NW ? s_lm[lane] : -1e30f;
   M = warp_max(M);
   const float L = warp_sum(lane < NW ? s_l[lane] * ex2(s_lm[lane] - M) : 0.0f);
-  const float mine = lane < NW && s_m[lane] != -INFINITY ? exp2f(s_m[lane] - HEAD - M) : 0.0f;
+  const float factor = lane < NW && s_m[lane] != -INFINITY ? exp2f(s_m[lane] - HEAD - M) : 0.0f;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   for (int d = threadIdx.x; d < D; d += blockDim.x) {
     float O = 0.0f;
 #pragma unroll 8
     for (int v = 0; v < NW; ++v) {
-      const float f = __shfl_sync(0xffffffffu, mine, v);
+      const float f = __shfl_sync(0xffffffffu, factor, v);
       if (f != 0.0f) O = fmaf(s_acc[v][d], f, O);
     }
     const float o = O * inv;
@@ -324,8 +329,8 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
 }
 
 int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, int pw, int cs, void* out, cudaStream_t st) {
-  const int smem = pw * STAGES * (int)sizeof(Stage) + pw * cs * D * (int)sizeof(float);
-  constexpr int most = MAX_PW * STAGES * (int)sizeof(Stage) + MAX_PW * MAX_CS * D * (int)sizeof(float);
+  const int smem = pw * (int)sizeof(Warp) + pw * cs * D * (int)sizeof(float);
+  constexpr int most = MAX_PW * (int)sizeof(Warp) + MAX_PW * MAX_CS * D * (int)sizeof(float);
   static std::atomic<uint64_t> told{0};
   const int r = allow_smem(picks_kernel, most, told, "kv8_attend_picks");
   if (r != FATHOM_OK) return r;
@@ -437,12 +442,11 @@ extern "C" int fathom_kv8_attend_picks(const void* q, int dtype, int64_t B, int6
     if (r != FATHOM_OK) return r;
     a.slot = w.slot, a.rows = w.rows, a.row_cap = M;
   }
-  // as many warps per head as the GPU holds at once, 32 at most, and no more than there are chunks; in CTAs of 2 (in
-  // whose number a wave is filled best) or of 4
-  const int64_t heads = B * Hkv * G, chunks = cdiv(k, CHUNK);
-  int64_t warps = (int64_t)WARPS_PER_SM * sm_count() / heads;
-  if (warps > chunks) warps = chunks;
-  const int pw = warps > 2 * MAX_CS ? 4 : warps > 1 ? 2 : 1;
-  const int64_t cs = warps / pw < 1 ? 1 : warps / pw > MAX_CS ? MAX_CS : warps / pw;
-  return launch_picks(q, dtype, a, heads, pw, (int)cs, out, st);
+  // as many warps per head as the GPU holds at once, 32 at most, and no more than there are chunks
+  const int64_t heads = B * Hkv * G, chunks = cdiv(k, CHUNK), fit = (int64_t)WARPS_PER_SM * sm_count() / heads;
+  int64_t warps = fit < chunks ? fit : chunks;
+  warps = warps < 1 ? 1 : warps > MAX_PW * MAX_CS ? MAX_PW * MAX_CS : warps;
+  const int pw = warps > 2 * MAX_CS ? 4 : warps > MAX_CS ? 2 : 1;
+  const int64_t cs = cdiv(warps, pw) * pw <= fit ? cdiv(warps, pw) : warps / pw;
+  return launch_picks(q, dtype, a, heads, pw, (int)(cs < 1 ? 1 : cs), out, st);
 }

@@ -62,12 +62,6 @@ __device__ __forceinline__ uint64_t weight_operand(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(TILE * 16 >> 4) << 32 | 1ull << 46;
 }
 
-__device__ __forceinline__ float redux_max(float x) {      // over the warp; NaN if none is a number
-  float y;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;\n" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <typename T> __device__ __forceinline__ void unpack4(uint2 v, float (&x)[4]) {
   const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
