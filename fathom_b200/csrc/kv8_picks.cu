@@ -14,9 +14,11 @@
 // for the output and of s for the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their
 // states are joined in warp order in the first CTA's shared memory.
 //
-// Measured over 128k: 2116 picks for each of 224 heads 32.5 us, 3.7 TB/s of rows (34 with 16-bit matrix instructions on
-// rows turned to f16, 58 on the fp32 pipes); with the rows in L2 25.6.  580 picks for 32 heads: 5.6 us with its launch (8.0
-// with 16 picks per step).  Issuing the copies is the bound: 1,800 of the 3,200 cycles that a warp takes per 32 picks.
+// Measured over 128k: 2116 picks for each of 224 heads 26 us, 4.7 TB/s of rows (34 with 16-bit matrix instructions on
+// rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24:
+// the copies' way into shared memory is the bound, some 340 cycles per 32 picks and SM.  12 warps per SM, or 3 stages, are
+// slower (29 us), so are TMA gathers of 4 rows (28), bulk copies of one (34) and rows loaded into registers (29).  580
+// picks for 32 heads: 5.5 us with its launch.
 #include "dedupe.cuh"
 #include "kv8_attn.cuh"
 
@@ -32,7 +34,7 @@ namespace cg = cooperative_groups;
 
 constexpr int CHUNK = 32;                // picks per step of a warp
 constexpr int STAGES = 2;                // chunks in shared memory: being used, and on its way
-constexpr int WARPS_PER_SM = 9;          // 9 x 23 KB of shared memory: all are resident at once
+constexpr int WARPS_PER_SM = 8;          // what the SM holds with ~180 registers per thread
 constexpr int MAX_CS = 8, MAX_PW = 4;    // CTAs of a cluster, warps of a CTA
 constexpr int TERMS = 6;                 // e4m3 terms of q and of the weights, 4 bits each
 constexpr float SLACK = 6.0f;            // a chunk may exceed the reference by 2^6
@@ -137,13 +139,21 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
 
   // lane: the next chunk's pick and the row that holds it (-1: none)
   int next = gw * CHUNK + lane;
-  auto pick = [&](int& tok, int& row) {
-    tok = row = -1;
+  // listed() only loads; what it loads is looked at one step later, in pick(): a step never waits for the list.
+  int64_t listed_tok = -1;
+  int listed_row = -1;
+  auto listed = [&]() {
+    listed_tok = -1;
     if (next < k) {
-      const int64_t t = a.idx[bhg * k + next];
-      if (t >= 0 && t < end) tok = (int)t, row = a.slot ? a.slot[bhg * k + next] : tok;
+      listed_tok = a.idx[bhg * k + next];
+      if (a.slot) listed_row = a.slot[bhg * k + next];
       next += NW * CHUNK;
     }
+  };
+  auto pick = [&](int& tok, int& row) {
+    const bool there = listed_tok >= 0 && listed_tok < end;
+    tok = there ? (int)listed_tok : -1;
+    row = there && a.slot ? listed_row : tok;
   };
   // copies of a chunk into stage s: a lane has piece lane & 15 of rows 2 u + (lane >> 4)
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(st);
@@ -160,14 +170,15 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
     }
   };
   auto commit = []() { asm volatile("cp.async.commit_group;\n" ::: "memory"); };
-  int tok, row;
+  listed();
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
+    int tok, row;
     pick(tok, row);
+    listed();
     if (i < n) bring(i, tok, row);
     commit();
   }
-  pick(tok, row);
   if (lane < 2 * 8) mine.weight[TERMS + lane / 8][lane % 8] = 0;
 
   // q as terms: one warp, a lane 4 dims; then term g of this lane's dims, 16 j .. and 64 + 16 j ..
@@ -214,9 +225,11 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   for (int i = 0; i < n; ++i) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(STAGES - 2) : "memory");
     __syncwarp();                                      // chunk i is there; chunk i - 1 has been read
+    int tok, row;
+    pick(tok, row);
+    listed();
     if (i + STAGES - 1 < n) bring(here == 0 ? STAGES - 1 : here - 1, tok, row);
     commit();
-    pick(tok, row);
     const Stage& s = st[here];
     const uint8_t* const bytes = &s.row[0][0];
     here = here + 1 == STAGES ? 0 : here + 1;
