@@ -70,6 +70,7 @@ class KVCache8:
             raise ValueError(f"KVCache8: scales must be contiguous float32 [{self.BH}, {self.nblk}, 2] beside the rows")
         self.rows, self.scales, self.device = rows, scales, rows.device
         self._ws = {}              # workspace bytes of a call's shape
+        self._unused = torch.empty(256, dtype=torch.uint8, device=self.device)   # workspace of picks of rows in HBM
 
     def nbytes(self):
         return self.rows.numel() + self.scales.numel() * 4
@@ -104,21 +105,22 @@ class KVCache8:
         this and in earlier calls; a block written from its first token on starts afresh.  NaN and infinities
         are stored as NaN and do not enter the scale."""
         self._check_on("KVCache8.write", K, V)
-        if K.dim() != 4 or K.shape[0] != self.B or K.shape[1] != self.Hkv or K.shape[3] != D or V.shape != K.shape:
+        shape = K.shape
+        if len(shape) != 4 or shape[0] != self.B or shape[1] != self.Hkv or shape[3] != D or V.shape != shape:
             raise ValueError(f"KVCache8.write: K and V must be [{self.B}, {self.Hkv}, T, {D}] "
-                             f"(got {tuple(K.shape)}, {tuple(V.shape)})")
+                             f"(got {tuple(shape)}, {tuple(V.shape)})")
         if K.dtype not in _lib.DTYPE_CODE or V.dtype != K.dtype:
             raise TypeError(f"KVCache8.write: K and V must both be fp32, bf16 or fp16 (got {K.dtype}, {V.dtype})")
-        T = K.shape[2]
+        T = shape[2]
         num, dev = _position(start, self.B, self.device, "KVCache8.write: start")
         if dev is None and not 0 <= num <= self.cap - T:
             raise ValueError(f"KVCache8.write: tokens [{num}, {num + T}) are outside the cache's {self.cap}")
         if T == 0:
             return
-        K, V = _rows16(K), _rows16(V)
-        if K.stride() != V.stride():
+        (K, sb, sh, st), (V, *strides) = _rows16(K), _rows16(V)
+        if strides != [sb, sh, st]:
             K, V = K.contiguous(), V.contiguous()
-        sb, sh, st, _ = K.stride()
+            sb, sh, st, _ = K.stride()
         check(lib().fathom_kv8_write(K.data_ptr(), V.data_ptr(), _lib.DTYPE_CODE[K.dtype], self.B, self.Hkv, T, sb, sh,
                                      st, num, ptr(dev), self.cap, self.rows.data_ptr(), self.scales.data_ptr(),
                                      self._stream()), "KVCache8.write")
@@ -148,22 +150,22 @@ class KVCache8:
         self._check_on("KVCache8.attend", q)
         if self.host:
             raise ValueError("KVCache8.attend: the rows are in host memory (attend_picks reads those)")
-        if q.dim() != 4 or q.shape[0] != self.B or q.shape[1] < 1 or q.shape[1] % self.Hkv or q.shape[3] != D:
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != self.B or shape[1] < 1 or shape[1] % self.Hkv or shape[3] != D:
             raise ValueError(f"KVCache8.attend: q must be [{self.B}, a multiple of {self.Hkv}, T, {D}] "
-                             f"(got {tuple(q.shape)})")
+                             f"(got {tuple(shape)})")
         if q.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError(f"KVCache8.attend: q must be bf16 or fp16 (got {q.dtype})")
-        B, Hq, T, _ = q.shape
+        B, Hq, T, _ = shape
         num, dev = _position(end, B, self.device, "KVCache8.attend: end")
         if dev is None and not 0 <= num <= self.cap:
             raise ValueError(f"KVCache8.attend: end {num} is outside the cache's {self.cap}")
-        out = torch.empty_strided(q.shape, (T * Hq * D, D, Hq * D, 1), dtype=q.dtype, device=self.device)
+        out = torch.empty_strided(shape, (T * Hq * D, D, Hq * D, 1), dtype=q.dtype, device=self.device)
         if T == 0:
             return out
-        q = _rows16(q)
+        q, sb, sh, st = _rows16(q)
         G = Hq // self.Hkv
         ws, nws = self._workspace((G, T), lib().fathom_kv8_attend_workspace_bytes, G, T)
-        sb, sh, st, _ = q.stride()
         check(lib().fathom_kv8_attend(q.data_ptr(), _lib.DTYPE_CODE[q.dtype], B, self.Hkv, G, T, sb, sh, st,
                                       self.rows.data_ptr(), self.scales.data_ptr(), self.cap, num, ptr(dev),
                                       out.data_ptr(), T * Hq * D, D, Hq * D, ws.data_ptr(), nws, self._stream()),
@@ -177,25 +179,27 @@ class KVCache8:
         arithmetic; returns [BH, G, 128] in q's dtype.  Of rows in host memory each distinct one of a KV head is
         fetched once."""
         self._check_on("KVCache8.attend_picks", q, idx)
-        if q.dim() != 3 or q.shape[0] != self.BH or q.shape[1] < 1 or q.shape[2] != D:
-            raise ValueError(f"KVCache8.attend_picks: q must be [{self.BH}, G, {D}] (got {tuple(q.shape)})")
+        qs, ks = q.shape, idx.shape
+        if len(qs) != 3 or qs[0] != self.BH or qs[1] < 1 or qs[2] != D:
+            raise ValueError(f"KVCache8.attend_picks: q must be [{self.BH}, G, {D}] (got {tuple(qs)})")
         if q.dtype not in _lib.DTYPE_CODE:
             raise TypeError(f"KVCache8.attend_picks: q must be fp32, bf16 or fp16 (got {q.dtype})")
-        BH, G, _ = q.shape
-        if idx.dim() != 3 or tuple(idx.shape[:2]) != (BH, G) or idx.dtype != torch.int64:
-            raise ValueError(f"KVCache8.attend_picks: idx must be int64 [{BH}, {G}, k] (got {idx.dtype} "
-                             f"{tuple(idx.shape)})")
+        BH, G, _ = qs
+        if len(ks) != 3 or ks[0] != BH or ks[1] != G or idx.dtype != torch.int64:
+            raise ValueError(f"KVCache8.attend_picks: idx must be int64 [{BH}, {G}, k] (got {idx.dtype} {tuple(ks)})")
         num, dev = _position(self.cap if end is None else end, self.B, self.device, "KVCache8.attend_picks: end")
         if dev is None and not 0 <= num <= self.cap:
             raise ValueError(f"KVCache8.attend_picks: end {num} is outside the cache's {self.cap}")
-        k = idx.shape[2]
+        k = ks[2]
         if k == 0:
             return torch.zeros(BH, G, D, dtype=q.dtype, device=self.device)
         q, idx = q.contiguous(), idx.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-        out = torch.empty(BH, G, D, dtype=q.dtype, device=self.device)
-        ws, nws = self._workspace((G, k, "picks"), lib().fathom_kv8_attend_picks_workspace_bytes, G, k, int(self.host))
+        out = torch.empty_like(q)
+        ws, nws = self._unused, 256
+        if self.host:
+            ws, nws = self._workspace((G, k, "picks"), lib().fathom_kv8_attend_picks_workspace_bytes, G, k, 1)
         check(lib().fathom_kv8_attend_picks(q.data_ptr(), _lib.DTYPE_CODE[q.dtype], self.B, self.Hkv, G, idx.data_ptr(), k,
                                             self.rows.data_ptr(), int(self.host), self.scales.data_ptr(), self.cap, num,
                                             ptr(dev), out.data_ptr(), ws.data_ptr(), nws, self._stream()),
@@ -204,8 +208,9 @@ class KVCache8:
 
 
 def _rows16(x):
-    """x with 16-byte aligned, contiguous 128-element rows (a copy where it has none)."""
+    """x with 16-byte aligned, contiguous 128-element rows (a copy where it has none), and its other strides."""
     sb, sh, st, sd = x.stride()
     if sd != 1 or (sb | sh | st) * x.element_size() % 16 or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+        x = x.clone(memory_format=torch.contiguous_format)
+        sb, sh, st, sd = x.stride()
+    return x, sb, sh, st
