@@ -75,6 +75,8 @@ struct WriteArgs {
 template <typename T>
 __global__ void __launch_bounds__(WT) kv8_write_kernel(WriteArgs a) {
   __shared__ uint32_t s_max[WT / 32];
+  tc::launch_dependents();
+  tc::wait_dependency();
   const int64_t bh = blockIdx.y;
   const int b = (int)bh / a.Hkv, h = (int)bh % a.Hkv, which = blockIdx.z;
   const int64_t start = a.start_dev ? a.start_dev[b] : a.start;
@@ -181,6 +183,8 @@ __global__ void __launch_bounds__(RT) kv8_read_kernel(const uint8_t* __restrict_
   using Codes = std::conditional_t<sizeof(T) == 4, uint32_t, uint2>;
   constexpr int E = sizeof(Codes), PER = KV8_ROW / E;        // codes of a thread; threads per token
   constexpr int TOK = RT / PER;                              // tokens per pass
+  tc::launch_dependents();
+  tc::wait_dependency();
   const int64_t bh = blockIdx.y;
   const int c = threadIdx.x % PER, which = c / (PER / 2);
   const int64_t t0 = (int64_t)blockIdx.x * (TOK * RPASS) + threadIdx.x / PER;
@@ -204,11 +208,12 @@ __global__ void __launch_bounds__(RT) kv8_read_kernel(const uint8_t* __restrict_
 }
 
 template <typename T>
-void launch_read(const uint8_t* rows, const float* scales, int64_t BH, int64_t cap, int64_t start, int64_t n, void* K, void* V,
-                 cudaStream_t st) {
+int launch_read(const uint8_t* rows, const float* scales, int64_t BH, int64_t cap, int64_t start, int64_t n, void* K, void* V,
+                cudaStream_t st) {
   constexpr int tokens = RT / (KV8_ROW / (sizeof(T) == 4 ? 4 : 8)) * RPASS;
   const dim3 grid((unsigned)cdiv(n, tokens), (unsigned)BH);
-  kv8_read_kernel<T><<<grid, RT, 0, st>>>(rows, scales, cap, start, n, (T*)K, (T*)V);
+  return launch_after(kv8_read_kernel<T>, grid, RT, 0, st, "kv8_read", rows, scales, cap, start, n,
+                      reinterpret_cast<T*>(K), reinterpret_cast<T*>(V));
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -240,10 +245,10 @@ extern "C" int fathom_kv8_write(const void* K, const void* V, int dtype, int64_t
   const WriteArgs a{K, V, stride_b, stride_h, stride_t, T, cap, start, start_dev, (int)Hkv, rows, scales};
   const dim3 grid((unsigned)nb, (unsigned)(B * Hkv), 2);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == FATHOM_DTYPE_F32) kv8_write_kernel<float><<<grid, WT, 0, st>>>(a);
-  else if (dtype == FATHOM_DTYPE_BF16) kv8_write_kernel<__nv_bfloat16><<<grid, WT, 0, st>>>(a);
-  else kv8_write_kernel<__half><<<grid, WT, 0, st>>>(a);
-  return check_launch("kv8_write");
+  return launch_after(dtype == FATHOM_DTYPE_F32    ? kv8_write_kernel<float>
+                      : dtype == FATHOM_DTYPE_BF16 ? kv8_write_kernel<__nv_bfloat16>
+                                                   : kv8_write_kernel<__half>,
+                      grid, WT, 0, st, "kv8_write", a);
 }
 
 extern "C" int fathom_kv8_read(const uint8_t* rows, const float* scales, int64_t BH, int64_t cap, int64_t start, int64_t n,
@@ -259,8 +264,7 @@ extern "C" int fathom_kv8_read(const uint8_t* rows, const float* scales, int64_t
                  "kv8_read: rows, K and V must be 16-byte aligned");
   if (n == 0) return FATHOM_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == FATHOM_DTYPE_F32) launch_read<float>(rows, scales, BH, cap, start, n, K, V, st);
-  else if (dtype == FATHOM_DTYPE_BF16) launch_read<__nv_bfloat16>(rows, scales, BH, cap, start, n, K, V, st);
-  else launch_read<__half>(rows, scales, BH, cap, start, n, K, V, st);
-  return check_launch("kv8_read");
+  if (dtype == FATHOM_DTYPE_F32) return launch_read<float>(rows, scales, BH, cap, start, n, K, V, st);
+  if (dtype == FATHOM_DTYPE_BF16) return launch_read<__nv_bfloat16>(rows, scales, BH, cap, start, n, K, V, st);
+  return launch_read<__half>(rows, scales, BH, cap, start, n, K, V, st);
 }

@@ -10,6 +10,7 @@
 // become e4m3 subnormals, a dequantised value is exact in bf16, and a scale folded into a score is exact.
 #pragma once
 #include "common.cuh"
+#include "tc.cuh"
 
 #include <cuda_fp8.h>
 
@@ -41,6 +42,25 @@ __device__ __forceinline__ uint32_t kv8_encode2(float y0, float y1) {
 __device__ __forceinline__ float2 kv8_decode2(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xFFFFu), __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Launches a kernel that may start while the one before it in the stream still ends: every thread
+// calls tc::wait_dependency() before it touches memory or returns (so a kernel that has ended says that those before it have).
+template <typename K, typename... A>
+int launch_after(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const char* what, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "%s: launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
 }
 
 }  // namespace fathom

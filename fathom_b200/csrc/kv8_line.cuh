@@ -210,21 +210,5 @@ inline int plan_shares(Args& a, int most, int piece, int whole, int least) {
   return (int)cdiv(items * a.stride, a.share);
 }
 
-// Launches the kernel that joins the parts of cut items; it may start while the kernel before still runs, and waits for it.
-template <typename K> int launch_join(K kernel, dim3 grid, int threads, const Args& a, int ctas, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, ctas);
-  if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend: %s", cudaGetErrorString(e));
-  return check_launch("kv8_attend");
-}
-
 }  // namespace kv8
 }  // namespace fathom

@@ -129,6 +129,8 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   const unsigned crank = blockIdx.y;
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();                            // waited for before the first store into another CTA
+  tc::wait_dependency();                               // (nothing is let start early: clusters of the next call in the gaps
+                                                       // of this one's leave it no room for whole ones, 39 us for 26)
   const int64_t bhg = blockIdx.x;
   const int bh = (int)bhg / a.G, gw = (int)crank * PW + warp;
   int64_t end = a.end_dev ? a.end_dev[bh / a.Hkv] : a.end;
@@ -352,13 +354,15 @@ int launch_picks(const void* q, int dtype, const PicksArgs& a, int64_t heads, in
   cfg.blockDim = dim3((unsigned)pw * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = (unsigned)cs;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;     // may start while the kernel before it ends
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, picks_kernel, q, dtype, a, out);
   if (e != cudaSuccess) return set_error(FATHOM_ERR_CUDA, "kv8_attend_picks: launch: %s", cudaGetErrorString(e));
   return check_launch("kv8_attend_picks");

@@ -121,6 +121,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     s_gave_up = 0;
   }
   if (warp == 20) tc::tmem_alloc(tc::smem_u32(&s_tmem), 512);
+  tc::wait_dependency();
   int count, share;
   const Place place = my_share(a, &count, &share);
   tc::fence_before();
@@ -537,6 +538,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
 constexpr int JOIN_WARPS = 8, JOIN_BLOCKS = 16;    // blocks per cut
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args a, int ctas) {
+  tc::launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = items_per_bh(a);
   tc::wait_dependency();                           // the parts are written; and nothing ends before they are
   const int4 cut = cuts_of(a)[blockIdx.x];         // item, its tiles, those in share c, tiles per share
@@ -582,9 +584,9 @@ template <typename T, int QT> int launch(const CUtensorMap& map, const Args& a, 
   static std::atomic<uint64_t> told{0};
   const int r = allow_smem(prompt_kernel<T, QT>, S::SMEM, told, "kv8_attend");
   if (r != FATHOM_OK) return r;
-  prompt_kernel<T, QT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (ctas == 1 || (a.share && a.share == a.stride)) return check_launch("kv8_attend");   // no item is cut
-  return launch_join(prompt_join_kernel<T>, dim3(ctas - 1, JOIN_BLOCKS), JOIN_WARPS * 32, a, ctas, st);
+  const int e = launch_after(prompt_kernel<T, QT>, dim3(ctas), THREADS, S::SMEM, st, "kv8_attend", map, a);
+  if (e != FATHOM_OK || ctas == 1 || (a.share && a.share == a.stride)) return e;          // no item is cut
+  return launch_after(prompt_join_kernel<T>, dim3(ctas - 1, JOIN_BLOCKS), JOIN_WARPS * 32, 0, st, "kv8_attend", a, ctas);
 }
 
 }  // namespace

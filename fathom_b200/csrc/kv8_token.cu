@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
   const int tid = threadIdx.x, lane = tid & 31, warp = (int)tc::uniform(tid >> 5);
   volatile int* gave_up = &s_gave_up;
 
+  tc::wait_dependency();
   int count, share;
   const Place place = my_share(a, &count, &share);
   Walk w(a, place, count);
@@ -505,6 +506,7 @@ template <typename T>
 __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   __shared__ int64_t s_before, s_total;
   __shared__ float s_m[MAX_CTAS], s_e[MAX_CTAS], s_red[2][D / 32];
+  tc::launch_dependents();
   const int R = rows_of(a), tid = threadIdx.x, lane = tid & 31;
   const int bh = blockIdx.x / R, r = blockIdx.x % R, b = bh / a.Hkv, h = bh % a.Hkv;
   const int nt = tiles_of(a, seq_end(a, b), 0);
@@ -561,9 +563,9 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> told{0};
   const int r = allow_smem(token_kernel<T, NR, QT, SPLIT>, S::SMEM, told, "kv8_attend");
   if (r != FATHOM_OK) return r;
-  token_kernel<T, NR, QT, SPLIT><<<ctas, THREADS, S::SMEM, st>>>(map, a);
-  if (a.share && a.share == a.stride) return check_launch("kv8_attend");     // every row whole: nothing to join
-  return launch_join(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, a, ctas, st);
+  const int e = launch_after(token_kernel<T, NR, QT, SPLIT>, dim3(ctas), THREADS, S::SMEM, st, "kv8_attend", map, a);
+  if (e != FATHOM_OK || (a.share && a.share == a.stride)) return e;     // every row whole: nothing to join
+  return launch_after(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, 0, st, "kv8_attend", a, ctas);
 }
 
 template <typename T, int QT>
