@@ -18,7 +18,8 @@
 // leaves e4m3's range room on both sides.  The denominator is kept per thread in fp32 with a reference of its
 // own, because the value scale must not enter it.  One tile's chain of steps is longer than its bytes take, so there are
 // two softmax warpgroups: up to 16 rows they take the even and the odd tiles, each with its own references and its own
-// O^T; up to 32 rows (SPLIT) each takes 16 rows of every tile.
+// O^T; up to 32 rows (SPLIT) each takes 12 or 16 rows
+// of every tile.
 //
 // A row's parts in different CTAs (kv8_line.cuh) are joined by a second kernel in a fixed order.
 //
@@ -43,9 +44,9 @@ constexpr int MAX_CTAS = 512;                    // shares that the join kernel 
 
 constexpr int up16(int n) { return (n + 15) / 16 * 16; }
 
-// NR: rows of a softmax thread; SPLIT: the two warpgroups have NR rows each.
+// NR: rows of a softmax thread; SPLIT: the two warpgroups have NR rows each, in NC = 16 columns of a term's RT.
 template <int NR, int QT, bool SPLIT> struct Shape {
-  static constexpr int RT = SPLIT ? 2 * NR : NR;
+  static constexpr int ROWS = SPLIT ? 2 * NR : NR, NC = SPLIT ? 16 : NR, RT = SPLIT ? 2 * NC : NR;
   static constexpr int NQ = up16(RT * QT), NP = up16(RT * TERMS);
   static constexpr int COLS = 2 * NQ + (SPLIT ? 1 : 2) * NP;     // S^T of even and odd tiles, then O^T
   static constexpr int TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
@@ -72,17 +73,17 @@ template <typename T, int NR, int QT, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant__ CUtensorMap map,
                                                           const __grid_constant__ Args a) {
   using S = Shape<NR, QT, SPLIT>;
-  constexpr int STAGES = S::STAGES, RT = S::RT;
+  constexpr int STAGES = S::STAGES, RT = S::RT, NC = S::NC, ROWS = S::ROWS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (tc::smem_u32(smem_raw) & 1023)) & 1023);
   const uint32_t sbase = tc::smem_u32(smem);
   __shared__ __align__(8) uint64_t bars[2 * STAGES + 10];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
-  __shared__ float s_rs[RT];                     // scale of a row's scores: 2^e log2(e) / sqrt(128)
+  __shared__ float s_rs[ROWS];                    // scale of a row's scores: 2^e log2(e) / sqrt(128)
   __shared__ float s_top[2][4][NR];              // a tile's largest s + log2 vs, by warpgroup and warp
   // at a row's end: references; denominators by warp; then the denominator, its reference, and what brings O^T there
-  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[RT], s_ref[RT], s_f[2][RT];
+  __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[ROWS], s_ref[ROWS], s_f[2][ROWS];
   const uint32_t bar0 = tc::smem_u32(bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   auto empty = [&](uint32_t s) { return bar0 + 8 * (STAGES + s); };
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     const int R = rows_of(a), late = (int)a.T - 1, g = warp >> 2, t = tid & (GROUP - 1);
     const int first = SPLIT ? g * NR : 0;         // this thread's rows: first + (0 .. NR - 1)
     // A warp brings every eighth row of q, a lane 4 dims of it; the share's first row ahead of everything else.
-    constexpr int QR = (RT + 7) / 8;
+    constexpr int QR = (ROWS + 7) / 8;
     uint2 qv[QR];
     auto q_at = [&](int r, int h) {               // rows are token-major: row = token * G + head
       const int tt = late ? r / a.G : 0;
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     tc::launch_dependents();
     const uint32_t tm = s_tmem;
     const uint32_t my = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tm_s = tm + first + my, tm_o = tm + 2 * S::NQ + first + my;
+    const uint32_t tm_s = tm + (SPLIT ? g * NC : 0) + my, tm_o = tm_s + 2 * S::NQ;
     uint8_t* const pb = smem + S::P + t * 16;
     uint32_t i0 = 0;                              // the share's tiles before this row
     bool ok = true, bad = false;                  // ok: this thread's waits; bad: some thread's gave up
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
         for (int term = 0; term < QT; ++term) {
           const uint32_t code = kv8_encode2(x[0], x[1]) | kv8_encode2(x[2], x[3]) << 16;
-          const int c = term * RT + r;
+          const int c = term * RT + (SPLIT ? r / NR * NC + r % NR : r);
           *reinterpret_cast<uint32_t*>(smem + S::Q + c * D + (((lane >> 2) ^ (c & 7)) << 4) + (lane & 3) * 4) = code;
           const float2 lo = kv8_decode2(code), hi = kv8_decode2(code >> 16);
           x[0] = (x[0] - lo.x) * 16.0f, x[1] = (x[1] - lo.y) * 16.0f;
@@ -288,9 +289,9 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
         tc::fence_after();
         float s[NR];
         {
-          uint32_t c[QT][NR];
+          uint32_t c[QT][NC];
 #pragma unroll
-          for (int term = 0; term < QT; ++term) tc::Tmem<NR>::ld(tm_s + k * S::NQ + term * RT, c[term]);
+          for (int term = 0; term < QT; ++term) tc::Tmem<NC>::ld(tm_s + k * S::NQ + term * RT, c[term]);
           tc::wait_ld();
           tc::fence_before();
           __syncwarp();
@@ -362,18 +363,18 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             tc::fence_after();
 #pragma unroll
             for (int term = 0; term < TERMS; ++term) {
-              uint32_t o[NR];
-              tc::Tmem<NR>::ld(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
+              uint32_t o[NC];
+              tc::Tmem<NC>::ld(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
               tc::wait_ld();
 #pragma unroll
               for (int r = 0; r < NR; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * f[r]);
-              tc::Tmem<NR>::st(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
+              tc::Tmem<NC>::st(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
             }
             tc::wait_st();
           }
         }
         // weights as terms into the operand buffer: 11 bits in f16, whose remainders after e4m3 are exact
-        uint32_t codes[TERMS * NR / 4];
+        uint32_t codes[TERMS * NC / 4] = {};
 #pragma unroll
         for (int r = 0; r < NR; r += 2) {
           float x[2];
@@ -390,14 +391,14 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
           for (int term = 0; term < TERMS; ++term) {
             const __half2_raw yr = *reinterpret_cast<const __half2_raw*>(&y);
             const uint32_t code = __nv_cvt_halfraw2_to_fp8x2(yr, __NV_SATFINITE, __NV_E4M3);
-            uint32_t& word = codes[(term * NR + r) / 4];
+            uint32_t& word = codes[(term * NC + r) / 4];
             word = (r & 2) ? word | code << 16 : code;
             const __half2_raw c = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code, __NV_E4M3);
             const __half2 sixteen = __float2half2_rn(16.0f);
             y = __hmul2(__hsub2(y, *reinterpret_cast<const __half2*>(&c)), sixteen);
           }
         }
-        // columns term * RT + first + r; with NR = 16 a term's rows are a 16-byte piece of their own
+        // columns as q's; with NC = 16 a term's rows are a 16-byte piece of their own
         constexpr int PIECES = SPLIT ? TERMS : S::NP / 16;
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) {
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int at = 4 * c + e;
-            x[e] = at < TERMS * NR / 4 ? codes[at < TERMS * NR / 4 ? at : 0] : 0;
+            x[e] = at < TERMS * NC / 4 ? codes[at < TERMS * NC / 4 ? at : 0] : 0;
           }
           uint8_t* const at = pb + k * S::NP * TILE + (SPLIT ? 2 * c + g : c) * TILE * 16;
           *reinterpret_cast<uint4*>(at) = make_uint4(x[0], x[1], x[2], x[3]);
@@ -431,7 +432,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       const Walk now = w;
       more = w.next();
       if (more) load_q();                         // the next row's q, on its way while this one is finished
-      if (tid < RT) {
+      if (tid < ROWS) {
         // the warps that have the row, and its place among their rows
         const int v0 = SPLIT ? tid / NR * 4 : 0, r = SPLIT ? tid % NR : tid;
         constexpr int NV = SPLIT ? 4 : 8;
@@ -574,6 +575,7 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   if (R <= 4) return launch<T, 4, QT, false>(map, a, ctas, st);
   if (R <= 8) return launch<T, 8, QT, false>(map, a, ctas, st);
   if (R <= 16) return launch<T, 16, QT, false>(map, a, ctas, st);
+  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);
   return launch<T, 16, QT, true>(map, a, ctas, st);
 }
 
