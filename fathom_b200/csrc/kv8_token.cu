@@ -575,7 +575,7 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   if (R <= 4) return launch<T, 4, QT, false>(map, a, ctas, st);
   if (R <= 8) return launch<T, 8, QT, false>(map, a, ctas, st);
   if (R <= 16) return launch<T, 16, QT, false>(map, a, ctas, st);
-  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);
+  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);      // 20 rows over 16k: 22 us, with 16 per thread 25
   return launch<T, 16, QT, true>(map, a, ctas, st);
 }
 
