@@ -1,8 +1,9 @@
 // Attention over listed rows of the 8-bit cache (layout in kv8.cuh), one list per query head.
 //
 // The floor is the rows' bytes, 256 at random addresses per pick, and for one sequence latency.  A warp takes 32 picks at
-// a time; their rows come into shared memory by 16-byte asynchronous copies while it works on the 32 before.  With one query row per list a product has nothing to share, but the matrix instructions take e4m3 as
-// it lies in memory, so nothing is dequantised:
+// a time; their rows come into shared memory by 16-byte asynchronous copies while it works on the 32 before.  With one
+// query row per list a product has nothing to share, but the matrix instructions take e4m3 as it lies in memory, so
+// nothing is dequantised:
 //
 //   scores   [32 picks x 8] = K [32 x 128] q^T          columns: q as a sum of six e4m3 terms, 16^-n apart (24 bits)
 //   output^T [128 dims x 8] += V^T [128 x 32 picks] p   columns: the weights as six such terms
@@ -15,10 +16,10 @@
 // states are joined in warp order in the first CTA's shared memory.
 //
 // Measured over 128k: 2116 picks for each of 224 heads 26 us, 4.7 TB/s of rows (34 with 16-bit matrix instructions on
-// rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24:
-// the copies' way into shared memory is the bound, some 340 cycles per 32 picks and SM.  12 warps per SM, or 3 stages, are
-// slower (29 us), so are TMA gathers of 4 rows (28), bulk copies of one (34) and rows loaded into registers (29).  580
-// picks for 32 heads: 5.5 us with its launch.
+// rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24.
+// ~5 us of it begin and join; the rest is 32 picks per 340 cycles and SM, 6 TB/s.  12 warps per SM, or 3 stages, are
+// slower (29 us), so are TMA gathers of 4 rows (28; for the keys alone 28.5), bulk copies of one (34) and rows loaded into
+// registers (29).  580 picks for 32 heads: 5.3 us in a graph.
 #include "dedupe.cuh"
 #include "kv8_attn.cuh"
 

@@ -566,7 +566,8 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   if (r != FATHOM_OK) return r;
   const int e = launch_after(token_kernel<T, NR, QT, SPLIT>, dim3(ctas), THREADS, S::SMEM, st, "kv8_attend", map, a);
   if (e != FATHOM_OK || (a.share && a.share == a.stride)) return e;     // every row whole: nothing to join
-  return launch_after(token_join_kernel<T>, dim3((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T)), D, 0, st, "kv8_attend", a, ctas);
+  const dim3 rows((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T));
+  return launch_after(token_join_kernel<T>, rows, D, 0, st, "kv8_attend", a, ctas);
 }
 
 template <typename T, int QT>
