@@ -187,6 +187,19 @@ def test_attend_matches_the_oracle(dtype, G, T, n):
     _close(out, ref, mag)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("G,T,n", [(4, 5, 1000), (3, 6, 777), (6, 3, 65), (8, 3, 640), (1, 24, 300), (5, 5, 901), (1, 18, 20),
+                                   (1, 25, 128), (7, 4, 515), (4, 8, 2049)])
+def test_attend_of_17_to_32_rows(dtype, G, T, n):
+    """Rows shared by two groups of threads, at one length and at ragged ones (the first rows of which see nothing)."""
+    B, H = 3, 2
+    c, rows, scales = _filled(B, H, n, G + T + n, cap=n + 40)
+    q = (2 * torch.randn(B, H * G, T, 128, generator=torch.Generator().manual_seed(n))).to(DT[dtype])
+    for ends in ([n] * B, [n, T - 2, n // 2]):
+        ref, mag = O.attend(_np(q), rows, scales, ends, H)
+        _close(c.attend(q.cuda(), torch.tensor(ends, device="cuda")), ref, mag)
+
+
 @pytest.mark.parametrize("T", [1, 3, 7, 40, 129])
 def test_attend_at_device_lengths(T):
     """Ragged lengths on the device: none, one, fewer than the queries, a block's edge, the whole cache, above it."""
@@ -311,6 +324,58 @@ def test_picks_match_the_oracle(dtype, B, H, G, k):
     idx = torch.randint(0, n, (B * H, G, k), generator=g)
     ref, mag = O.attend_picks(_np(q), idx.numpy(), rows, scales, [n] * (B * H))
     _close(c.attend_picks(q.cuda(), idx.cuda()), ref, mag, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("k", [31, 32, 33, 95, 200])
+def test_picks_of_wide_ranges(k):
+    """Values of very different block scales, queries of very different elements, lists around whole steps of 32."""
+    from fathom_b200.kv8 import KVCache8
+    n, H, G = 512, 2, 3
+    K, V = _kv(1, H, n, torch.float32, k)
+    V[:, 0, 64:128] *= 2.0 ** 30
+    V[:, 0, 256:320] *= 2.0 ** -30
+    V[:, 1, :64] = 0
+    K[:, 1, 128:192] *= 2.0 ** -20
+    c = KVCache8(1, H, n)
+    c.write(K, V)
+    g = torch.Generator().manual_seed(k)
+    q = 2 * torch.randn(H, G, 128, generator=g)
+    q[:, 1] *= torch.exp2(torch.randint(-30, 1, (128,), generator=g).float())
+    q[:, 2] = 0
+    idx = torch.randint(0, n, (H, G, k), generator=g)
+    rows, scales = c.rows.cpu().numpy(), c.scales.cpu().numpy()
+    ref, mag = O.attend_picks(_np(q), idx.numpy(), rows, scales, [n] * H)
+    _close(c.attend_picks(q.cuda(), idx.cuda()), ref, mag, 2.0 ** -17)
+
+
+def test_calls_in_a_row_see_each_other():
+    """Each call may be launched while the one before it ends: 40 steps whose inputs are the outputs before them give the
+    same bits as with a wait after every call."""
+    from fathom_b200.kv8 import KVCache8
+    B, H, G, n0 = 2, 4, 4, 500
+    K, V = _kv(B, H, n0, torch.bfloat16, 50)
+    idx = torch.randint(0, n0, (B * H, G, 100), generator=torch.Generator().manual_seed(51)).cuda()
+
+    def steps(wait):
+        c = KVCache8(B, H, 1024)
+        done = torch.cuda.synchronize if wait else (lambda: None)
+        c.write(K, V, 0)
+        pos = torch.full((B,), n0, device="cuda")
+        out = K[:, :, -1:].repeat_interleave(G, 1)
+        for t in range(40):
+            c.write(out[:, ::G], out[:, 1::G], pos)
+            done()
+            pos += 1
+            x = c.attend((out + K[:, :, t:t + 1].repeat_interleave(G, 1)).contiguous(), pos if t % 2 else n0 + t + 1)
+            done()
+            y = c.attend_picks(x.reshape(B * H, G, 128), idx + t, pos)
+            done()
+            z, _ = c.read(n0 + t, 1)
+            done()
+            out = x + y.view_as(x) + z.repeat_interleave(G, 1)
+        return out
+
+    assert torch.equal(steps(False), steps(True))
 
 
 def test_picks_outside_are_ignored():
