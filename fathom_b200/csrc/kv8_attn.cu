@@ -110,7 +110,8 @@ extern "C" int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hk
   unsigned long long* timeouts = timeout_counter();
   if (!timeouts) return set_error(FATHOM_ERR_CUDA, "kv8_attend: no address of the wait counter");
   const Args a{q, q_stride_b, q_stride_h, q_stride_t, out, o_stride_b, o_stride_h, o_stride_t, rows, scales, cap, end,
-               end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts, 0, 0, 1, 0, 0};
+               end_dev, (int)B, (int)Hkv, G, T, reinterpret_cast<float*>(workspace), timeouts, 0, 0, 1, 0, 0,
+               1.0f / (float)G, 1.0f / (float)Hkv};
   CUtensorMap map;
   const int r = rows_map(a, &map);
   if (r != FATHOM_OK) return r;

@@ -31,7 +31,12 @@ struct Args {
   int share, stride, least;
   int64_t tiles_bh;               // tiles of one row bh, where the host knows them; else 0
   int ctas;                       // of the prompt kernel
+  float inv_g, inv_hkv;           // 1 / G, 1 / Hkv for div_small
 };
+
+// x / d for 0 <= x < 2^20 from 1 / d: x + 0.5 is half a step of 1 / d away from the next whole number, which the three
+// roundings cannot cross.  (Code that runs once is paid for by its instructions' way to the SM: a division has ~25.)
+__device__ __forceinline__ int div_small(int x, float inv_d) { return __float2int_rd(((float)x + 0.5f) * inv_d); }
 
 // Tokens of sequence b that exist.
 __device__ __forceinline__ int seq_end(const Args& a, int b) {

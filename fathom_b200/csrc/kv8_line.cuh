@@ -20,8 +20,9 @@ __device__ __forceinline__ int items_per_bh(const Args& a) { return (rows_of(a) 
 // Keys that row `row` (token-major) of a sequence with `end` tokens sees.
 __device__ __forceinline__ int seen(const Args& a, int end, int row) { return end - ((int)a.T - 1) + row / a.G; }
 
-// Tiles of item `it` of a row bh: up to its last row's last key, one at least.
-__device__ __forceinline__ int tiles_of(const Args& a, int end, int it) {
+// Tiles of item `it` of a row bh: up to its last row's last key, one at least.  ONE: every bh is known to be one item.
+template <bool ONE = false> __device__ __forceinline__ int tiles_of(const Args& a, int end, int it) {
+  if (ONE) return max(1, (end + TILE - 1) / TILE);
   const int last = min((int64_t)(it + 1) * ROWS, (int64_t)rows_of(a)) - 1;
   return max(1, (seen(a, end, last) + TILE - 1) / TILE);
 }
@@ -116,7 +117,7 @@ __device__ __forceinline__ int64_t share_of(const Args& a, int64_t total, int ct
 
 // One warp: where this CTA's share begins, how many tiles it has (0 or less: none) and how many a CTA has at most.  A
 // token's latency counts on this: the common forms, a plan or up to 32 sequences of one item per bh, take one pass.
-__device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
+template <bool ONE = false> __device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
   const int lane = threadIdx.x & 31;
   Place p{0, 0};
   if (a.share) {
@@ -124,13 +125,13 @@ __device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
     *per_cta = a.share;
     p.item = (int)quotient(at, a.stride);
     p.tile = (int)(at - (int64_t)p.item * a.stride);
-    const int nt = tiles_of(a, seq_end(a, 0), p.item % items_per_bh(a));
+    const int nt = tiles_of<ONE>(a, seq_end(a, 0), ONE ? 0 : p.item % items_per_bh(a));
     const bool apart = a.stride > nt || a.share == a.stride;       // no other item's tiles in this share
     *count = (int)min((int64_t)a.share, apart ? (int64_t)nt - p.tile : (int64_t)a.B * a.Hkv * nt - at);
     return p;
   }
-  if (items_per_bh(a) == 1 && a.B <= 32) {       // (ragged: equal lengths have a plan)
-    const int nt = lane < a.B ? tiles_of(a, seq_end(a, lane), 0) : 0;
+  if ((ONE || items_per_bh(a) == 1) && a.B <= 32) {       // (ragged: equal lengths have a plan)
+    const int nt = lane < a.B ? tiles_of<ONE>(a, seq_end(a, lane), 0) : 0;
     const int64_t mine = (int64_t)nt * a.Hkv;
     int64_t x = mine;
 #pragma unroll
@@ -157,22 +158,22 @@ __device__ inline Place my_share(const Args& a, int* count, int* per_cta) {
 
 // A share as its pieces of items, the same walk in every role; made by a converged warp and uniform as the compiler sees
 // it, so that loops over it are.
-struct Walk {
+template <bool ONE = false> struct Walk {
   const Args& a;
   int per, item, tile, left;
   int b, bh, it, end, n, j0, j1;   // item within bh; its sequence's tokens; its tiles; this piece's tiles [j0, j1)
   __device__ Walk(const Args& a_, const Place& p, int count)
-      : a(a_), per(items_per_bh(a_)), item(tc::uniform(p.item)), tile(tc::uniform(p.tile)),
+      : a(a_), per(ONE ? 1 : items_per_bh(a_)), item(tc::uniform(p.item)), tile(tc::uniform(p.tile)),
         left(tc::uniform(max(count, 0))) {}
   // accumulators of 128 rows that the item needs
   __device__ int halves() const { return rows_of(a) - it * ROWS > ROWS / 2 ? 2 : 1; }
   __device__ bool next() {
     if (left <= 0) return false;
-    bh = item / per;
+    bh = ONE ? item : item / per;
     it = item - bh * per;
-    b = bh / a.Hkv;
+    b = div_small(bh, a.inv_hkv);
     end = seq_end(a, b);
-    n = tiles_of(a, end, it);
+    n = tiles_of<ONE>(a, end, it);
     j0 = tile;
     j1 = min(n, j0 + left);
     left -= j1 - j0;

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   tc::fence_after();
   tc::launch_dependents();
   const uint32_t tm = s_tmem;                      // S_0, S_1, O_0, O_1: 128 columns each
-  Walk w(a, place, count);
+  Walk<> w(a, place, count);
 
   if (group < 4) {
     // ---- softmax of half h2: two threads per row, thread `ch` for the tile's 64-token block ch and dims 64 ch ..

@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
   __shared__ float s_top[2][4][NR];              // a tile's largest s + log2 vs, by warpgroup and warp
   // at a row's end: references; denominators by warp; then the denominator, its reference, and what brings O^T there
   __shared__ float s_m[2][NR], s_lm[8][NR], s_l[8][NR], s_sum[ROWS], s_ref[ROWS], s_f[2][ROWS];
+  __shared__ int64_t s_out[ROWS];                // where a row's output begins
   const uint32_t bar0 = tc::smem_u32(bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };
   auto empty = [&](uint32_t s) { return bar0 + 8 * (STAGES + s); };
@@ -98,8 +99,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 
   tc::wait_dependency();
   int count, share;
-  const Place place = my_share(a, &count, &share);
-  Walk w(a, place, count);
+  const Place place = my_share<true>(a, &count, &share);
+  Walk<true> w(a, place, count);
   if (warp == 8) {
     // ---- loads: the share's tiles in order, as stages come free.  They begin while the CTA still sets itself up.
     if (lane == 0) {
@@ -205,16 +206,13 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     // A warp brings every eighth row of q, a lane 4 dims of it; the share's first row ahead of everything else.
     constexpr int QR = (ROWS + 7) / 8;
     uint2 qv[QR];
-    auto q_at = [&](int r, int h) {               // rows are token-major: row = token * G + head
-      const int tt = late ? r / a.G : 0;
-      return w.b * a.qb + (int64_t)(h * a.G + r - tt * a.G) * a.qh + tt * a.qt;
-    };
-    auto load_q = [&]() {
-      const int h = w.bh % a.Hkv;
+    auto load_q = [&]() {                         // rows are token-major: row = token * G + head
+      const int64_t step = a.qt - a.G * a.qh;
+      const T* const q0 = reinterpret_cast<const T*>(a.q) + w.b * a.qb + (int64_t)(w.bh - w.b * a.Hkv) * a.G * a.qh + lane * 4;
 #pragma unroll
       for (int i = 0; i < QR; ++i) {
         const int r = warp + 8 * i;
-        if (r < R) qv[i] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(a.q) + q_at(r, h) + lane * 4);
+        if (r < R) qv[i] = *reinterpret_cast<const uint2*>(q0 + r * a.qh + (late ? div_small(r, a.inv_g) : 0) * step);
       }
     };
     bool more = w.next();
@@ -233,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     uint32_t i0 = 0;                              // the share's tiles before this row
     bool ok = true, bad = false;                  // ok: this thread's waits; bad: some thread's gave up
     while (more) {
-      const int h = w.bh % a.Hkv, n = w.j1 - w.j0;
+      const int h = w.bh - w.b * a.Hkv, n = w.j1 - w.j0;
       // this row's queries as terms.  The products of the row before are complete (its O^T was read below), so its q
       // may go.
 #pragma unroll
@@ -326,7 +324,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) vrow[c] = make_uint4(0, 0, 0, 0);
           }
-          int room = w.end - tok - late + first / a.G, head = first % a.G;     // keys left to the row's token: seen if > 0
+          int room = div_small(first, a.inv_g), head = first - room * a.G;
+          room += w.end - tok - late;                          // keys left to the row's token: seen if > 0
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             if (room <= 0) s[r] = -INFINITY;
@@ -429,9 +428,11 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       tc::fence_before();
       bad = tc::uniform(tc::named_or(3, 2 * GROUP, !ok));
       tc::fence_after();
-      const Walk now = w;
+      const Walk<true> now = w;
       more = w.next();
       if (more) load_q();                         // the next row's q, on its way while this one is finished
+      const bool whole = now.j0 == 0 && now.j1 == now.n;
+      float* const parts = a.part + ((int64_t)blockIdx.x + now.bh) * R * PART;
       if (tid < ROWS) {
         // the warps that have the row, and its place among their rows
         const int v0 = SPLIT ? tid / NR * 4 : 0, r = SPLIT ? tid % NR : tid;
@@ -443,16 +444,19 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
         for (int v = 0; v < NV; ++v) sum = fmaf(s_l[v0 + v][r], ex2(s_lm[v0 + v][r] - mx), sum);
         s_sum[tid] = sum;
         s_ref[tid] = mx;
+        const int tt = late ? div_small(tid, a.inv_g) : 0;
+        s_out[tid] = now.b * a.ob + (int64_t)(h * a.G + tid - tt * a.G) * a.oh + tt * a.ot;
+        const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         // O^T is relative to m - HEAD: both come to the denominator's reference.  A warpgroup that had no tile left its
         // columns as they were.
 #pragma unroll
         for (int k = 0; k < (SPLIT ? 1 : 2); ++k) {
           const float m0 = s_m[SPLIT ? tid / NR : k][r];
-          s_f[k][tid] = (!SPLIT && n == 1 && k != (int)(i0 & 1)) || m0 == -INFINITY ? 0.0f : exp2f(m0 - HEAD - mx);
+          const bool none = (!SPLIT && n == 1 && k != (int)(i0 & 1)) || m0 == -INFINITY;
+          s_f[k][tid] = (none ? 0.0f : exp2f(m0 - HEAD - mx)) * scale;       // (NaN where the denominator is)
         }
       }
       tc::named_sync(3, 2 * GROUP);
-      const bool whole = now.j0 == 0 && now.j1 == now.n;
       // warpgroup g finishes its own rows, or of 4 rows r = g mod 2 (4 at a time: run once a row, small code is fast code)
 #pragma unroll 1
       for (int r0 = 0; r0 < NR; r0 += 4) {
@@ -477,16 +481,12 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             for (int term = TERMS - 2; term >= 0; --term) v = fmaf(v, 0.0625f, __uint_as_float(c[k][term][rr]));
             if (s_f[k][r] != 0.0f) x = fmaf(v, s_f[k][r], x);
           }
-          const float sum = s_sum[r];
           if (bad) x = __uint_as_float(0x7FFFFFFFu);
           if (whole) {
-            const int tt = late ? r / a.G : 0;
-            T* op = reinterpret_cast<T*>(a.out) + now.b * a.ob + (int64_t)(h * a.G + r - tt * a.G) * a.oh + tt * a.ot;
-            from_f32(bad ? x : sum == 0.0f ? 0.0f : x / sum, op + t);
+            from_f32(x, reinterpret_cast<T*>(a.out) + s_out[r] + t);
           } else {
-            float* part = a.part + (((int64_t)blockIdx.x + now.bh) * R + r) * PART;
-            part[t] = x;
-            if (t == 0) part[D] = s_ref[r], part[D + 1] = sum;
+            parts[r * PART + t] = x;
+            if (t == 0) parts[r * PART + D] = s_ref[r], parts[r * PART + D + 1] = s_sum[r];
           }
         }
       }
@@ -509,13 +509,13 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   __shared__ float s_m[MAX_CTAS], s_e[MAX_CTAS], s_red[2][D / 32];
   tc::launch_dependents();
   const int R = rows_of(a), tid = threadIdx.x, lane = tid & 31;
-  const int bh = blockIdx.x / R, r = blockIdx.x % R, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int nt = tiles_of(a, seq_end(a, b), 0);
+  const int bh = blockIdx.y, r = blockIdx.x, b = div_small(bh, a.inv_hkv), h = bh - b * a.Hkv;
+  const int nt = tiles_of<true>(a, seq_end(a, b), 0);
   if (a.end_dev && tid < 32) {
     // tiles of the sequences before b, and of all
     int64_t before = 0, total = 0;
     for (int j = tid; j < a.B; j += 32) {
-      const int64_t x = (int64_t)tiles_of(a, seq_end(a, j), 0) * a.Hkv;
+      const int64_t x = (int64_t)tiles_of<true>(a, seq_end(a, j), 0) * a.Hkv;
       total += x;
       if (j < b) before += x;
     }
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   float O = 0.0f;
 #pragma unroll 8
   for (int p = 0; p < n; ++p) O = fmaf(part[p * step + tid], s_e[p], O);
-  const int tt = r / a.G, hq = h * a.G + r - tt * a.G;
+  const int tt = div_small(r, a.inv_g), hq = h * a.G + r - tt * a.G;
   from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
 
@@ -566,7 +566,7 @@ int launch(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st) {
   if (r != FATHOM_OK) return r;
   const int e = launch_after(token_kernel<T, NR, QT, SPLIT>, dim3(ctas), THREADS, S::SMEM, st, "kv8_attend", map, a);
   if (e != FATHOM_OK || (a.share && a.share == a.stride)) return e;     // every row whole: nothing to join
-  const dim3 rows((unsigned)((int64_t)a.B * a.Hkv * a.G * a.T));
+  const dim3 rows((unsigned)(a.G * a.T), (unsigned)(a.B * a.Hkv));
   return launch_after(token_join_kernel<T>, rows, D, 0, st, "kv8_attend", a, ctas);
 }
 
