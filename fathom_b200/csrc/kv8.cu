@@ -177,9 +177,8 @@ constexpr int RPASS = 4;
 // the fp32 stores were 64 bytes apart: 69% of the copy rate).  Bound by HBM: a code read, 2 or 4 bytes written.
 // Measured, 128k tokens of 8 KV heads: to bf16 122 us, 6.6 TB/s; to fp32 207 us, 6.5 TB/s; the copy rate.
 template <typename T>
-__global__ void __launch_bounds__(RT) kv8_read_kernel(const uint8_t* __restrict__ rows, const float* __restrict__ scales,
-                                                      int64_t cap, int64_t start, int64_t n, T* __restrict__ K,
-                                                      T* __restrict__ V) {
+__global__ void __launch_bounds__(RT) kv8_read_kernel(const uint8_t* rows, const float* scales, int64_t cap, int64_t start,
+                                                      int64_t n, T* K, T* V) {
   using Codes = std::conditional_t<sizeof(T) == 4, uint32_t, uint2>;
   constexpr int E = sizeof(Codes), PER = KV8_ROW / E;        // codes of a thread; threads per token
   constexpr int TOK = RT / PER;                              // tokens per pass

@@ -45,7 +45,8 @@ __device__ __forceinline__ float2 kv8_decode2(uint32_t two) {
 }
 
 // Launches a kernel that may start while the one before it in the stream still ends: every thread
-// calls tc::wait_dependency() before it touches memory or returns (so a kernel that has ended says that those before it have).
+// calls tc::wait_dependency() before it touches memory or returns (so a kernel that has ended says that those before it have).  No
+// pointer is __restrict__: a load of memory declared constant could be moved before the wait.
 template <typename K, typename... A>
 int launch_after(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const char* what, const A&... args) {
   cudaLaunchConfig_t cfg = {};

@@ -116,7 +116,7 @@ __device__ __forceinline__ void load4(const void* p, int dtype, int64_t i, float
 }
 
 __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
-    picks_kernel(const void* __restrict__ q, int dtype, const PicksArgs a, void* __restrict__ out) {
+    picks_kernel(const void* q, int dtype, const PicksArgs a, void* out) {
   const int PW = blockDim.x >> 5, NW = PW * (int)gridDim.y;      // one cluster of gridDim.y CTAs per (batch, query head)
   extern __shared__ __align__(128) uint8_t smem_raw[];
   constexpr int MAX_NW = MAX_PW * MAX_CS;

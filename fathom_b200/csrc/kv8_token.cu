@@ -63,6 +63,13 @@ __device__ __forceinline__ uint64_t weight_operand(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(TILE * 16 >> 4) << 32 | 1ull << 46;
 }
 
+// 8 bytes if `there`.  (Written as a branch around a load, each row waited for the one before.)
+__device__ __forceinline__ void load8(uint2& x, const void* p, bool there) {
+  asm volatile("{ .reg .pred p; setp.ne.u32 p, %3, 0; @p ld.global.v2.u32 {%0, %1}, [%2]; }\n"
+               : "+r"(x.x), "+r"(x.y)
+               : "l"(p), "r"((uint32_t)there)
+               : "memory");
+}
 template <typename T> __device__ __forceinline__ void unpack4(uint2 v, float (&x)[4]) {
   const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
@@ -205,14 +212,14 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
     const int first = SPLIT ? g * NR : 0;         // this thread's rows: first + (0 .. NR - 1)
     // A warp brings every eighth row of q, a lane 4 dims of it; the share's first row ahead of everything else.
     constexpr int QR = (ROWS + 7) / 8;
-    uint2 qv[QR];
+    uint2 qv[QR] = {};
     auto load_q = [&]() {                         // rows are token-major: row = token * G + head
       const int64_t step = a.qt - a.G * a.qh;
       const T* const q0 = reinterpret_cast<const T*>(a.q) + w.b * a.qb + (int64_t)(w.bh - w.b * a.Hkv) * a.G * a.qh + lane * 4;
 #pragma unroll
       for (int i = 0; i < QR; ++i) {
         const int r = warp + 8 * i;
-        if (r < R) qv[i] = *reinterpret_cast<const uint2*>(q0 + r * a.qh + (late ? div_small(r, a.inv_g) : 0) * step);
+        load8(qv[i], q0 + r * a.qh + (late ? div_small(r, a.inv_g) : 0) * step, r < R);
       }
     };
     bool more = w.next();
