@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 template <typename T>
 __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   __shared__ int64_t s_before, s_total;
-  __shared__ float s_m[MAX_CTAS], s_e[MAX_CTAS], s_red[2][D / 32];
+  __shared__ float s_m[MAX_CTAS], s_l[MAX_CTAS], s_e[MAX_CTAS], s_red[2][D / 32];
   tc::launch_dependents();
   const int R = rows_of(a), tid = threadIdx.x, lane = tid & 31;
   const int bh = blockIdx.y, r = blockIdx.x, b = div_small(bh, a.inv_hkv), h = bh - b * a.Hkv;
@@ -541,8 +541,17 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   if (n == 1) return;
   const float* part = a.part + ((int64_t)(c0 + bh) * R + r) * PART;
   const int64_t step = (int64_t)R * PART;
+  // the first parts' dims are on their way while references and denominators are worked out
+  constexpr int AHEAD = 20;
+  float x[AHEAD];
+#pragma unroll
+  for (int p = 0; p < AHEAD; ++p) x[p] = part[min(p, n - 1) * step + tid];
   float M = -INFINITY;
-  for (int p = tid; p < n; p += D) M = fmaxf(M, s_m[p] = part[p * step + D]);
+  for (int p = tid; p < n; p += D) {
+    const float2 ml = *reinterpret_cast<const float2*>(part + p * step + D);
+    s_l[p] = ml.y;
+    M = fmaxf(M, s_m[p] = ml.x);
+  }
   M = warp_max(M);
   if (lane == 0) s_red[0][tid >> 5] = M;
   __syncthreads();
@@ -551,15 +560,18 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   for (int p = tid; p < n; p += D) {
     const float e = ex2(s_m[p] - M);
     s_e[p] = e;
-    L = fmaf(part[p * step + D + 1], e, L);
+    L = fmaf(s_l[p], e, L);
   }
   L = warp_sum(L);
   if (lane == 0) s_red[1][tid >> 5] = L;
   __syncthreads();
   L = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
   float O = 0.0f;
+#pragma unroll
+  for (int p = 0; p < AHEAD; ++p)
+    if (p < n) O = fmaf(x[p], s_e[p], O);
 #pragma unroll 8
-  for (int p = 0; p < n; ++p) O = fmaf(part[p * step + tid], s_e[p], O);
+  for (int p = AHEAD; p < n; ++p) O = fmaf(part[p * step + tid], s_e[p], O);
   const int tt = div_small(r, a.inv_g), hq = h * a.G + r - tt * a.G;
   from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
