@@ -23,8 +23,8 @@
 //
 // A row's parts in different CTAs (kv8_line.cuh) are joined by a second kernel in a fixed order.
 //
-// Measured (8 KV heads, G = 4, bf16): one token over 128k 43.8 us, 6.1 TB/s or 0.94 of the copy rate; 8 sequences of 80k,
-// 4 KV heads, G = 7: 101 us, 6.6 TB/s; over 700 tokens 6.9 us, a chain of latencies.  With one softmax warpgroup the
+// Measured (8 KV heads, G = 4, bf16): one token over 128k 43.6 us, 6.2 TB/s or 0.94 of the copy rate; 8 sequences of 80k,
+// 4 KV heads, G = 7: 99 us, 6.8 TB/s; over 700 tokens 6.3 us, a chain of latencies.  With one softmax warpgroup the
 // softmax was the bound: 58 us and 150 us.
 #include "kv8_line.cuh"
 
@@ -595,7 +595,7 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   if (R <= 4) return launch<T, 4, QT, false>(map, a, ctas, st);
   if (R <= 8) return launch<T, 8, QT, false>(map, a, ctas, st);
   if (R <= 16) return launch<T, 16, QT, false>(map, a, ctas, st);
-  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);      // 20 rows over 16k: 22 us, with 16 per thread 25
+  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);      // 20 rows over 16k: 19.2 us, with 16 per thread ~22
   return launch<T, 16, QT, true>(map, a, ctas, st);
 }
 
