@@ -97,14 +97,21 @@ __device__ __forceinline__ uint32_t next_term(float2& y) {
   return code;
 }
 
-// 4 consecutive elements of q.
-__device__ __forceinline__ void load4(const void* p, int dtype, int64_t i, float (&x)[4]) {
+// 4 consecutive elements of q, as they are and as fp32.  (A branch around the load would wait for it.)
+__device__ __forceinline__ uint4 load4(const void* p, bool f32) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %5, 0; @p ld.global.v4.u32 {%0, %1, %2, %3}, [%4]; @!p ld.global.v2.u32 {%0, %1}, [%4]; }\n"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(p), "r"((uint32_t)f32)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ void unpack4(uint4 v, int dtype, float (&x)[4]) {
   if (dtype == FATHOM_DTYPE_F32) {
-    const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
     return;
   }
-  const uint2 v = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
   const uint32_t w[2] = {v.x, v.y};
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -134,6 +141,8 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
                                                        // of this one's leave it no room for whole ones, 39 us for 26)
   const int64_t bhg = blockIdx.x;
   const int bh = (int)bhg / a.G, gw = (int)crank * PW + warp;
+  const uint4 qv = load4(reinterpret_cast<const char*>(q) + (bhg * D + 4 * lane) * (dtype == FATHOM_DTYPE_F32 ? 4 : 2),
+                         dtype == FATHOM_DTYPE_F32);
   int64_t end = a.end_dev ? a.end_dev[bh / a.Hkv] : a.end;
   if (end > a.cap) end = a.cap;
   const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)bh * (a.cap / BLK);
@@ -187,7 +196,7 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   // q as terms: one warp, a lane 4 dims; then term g of this lane's dims, 16 j .. and 64 + 16 j ..
   if (warp == 0) {
     float x[4];
-    load4(q, dtype, bhg * D + 4 * lane, x);
+    unpack4(qv, dtype, x);
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
