@@ -107,6 +107,19 @@ __device__ __forceinline__ uint4 load4(const void* p, bool f32) {
       : "memory");
   return v;
 }
+// An entry of a list, if `there`.
+__device__ __forceinline__ void load_entry(int64_t& x, const int64_t* p, bool there) {
+  asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; @p ld.global.b64 %0, [%1]; }\n"
+               : "+l"(x)
+               : "l"(p), "r"((uint32_t)there)
+               : "memory");
+}
+__device__ __forceinline__ void load_entry(int& x, const int32_t* p, bool there) {
+  asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; @p ld.global.b32 %0, [%1]; }\n"
+               : "+r"(x)
+               : "l"(p), "r"((uint32_t)there)
+               : "memory");
+}
 __device__ __forceinline__ void unpack4(uint4 v, int dtype, float (&x)[4]) {
   if (dtype == FATHOM_DTYPE_F32) {
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
@@ -156,11 +169,10 @@ __global__ void __launch_bounds__(MAX_PW * 32, WARPS_PER_SM / MAX_PW)
   int listed_row = -1;
   auto listed = [&]() {
     listed_tok = -1;
-    if (next < k) {
-      listed_tok = a.idx[bhg * k + next];
-      if (a.slot) listed_row = a.slot[bhg * k + next];
-      next += NW * CHUNK;
-    }
+    const bool more = next < k;
+    load_entry(listed_tok, a.idx + bhg * k + next, more);
+    load_entry(listed_row, a.slot ? a.slot + bhg * k + next : nullptr, more && a.slot);
+    next += more ? NW * CHUNK : 0;
   };
   auto pick = [&](int& tok, int& row) {
     const bool there = listed_tok >= 0 && listed_tok < end;

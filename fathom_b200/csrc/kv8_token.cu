@@ -277,7 +277,9 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
       const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
       auto scale_of = [&](int tile) {
         const int tok = tile * TILE + t;
-        return tok < w.end ? sc[tok / BLK] : make_float2(0.0f, 1.0f);
+        uint2 x = make_uint2(0u, 0x3F800000u);    // 0 and 1
+        load8(x, sc + tok / BLK, tok < w.end);
+        return make_float2(__uint_as_float(x.x), __uint_as_float(x.y));
       };
       constexpr uint32_t STEP = SPLIT ? 1 : 2;
       const uint32_t mine = SPLIT ? i0 : i0 + ((i0 ^ g) & 1);      // this warpgroup's first tile of the row
