@@ -19,7 +19,7 @@
 // rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24.
 // ~5 us of it begin and join; the rest is 32 picks per 340 cycles and SM, 6 TB/s.  12 warps per SM, or 3 stages, are
 // slower (29 us), so are TMA gathers of 4 rows (28; for the keys alone 28.5), bulk copies of one (34) and rows loaded into
-// registers (29).  580 picks for 32 heads: 5.3 us in a graph.
+// registers (29).  580 picks for 32 heads: 5.1 us in a graph.
 #include "dedupe.cuh"
 #include "kv8_attn.cuh"
 
