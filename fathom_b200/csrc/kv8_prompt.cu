@@ -221,8 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         vt += w.j1 - w.j0;
         continue;
       }
-      ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
-      const int ev = s_ev[vt % VSTAGES];           // log2 of the sequence's largest value scale: comes with the first values
+      int ev = 0;                                  // log2 of the sequence's largest value scale: comes with the first values
       float m = -INFINITY, l = 0.0f;               // m is the same in both threads of a row, l is this thread's share
       for (int j = w.j0; j < w.j1; ++j, ++vt) {
         const int blk = j * (TILE / BLK) + ch;
@@ -233,6 +232,13 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         ++phase;
         __syncwarp();
         tc::fence_after();
+        if (j == w.j0) {
+          // Only now: S follows the products of every tile before, so v_full is at this tile's phase or the one before it,
+          // which its parity tells apart.  Earlier it could be further behind, where this half had no rows in the pieces before.
+          ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
+          __syncwarp();
+          ev = s_ev[vt % VSTAGES];
+        }
         const int evb = weight_ev(s2.y, ev);
         const float es = (float)evb;
         int see = BLK;                             // tokens of the block that this row sees

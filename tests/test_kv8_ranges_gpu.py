@@ -1,0 +1,64 @@
+"""8-bit key/value cache: attention where the ranges of values, weights and scores are wide, against the formula in 64 bits.
+
+Tolerances as in test_kv8_gpu.py: an output's own rounding, and 2^-10 of sum(weight * |V|) for weights of 11 bits."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8_oracle as O
+from tests.test_kv8_gpu import DT, ROUND
+
+pytestmark = pytest.mark.gpu
+
+
+def _exact(q, c, ends):
+    """(out, sum of weight * |V|) of q [B, Hq, T, 128] over the cache c, in 64 bits on the GPU."""
+    B, Hq, T, _ = q.shape
+    K, V = (torch.from_numpy(np.nan_to_num(x)).cuda() for x in O.values(c.rows.cpu().numpy(), c.scales.cpu().numpy()))
+    out, mag = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    at = torch.arange(c.cap, device="cuda")
+    G = Hq // c.Hkv
+    for b, end in enumerate(ends):
+        sees = min(max(int(end), 0), c.cap) - (T - 1 - torch.arange(T, device="cuda"))
+        for h in range(c.Hkv):
+            bh, heads = b * c.Hkv + h, slice(h * G, (h + 1) * G)
+            s = (q[b, heads].double() @ K[bh].T) / 128 ** 0.5
+            s.masked_fill_(at[None] >= sees[:, None], -np.inf)
+            w = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+            out[b, heads], mag[b, heads] = w @ V[bh], w @ V[bh].abs()
+    return out, mag
+
+
+def _close(got, ref, mag, weights=2.0 ** -10):
+    tol = ROUND[got.dtype] * ref.abs() + weights * mag + 1e-37
+    off = (got.double() - ref).abs() / tol
+    assert not (off > 1).any() and not off.isnan().any(), float(off.nan_to_num(np.inf).max())
+
+
+def _cache(K, V, cap=None):
+    from fathom_b200.kv8 import KVCache8
+    B, H, n, _ = K.shape
+    c = KVCache8(B, H, cap or n)
+    c.write(K, V, 0)
+    return c
+
+
+def _normal(*shape, seed, dtype=torch.float32):
+    return torch.randn(*shape, device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("G,T", [(4, 65), (4, 70), (4, 80), (4, 129), (1, 300)])
+def test_short_last_items_between_heads_of_other_scales(G, T, ragged):
+    """Query rows of a KV head that leave at most 128 for its last 256, and values 2^-20, 2^20, .. by head and sequence:
+    no head's rows meet another's scale."""
+    B, H, n = 2, 4, 3000
+    K, V = _normal(B, H, n, 128, seed=T), _normal(B, H, n, 128, seed=T + 1)
+    V *= torch.exp2(20.0 * (2 * (torch.arange(B * H, device="cuda") % 2) - 1)).view(B, H, 1, 1)
+    c = _cache(K, V)
+    q = _normal(B, H * G, T, 128, seed=G, dtype=torch.bfloat16)
+    ends = [n, 1777] if ragged else [n, n]
+    ref, mag = _exact(q, c, ends)
+    for _ in range(5):
+        out = c.attend(q, torch.tensor(ends, device="cuda") if ragged else n)
+        _close(out, ref, mag)
