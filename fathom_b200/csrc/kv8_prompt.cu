@@ -15,9 +15,9 @@
 // constant of each 64-token block, enters the weight's exponent, so a row sees its own range whatever other blocks
 // hold.  Softmax, two threads per row, one for each block of a tile: m, the reference of s + ev, follows the row's
 // maximum only when that exceeds it by 2^12 (then O is rescaled; at 2^7 that cost 3%); weights are 2^(s + ev - m + 3), at
-// most 2^15 in f16, rounded to 11 bits; sums in fp32, the denominator taking each block's sum times 2^(largest
-// ev - ev).  Blocks whose scale is below 2^-40 of the sequence's largest count as 2^-40 there and have the rest
-// multiplied into their f16 values, which keeps the denominator in range.  (One thread per row, 8 softmax warps instead
+// most 2^15 in f16, rounded to 11 bits down to 2^-17 of the reference and to steps of 2^-27 of it below; sums in fp32.  The
+// denominator has a reference of its own, without the value scales: each block's sum of weights enters it once.  Parts
+// and outputs are weighted means, whatever the values' range is.  (One thread per row, 8 softmax warps instead
 // of 16: 1.34 ms against 0.95 for the chunk below, the steps of a tile waiting for each other; exponentials partly by
 // polynomial: slower, the warps' issue is as near its limit as the special-function units.)
 //
@@ -45,24 +45,16 @@ static_assert(4 * REG_SOFT + REG_VALUE + REG_OTHER <= 6 * REG_LAUNCH, "register 
 constexpr int PIECE = 4;                     // tiles (~1.7 us each) that beginning and ending a piece takes
 constexpr int LEAST = 4;                     // so shares are no shorter
 constexpr int WHOLE = 6;                     // tiles that take no longer than their halves and the second kernel
-constexpr int EV_SPAN = 40;                  // value scales in the weights' exponents span at most 2^40
+constexpr float FAR = 60.0f;                 // below 2^-60 of the reference no weight of a block is above f16's least
 
 template <int QT> struct Shape {
   static constexpr int Q = 0, K = 2 * QT * HALF * D, V = K + KSTAGES * KBYTES, END = V + VSTAGES * VBYTES;
   static constexpr int SMEM = END + 1024;
 };
 
-// One warp: log2 of the largest value scale among the first `end` tokens' blocks.
-__device__ int largest_ev(const float2* sc, int64_t end) {
-  int ev = KV8_EMIN;
-#pragma unroll 8
-  for (int64_t b = threadIdx.x & 31; b < (end + BLK - 1) / BLK; b += 32)
-    ev = max(ev, (int)(__float_as_uint(sc[b].y) >> 23) - 127);
-  return __reduce_max_sync(0xffffffffu, ev);
-}
-// log2 of a block's value scale as the weights take it.
-__device__ __forceinline__ int weight_ev(float scale, int largest) {
-  return min(largest, max(largest - EV_SPAN, (int)(__float_as_uint(scale) >> 23) - 127));
+// log2 of a power of two, as a number (no conversion instruction: those share the special-function units).
+__device__ __forceinline__ float log2_of(float scale) {
+  return __uint_as_float(0x4B000000u | __float_as_uint(scale) >> 23) - (8388608.0f + 127.0f);
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -94,9 +86,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
   __shared__ uint32_t s_tmem;
   __shared__ int s_gave_up;
   __shared__ __align__(4) uint8_t s_nan[VSTAGES][TILE];   // tokens whose value holds a NaN (tiles whose mask differs by row)
-  __shared__ int s_ev[VSTAGES];                    // log2 of the largest value scale of the stage's sequence
   __shared__ float s_rs[2][HALF];                  // scale of a row's scores: 2^e log2(e) / sqrt(128)
-  __shared__ float s_pair[2 * SOFT];               // by thread: what a row's two threads (tid, tid ^ HALF) tell each other
+  __shared__ float2 s_pair[2 * SOFT];              // by thread: what a row's two threads (tid, tid ^ HALF) tell each other
   const uint32_t bar = tc::smem_u32(bars);
   auto k_full = [&](uint32_t i) { return bar + 8 * (i % KSTAGES); };
   auto k_free = [&](uint32_t i) { return bar + 8 * (KSTAGES + i % KSTAGES); };
@@ -221,8 +212,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         vt += w.j1 - w.j0;
         continue;
       }
-      int ev = 0;                                  // log2 of the sequence's largest value scale: comes with the first values
-      float m = -INFINITY, l = 0.0f;               // m is the same in both threads of a row, l is this thread's share
+      // m is the same in both threads of a row; l is this thread's share of the denominator, lm its reference
+      float m = -INFINITY, lm = -1e30f, l = 0.0f;
       for (int j = w.j0; j < w.j1; ++j, ++vt) {
         const int blk = j * (TILE / BLK) + ch;
         const float2 s2 = blk < a.cap / BLK ? sc[blk] : make_float2(0.0f, 0.0f);
@@ -232,19 +223,13 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         ++phase;
         __syncwarp();
         tc::fence_after();
-        if (j == w.j0) {
-          // Only now: S follows the products of every tile before, so v_full is at this tile's phase or the one before it,
-          // which its parity tells apart.  Earlier it could be further behind, where this half had no rows in the pieces before.
-          ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
-          __syncwarp();
-          ev = s_ev[vt % VSTAGES];
-        }
-        const int evb = weight_ev(s2.y, ev);
-        const float es = (float)evb;
+        const float es = log2_of(s2.y);
         int see = BLK;                             // tokens of the block that this row sees
         const bool masked = (j + 1) * TILE > all_see;
         if (masked) {
           see = min(max(limit - blk * BLK, 0), BLK);
+          // (this late the barrier is at this tile's phase or the one before, which its parity tells apart, also where this half
+          // had no rows in the pieces before: S follows every earlier tile's products)
           ok = ok && tc::mbar_wait(v_full(vt), (vt / VSTAGES) & 1, gave_up);
           for (int i = 0; i < BLK; i += 4)
             if (const uint32_t f = *reinterpret_cast<const uint32_t*>(&s_nan[vt % VSTAGES][ch * BLK + i]))
@@ -268,16 +253,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
             t1 = max3(t1, __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
           }
         }
-        float top = fmaf(fmaxf(t0, t1), cs, es);
+        const float smax = fmaxf(t0, t1) * cs, top = smax + es;
         if (tc::named_or(pair_bar, 64, top > m + SLACK)) {        // also the first time: m = -inf
-          s_pair[tid] = top;
+          s_pair[tid].x = top;
           tc::named_sync(pair_bar, 64);
-          top = fmaxf(top, s_pair[tid ^ HALF]);
+          const float both = fmaxf(top, s_pair[tid ^ HALF].x);
           tc::named_sync(pair_bar, 64);
-          const bool up = top > m + SLACK;
-          const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-          if (up) m = top;
-          l *= f;
+          const bool up = both > m + SLACK;
+          const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - both);
+          if (up) m = both;
           __syncwarp();
           if (j > w.j0) {                          // O of the tiles before is complete: their products precede this S
 #pragma unroll 1
@@ -291,7 +275,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
             }
           }
         }
-        const float off = m == -INFINITY ? 0.0f : HEAD - m + es;
+        // A block that is far below the reference weighs nothing in f16 but may still count in the denominator: its sum is
+        // taken from its own largest.
+        const bool far = top < m - FAR;
+        const float off = smax == -INFINITY ? 0.0f : far ? HEAD - smax : HEAD - m + es;
         const float2 cc = make_float2(cs, cs), oo = make_float2(off, off);
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         // weights over the scores they came from: columns 32 u .. 32 u + 15 of the block's 64
@@ -315,9 +302,19 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
             sum[i & 1] = __fadd2_rn(sum[i & 1], w2);
             p[i] = pack_h2(w2.x, w2.y);
           }
+          if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = far ? 0u : p[i];
+          }
           tc::Tmem<16>::st(tm_s + 32 * u, p);
         }
-        l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), pow2i(ev - evb), l);
+        {
+          // this block's sum is relative to -off, without the value scale
+          const float part = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), ref = smax == -INFINITY ? -1e30f : -off;
+          const float d = ref - lm, f = ex2(-fabsf(d));
+          l = d > 0.0f ? fmaf(l, f, part) : fmaf(part, f, l);
+          lm = fmaxf(lm, ref);
+        }
         tc::wait_st();
         tc::fence_before();
         __syncwarp();
@@ -326,13 +323,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       ok = ok && tc::mbar_wait(s_full(h2), phase & 1, gave_up);      // the piece's last product
       ++phase;
       __syncwarp();
-      s_pair[tid] = l;
+      s_pair[tid] = make_float2(l, lm);
       tc::named_sync(pair_bar, 64);
-      l += s_pair[tid ^ HALF];
+      const float2 other = s_pair[tid ^ HALF];
+      const float ref = fmaxf(lm, other.y);
+      l = ch == 0 ? fmaf(l, ex2(lm - ref), other.x * ex2(other.y - ref)) : fmaf(other.x, ex2(other.y - ref), l * ex2(lm - ref));
       tc::fence_after();
       const bool whole = w.j0 == 0 && w.j1 == w.n;
-      const float vscale = pow2i(ev);              // the denominator is relative to the largest scale
-      const float f = !ok ? __uint_as_float(0x7FFFFFFFu) : whole ? (l == 0.0f ? 0.0f : vscale / l) : vscale;
+      // O is relative to m - HEAD; the difference of the references is a block's value exponent at most
+      const float f = !ok ? __uint_as_float(0x7FFFFFFFu) : l == 0.0f ? 0.0f : ex2(m - HEAD - ref) / l;
       T* op = reinterpret_cast<T*>(a.out) + w.b * a.ob + hq * a.oh + tt * a.ot + 64 * ch;
       float* part = a.part + ((2 * (int64_t)blockIdx.x + (w.j0 == 0 ? 1 : 0)) * ROWS + h2 * HALF + r) * PART;
 #pragma unroll 1
@@ -358,7 +357,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
                             __uint_as_float(o[4 * c + 2]) * f, __uint_as_float(o[4 * c + 3]) * f);
         }
       }
-      if (real && !whole && ch == 0) part[D] = m, part[D + 1] = l;
+      if (real && !whole && ch == 0) part[D] = ref, part[D + 1] = l;
       __syncwarp();
       tc::fence_before();
     }
@@ -371,8 +370,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
     bool ok = true;
     while (ok && w.next()) {
       const uint8_t* base = a.rows + (int64_t)w.bh * a.cap * KV8_ROW + D + u * 16;
-      const float2* sc = reinterpret_cast<const float2*>(a.scales) + (int64_t)w.bh * (a.cap / BLK);
-      const int ev = largest_ev(sc, w.end);
       const int all_see = seen(a, w.end, w.it * ROWS);
       for (int j = w.j0; j < w.j1; ++j, ++i) {
         uint4 v[8];
@@ -381,17 +378,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
           const int tok = j * TILE + p * 16 + row0;
           v[p] = tok < w.end ? *reinterpret_cast<const uint4*>(base + (int64_t)tok * KV8_ROW) : make_uint4(0, 0, 0, 0);
         }
-        int rest[2];                               // log2 of what the weights leave of the block's scale
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int blk = j * 2 + e;
-          const float s = blk * BLK < w.end ? sc[blk].y : 1.0f;
-          rest[e] = blk * BLK < w.end ? (int)(__float_as_uint(s) >> 23) - 127 - weight_ev(s, ev) : 0;
-        }
         ok = ok && tc::mbar_wait(v_free(i), ((i / VSTAGES) & 1) ^ 1, gave_up);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (t == 0) s_ev[i % VSTAGES] = ev;
         uint8_t* vb = smem + S::V + (i % VSTAGES) * VBYTES + (u >> 2) * (TILE * 128);
         const bool differs = (j + 1) * TILE > all_see;
 #pragma unroll
@@ -416,14 +405,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
           for (int e = 0; e < 8; ++e) {
             const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x[e >> 1] >> (16 * (e & 1))), __NV_E4M3);
             y[e] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          if (rest[p >> 2] != 0) {
-            const __half2 k = __float2half2_rn(rest[p >> 2] < -40 ? 0.0f : pow2i(rest[p >> 2]));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y[e]), k);
-              y[e] = *reinterpret_cast<const uint32_t*>(&z);
-            }
           }
           uint8_t* dst = vb + tk * 128;
           const int c = (u & 3) * 2;
@@ -556,17 +537,17 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args
     if (row >= total) return;
     // parts: share c0 holds the item's first tiles (its second slot), the others begin with it (first slot)
     auto part = [&](int c) { return a.part + ((2 * (int64_t)c + (c == c0 ? 1 : 0)) * ROWS + r) * PART; };
-    // lane = part, 32 at a time, with a running reference
+    // lane = part, 32 at a time: the denominator, then each part's share of it (parts are weighted means)
     float M = -INFINITY, L = 0.0f;
+    for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, part(c)[D]);
+    M = warp_max(M);
+    for (int c = c0 + lane; c <= c1; c += 32) L = fmaf(part(c)[D + 1], ex2(part(c)[D] - M), L);
+    L = warp_sum(L);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int c = c0; c <= c1; c += 32) {
       const int n = min(32, c1 - c + 1);
-      const float2 ml = lane < n ? *reinterpret_cast<const float2*>(part(c + lane) + D) : make_float2(-INFINITY, 0.0f);
-      const float top = fmaxf(M, warp_max(ml.x)), f = M == -INFINITY ? 0.0f : ex2(M - top);
-      const float e = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-      M = top;
-      L = fmaf(L, f, ml.y * e);
-      O = make_float4(O.x * f, O.y * f, O.z * f, O.w * f);
+      const float e = lane < n ? part(c + lane)[D + 1] * ex2(part(c + lane)[D] - M) * inv : 0.0f;
 #pragma unroll 8
       for (int v = 0; v < n; ++v) {
         const float4 o = *reinterpret_cast<const float4*>(part(c + v) + 4 * lane);
@@ -574,10 +555,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) prompt_join_kernel(const Args
         O.x = fmaf(o.x, ev, O.x), O.y = fmaf(o.y, ev, O.y), O.z = fmaf(o.z, ev, O.z), O.w = fmaf(o.w, ev, O.w);
       }
     }
-    L = warp_sum(L);
-    const float f = L == 0.0f ? 0.0f : 1.0f / L;
     T y[4];
-    from_f32(O.x * f, &y[0]), from_f32(O.y * f, &y[1]), from_f32(O.z * f, &y[2]), from_f32(O.w * f, &y[3]);
+    from_f32(O.x, &y[0]), from_f32(O.y, &y[1]), from_f32(O.z, &y[2]), from_f32(O.w, &y[3]);
     const int tt = row / a.G, hq = (bh % a.Hkv) * a.G + row - tt * a.G;
     T* op = reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + 4 * lane;
     *reinterpret_cast<uint2*>(op) = *reinterpret_cast<const uint2*>(y);

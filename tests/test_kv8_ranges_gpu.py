@@ -62,3 +62,50 @@ def test_short_last_items_between_heads_of_other_scales(G, T, ragged):
     for _ in range(5):
         out = c.attend(q, torch.tensor(ends, device="cuda") if ragged else n)
         _close(out, ref, mag)
+
+
+def _blocks(n, exponents):
+    """2^exponent of each token's 64-token block, [n, 1]."""
+    e = torch.tensor(exponents, device="cuda", dtype=torch.float32).repeat_interleave(64)[:n]
+    return torch.exp2(e)[:, None]
+
+
+@pytest.mark.parametrize("low,high", [(-70, 0), (-60, 60), (0, 60), (-110, 110)])
+@pytest.mark.parametrize("G,T", [(1, 128), (1, 20), (4, 70), (2, 1)])
+def test_rows_that_see_only_small_values(G, T, low, high):
+    """Values near 2^low in the first tokens and near 2^high from the 64th on: queries of both keep their own range,
+    whichever the number of query rows."""
+    n = 128
+    K, V = _normal(1, 2, n, 128, seed=T), _normal(1, 2, n, 128, seed=T + 1)
+    c = _cache(K, V * _blocks(n, [low, high]))
+    q = _normal(1, 2 * G, T, 128, seed=G, dtype=torch.bfloat16)
+    for end in (n, 90, 64, 70):
+        ref, mag = _exact(q, c, [end])
+        _close(c.attend(q, end), ref, mag)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("G,T", [(4, 70), (1, 300), (8, 16), (4, 1), (4, 6)])
+def test_values_of_blocks_of_any_scale(G, T, ragged):
+    """Values 2^-60 .. 2^60 by block in no order, over contexts that several CTAs share; scores of some tens, so that the
+    largest weights and the largest values lie apart."""
+    B, H, n = 2, 2, 2500
+    K, V = _normal(B, H, n, 128, seed=T), _normal(B, H, n, 128, seed=T + 1)
+    e = torch.randint(-60, 61, (-(-n // 64),), generator=torch.Generator().manual_seed(G + T)).tolist()
+    c = _cache(K, V * _blocks(n, e))
+    q = _normal(B, H * G, T, 128, seed=G, dtype=torch.bfloat16) * 4
+    ends = [n, 1300] if ragged else [n, n]
+    ref, mag = _exact(q, c, ends)
+    _close(c.attend(q, torch.tensor(ends, device="cuda") if ragged else n), ref, mag)
+
+
+@pytest.mark.parametrize("e", [-100, 118])
+@pytest.mark.parametrize("G,T", [(4, 80), (1, 40)])
+def test_split_rows_of_the_largest_and_smallest_values(G, T, e):
+    """Rows that several CTAs share, with values near the ends of fp32's range: no part leaves it."""
+    n = 20011
+    K, V = _normal(1, 1, n, 128, seed=1), _normal(1, 1, n, 128, seed=2)
+    c = _cache(K, V * 2.0 ** e)
+    q = _normal(1, G, T, 128, seed=3, dtype=torch.bfloat16) * 0.1
+    ref, mag = _exact(q, c, [n])
+    _close(c.attend(q, n), ref, mag)
