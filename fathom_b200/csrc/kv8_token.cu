@@ -8,13 +8,16 @@
 //
 // The other operand of an e4m3 product has to be e4m3 too.  A row of q is split into terms q = s (t1 + t2 / 16 +
 // t3 / 256), each the rounding of what the ones before left (4 significant bits a term: 2 terms hold a
-// bf16 exactly, 3 an fp16), and so is a row of the weights; the terms are further columns of the product,
-// which the tensor cores have to spare: with M = 128 tokens a tile of 32 KB takes them ~250 cycles, its
+// bf16 exactly, 3 an fp16, down to 2^-21 and 2^-25 of the row's largest), and a row of the weights into five: three hold
+// the 11 bits of the largest, two more continue to steps of 2^-28 of the reference, because the tail of a long context weighs
+// that little a token beside one dominant key and a tenth of everything together (with three terms it was lost from O
+// and kept in the denominator; five cost a draft of 20 rows 6%, other calls 0 to 4%).  The terms are further columns
+// of the product, which the tensor cores have to spare: with M = 128 tokens a tile of 32 KB takes them up to ~450 cycles, its
 // bytes ~1400.  A score is then the sum of its term columns times the block's key scale; weights carry the
 // block's value scale (a power of two) in their exponent, so no value is ever rescaled.
 //
 // Softmax, thread = token: with m the running reference of a row's (score + log2 of the value scale), a weight is
-// 2^(s + log2 vs - m); m moves only when a tile exceeds it by 2^6 (then O^T in tensor memory is rescaled), which
+// 2^(s + log2 vs - m); m moves only when a tile exceeds it by 2^5 (then O^T in tensor memory is rescaled), which
 // leaves e4m3's range room on both sides.  The denominator is kept per thread in fp32 with a reference of its
 // own, because the value scale must not enter it.  One tile's chain of steps is longer than its bytes take, so there are
 // two softmax warpgroups: up to 16 rows they take the even and the odd tiles, each with its own references and its own
@@ -32,12 +35,13 @@ namespace fathom {
 namespace kv8 {
 namespace {
 
-constexpr int TERMS = 3;                         // e4m3 terms of a weight
+constexpr int TERMS = 5;                         // e4m3 terms of a weight: 2^8 down to steps of 2^-25
+constexpr int F16_UP = 7;                        // weights come to f16 times 2^7: up to 2^15, 11 bits down to 2^-21
 constexpr int GROUP = 128;                       // threads of a softmax warpgroup
 constexpr int THREADS = 2 * GROUP + 64;          // warps 0-3, 4-7: softmax; 8: loads; 9: products
 constexpr int STAGE_BYTES = 2 * TILE * D;        // key tile, value tile
-constexpr float SLACK = 6.0f;                    // a tile may exceed the reference by 2^6
-constexpr float HEAD = 2.0f;                     // weights at the reference are 4: 2^(HEAD + SLACK) = 256 <= 448
+constexpr float SLACK = 5.0f;                    // a tile may exceed the reference by 2^5
+constexpr float HEAD = 3.0f;                     // weights at the reference are 8: 2^(HEAD + SLACK) = 256 <= 448
 constexpr int PIECE = 6;                         // tiles (~0.4 us each) that beginning and ending a piece takes: ~2.5 us
 constexpr int SHORT = 8;                         // tiles that take less than the second kernel (~4 us)
 constexpr int MAX_CTAS = 512;                    // shares that the join kernel has room for
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             tc::wait_st();
           }
         }
-        // weights as terms into the operand buffer: 11 bits in f16, whose remainders after e4m3 are exact
+        // weights as terms into the operand buffer, by way of f16: 11 bits, whose remainders after e4m3 are exact
         uint32_t codes[TERMS * NC / 4] = {};
 #pragma unroll
         for (int r = 0; r < NR; r += 2) {
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float sv = s[r + e], mv = m[r + e];
-            x[e] = mv == -INFINITY && !(sv != sv) ? 0.0f : ex2(sv + (lv - mv + HEAD));
+            x[e] = mv == -INFINITY && !(sv != sv) ? 0.0f : ex2(sv + (lv - mv + (HEAD + F16_UP)));
             const float d = sv - lm[r + e], p = ex2(-fabsf(d));
             l[r + e] = d > 0.0f ? fmaf(l[r + e], p, 1.0f) : l[r + e] + p;
             lm[r + e] = fmaxf(lm[r + e], sv);
@@ -397,13 +401,14 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
           __half2 y = __floats2half2_rn(x[0], x[1]);
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) {
-            const __half2_raw yr = *reinterpret_cast<const __half2_raw*>(&y);
-            const uint32_t code = __nv_cvt_halfraw2_to_fp8x2(yr, __NV_SATFINITE, __NV_E4M3);
+            const float unit = (float)(1 << F16_UP) / (float)(1 << 4 * term);       // of this term in y
+            const __half2 z = __hmul2(y, __float2half2_rn(1.0f / unit));
+            const uint32_t code =
+                __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&z), __NV_SATFINITE, __NV_E4M3);
             uint32_t& word = codes[(term * NC + r) / 4];
             word = (r & 2) ? word | code << 16 : code;
             const __half2_raw c = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code, __NV_E4M3);
-            const __half2 sixteen = __float2half2_rn(16.0f);
-            y = __hmul2(__hsub2(y, *reinterpret_cast<const __half2*>(&c)), sixteen);
+            y = __hfma2(*reinterpret_cast<const __half2*>(&c), __float2half2_rn(-unit), y);
           }
         }
         // columns as q's; with NC = 16 a term's rows are a 16-byte piece of their own

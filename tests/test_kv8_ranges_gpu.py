@@ -109,3 +109,41 @@ def test_split_rows_of_the_largest_and_smallest_values(G, T, e):
     q = _normal(1, G, T, 128, seed=3, dtype=torch.bfloat16) * 0.1
     ref, mag = _exact(q, c, [n])
     _close(c.attend(q, n), ref, mag)
+
+
+def _steps(c, q, end):
+    """What weights in steps of 2^-27 of a row's largest weight times value scale can be off by, [B, Hq, T, 1]: half a step
+    of a code of at most 448 for every token (the reference may be half the largest)."""
+    B, Hq, T, _ = q.shape
+    scales = c.scales.double()[:, :, 1].repeat_interleave(64, 1)
+    K = torch.from_numpy(np.nan_to_num(O.values(c.rows.cpu().numpy(), c.scales.cpu().numpy())[0])).cuda()
+    out = torch.empty(B, Hq, T, 1, dtype=torch.float64, device="cuda")
+    for b in range(B):
+        for h in range(Hq):
+            bh = b * c.Hkv + h // (Hq // c.Hkv)
+            w = torch.softmax((q[b, h].double() @ K[bh, :end].T) / 128 ** 0.5, -1)
+            out[b, h] = end * 2.0 ** -27 * 448 * (w * scales[bh, :end]).amax(-1, keepdim=True)
+    return out
+
+
+@pytest.mark.parametrize("heads", [1, 148])             # a row in many CTAs, or whole in one
+@pytest.mark.parametrize("G,T", [(4, 1), (8, 1), (16, 1), (4, 5), (32, 1), (4, 20)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_a_long_tail_beside_one_dominant_key(heads, G, T, dtype):
+    """One key 13, 14 and 16 nats above 20k equal ones, whose values have a common mean: the tail's weights, 2^-18 .. 2^-23
+    of the largest, count in numerator and denominator alike."""
+    n = 20480
+    for extra in (9.0, 10.0, 11.0):                      # numbers of the cache's type: the scores are what is said here
+        K = torch.zeros(1, 1, n, 128, device="cuda")
+        K[..., :64] = 1.0
+        K[0, 0, 5, 64:] = extra
+        V = 1 + 0.25 * _normal(1, 1, n, 128, seed=1)
+        V[0, 0, 5] *= 0.25
+        one = _cache(K, V)
+        q = torch.full((1, G, T, 128), 0.25, device="cuda", dtype=DT[dtype])
+        ref, mag = _exact(q, one, [n])
+        tol = 2.0 ** -10 * mag + _steps(one, q, n)
+        c = one if heads == 1 else _cache(K.expand(heads, 1, n, 128), V.expand(heads, 1, n, 128))
+        out = c.attend(q.expand(heads, G, T, 128), n)
+        for b in {0, heads // 2, heads - 1}:
+            _close(out[b:b + 1], ref, tol, 1.0)
