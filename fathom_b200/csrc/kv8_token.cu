@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
         s_ref[tid] = mx;
         const int tt = late ? div_small(tid, a.inv_g) : 0;
         s_out[tid] = now.b * a.ob + (int64_t)(h * a.G + tid - tt * a.G) * a.oh + tt * a.ot;
-        const float scale = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;       // of parts too: a mean stays in range where a sum may not
         // O^T is relative to m - HEAD: both come to the denominator's reference.  A warpgroup that had no tile left its
         // columns as they were.
 #pragma unroll
@@ -565,22 +565,23 @@ __global__ void __launch_bounds__(D) token_join_kernel(const Args a, int ctas) {
   M = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
   float L = 0.0f;
   for (int p = tid; p < n; p += D) {
-    const float e = ex2(s_m[p] - M);
+    const float e = s_l[p] * ex2(s_m[p] - M);
     s_e[p] = e;
-    L = fmaf(s_l[p], e, L);
+    L += e;
   }
   L = warp_sum(L);
   if (lane == 0) s_red[1][tid >> 5] = L;
   __syncthreads();
   L = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-  float O = 0.0f;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  float O = 0.0f;                                 // parts are weighted means: each counts by its share of the denominator
 #pragma unroll
   for (int p = 0; p < AHEAD; ++p)
-    if (p < n) O = fmaf(x[p], s_e[p], O);
+    if (p < n) O = fmaf(x[p], s_e[p] * inv, O);
 #pragma unroll 8
-  for (int p = AHEAD; p < n; ++p) O = fmaf(part[p * step + tid], s_e[p], O);
+  for (int p = AHEAD; p < n; ++p) O = fmaf(part[p * step + tid], s_e[p] * inv, O);
   const int tt = div_small(r, a.inv_g), hq = h * a.G + r - tt * a.G;
-  from_f32(L == 0.0f ? 0.0f : O / L, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
+  from_f32(O, reinterpret_cast<T*>(a.out) + b * a.ob + hq * a.oh + tt * a.ot + tid);
 }
 
 template <typename T, int NR, int QT, bool SPLIT>

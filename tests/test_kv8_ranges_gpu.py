@@ -147,3 +147,17 @@ def test_a_long_tail_beside_one_dominant_key(heads, G, T, dtype):
         out = c.attend(q.expand(heads, G, T, 128), n)
         for b in {0, heads // 2, heads - 1}:
             _close(out[b:b + 1], ref, tol, 1.0)
+
+
+@pytest.mark.parametrize("G,T", [(4, 1), (16, 1), (4, 6), (4, 20)])
+def test_split_rows_of_large_values_of_one_sign(G, T):
+    """Shares of ~70 tiles whose weighted sums, unlike their means, are above fp32's range."""
+    n, H = 20011, 64
+    K, V = _normal(1, 1, n, 128, seed=1), (1 + 0.1 * _normal(1, 1, n, 128, seed=2)) * 2.0 ** 118
+    one = _cache(K, V)
+    q = _normal(1, G, T, 128, seed=3, dtype=torch.bfloat16) * 0.1
+    ref, mag = _exact(q, one, [n])
+    c = _cache(K.expand(1, H, n, 128), V.expand(1, H, n, 128))
+    out = c.attend(q.repeat(1, H, 1, 1), n).view(H, G, T, 128)
+    for h in range(0, H, 9):
+        _close(out[h:h + 1], ref, mag)
