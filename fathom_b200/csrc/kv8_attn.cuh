@@ -10,6 +10,8 @@ namespace fathom {
 namespace kv8 {
 
 constexpr float QSCALE = (float)(1.4426950408889634 / 11.313708498984761);   // log2(e) / sqrt(128): base-2 scores
+// (A weight's exponent s + (log2 vs - m + HEAD) is exact to a rounding of s for scores up to 2^24, where whole numbers are
+// multiples of their spacing; beyond it a weight may be off by the spacing's power of two.)
 constexpr int PART = D + 4;      // floats of a partial result: 128 dims, reference, denominator, padding
 
 // Attention over a whole cache: T queries for each of Hkv * G heads of B sequences.  Strides in elements.

@@ -161,3 +161,27 @@ def test_split_rows_of_large_values_of_one_sign(G, T):
     out = c.attend(q.repeat(1, H, 1, 1), n).view(H, G, T, 128)
     for h in range(0, H, 9):
         _close(out[h:h + 1], ref, mag)
+
+
+@pytest.mark.parametrize("amp", [2.0 ** 14, 2.0 ** 17])
+@pytest.mark.parametrize("G,T", [(4, 1), (16, 1), (4, 5), (4, 40), (1, 300)])
+def test_scores_of_millions(G, T, amp):
+    """Scores up to 2^21 (fp32 holds them to 2^-3): where one key leads by far the output is its value, whatever the scores'
+    size.  Rows whose two largest scores are within 64, which 32-bit scores may not tell apart, are left out."""
+    n, H = 1500, 2
+    K, V = _normal(1, H, n, 128, seed=T), _normal(1, H, n, 128, seed=T + 1)
+    c = _cache(K, V)
+    q = _normal(1, H * G, T, 128, seed=G, dtype=torch.bfloat16) * amp
+    ref, mag = _exact(q, c, [n])
+    Kd, Vd = (torch.from_numpy(x).cuda() for x in O.values(c.rows.cpu().numpy(), c.scales.cpu().numpy()))
+    s = (q.double().view(H, G * T, 128) @ Kd[:, :n].transpose(1, 2)) / 128 ** 0.5
+    sees = n - (T - 1 - torch.arange(T, device="cuda")).repeat(G)
+    top = s.masked_fill(torch.arange(n, device="cuda") >= sees[:, None], -np.inf).topk(2, -1).values
+    lead = (top[..., 0] - top[..., 1] > 64).view(1, H * G, T)
+    assert lead.float().mean() > 0.9
+    _close(c.attend(q, n)[lead], ref[lead], mag[lead])
+    if T == 1:
+        idx = torch.arange(n, device="cuda").expand(H, G, n).contiguous()
+        for dtype in (torch.float32, torch.bfloat16):
+            out = c.attend_picks(q.view(H, G, 128).to(dtype), idx).view_as(ref)
+            _close(out[lead], ref[lead], mag[lead], 2.0 ** -17)
