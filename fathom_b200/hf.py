@@ -35,7 +35,7 @@ import torch
 import torch.nn.functional as F
 
 from . import bitplane as bp, klt as klt_mod
-from .kv8 import KVCache8
+from .kv8 import BLK, KVCache8
 from .offload import HostPlaneStore, MappedBuffer, decode_attention
 
 SKIP = 16        # tokens left out of the key statistics (4 * SINK, scripts/sketch.py:44-46)
@@ -43,12 +43,12 @@ SKIP = 16        # tokens left out of the key statistics (4 * SINK, scripts/sket
 
 class _Layer:
     __slots__ = ("Kdev", "Vdev", "len", "n", "rows", "K_src", "V_src", "store", "var", "Krec", "Vrec", "nrec",
-                 "owned", "kv8")
+                 "owned", "kv8", "at")
 
     def __init__(self):
         self.Kdev = self.Vdev = self.rows = self.K_src = self.V_src = self.store = self.var = None
         self.Krec = self.Vrec = self.kv8 = None
-        self.len = self.n = self.nrec = 0
+        self.len = self.n = self.nrec = self.at = 0
         self.owned = []
 
 
@@ -181,7 +181,7 @@ class OffloadedDecoder:
         reference's --synthetic-kv mode, :280-283); offload=True builds the layer's stores at once, so
         only one layer's prefill K/V is ever on the device.  rows_of=L0 (< L, already offloaded): the
         layer's index is built from K, but attention reads layer L0's row buffers (V unused) -- for
-        timing runs whose host memory cannot hold every layer's rows."""
+        timing runs whose host memory cannot hold every layer's rows.  Generated tokens stay each layer's own."""
         if L == 0:
             self._reset(K.shape[0])
         c = self.cache[L]
@@ -252,6 +252,7 @@ class OffloadedDecoder:
             src = self.cache[rows_of]
             if not (0 <= rows_of < L) or src.kv8 is None or src.n != n:
                 raise ValueError(f"OffloadedDecoder: rows_of={rows_of} must name an offloaded earlier layer")
+            c.at = self._own_tokens(src, len(self.cache) - L)
             c.kv8, K = src.kv8, c.Kdev.to(torch.bfloat16)
         elif not dense:
             K = c.kv8.read(0, n)[0]
@@ -271,7 +272,26 @@ class OffloadedDecoder:
             c.kv8.scales.copy_(dev8.scales)
             c.owned.append(c.kv8)
         c.n, c.nrec = n, 0
+        if rows_of is None:
+            c.at = n
         c.Kdev = c.Vdev = None
+
+    def _own_tokens(self, src, layers):
+        """Where the generated tokens of one more layer that reads src's 8-bit rows go: past those of src and of the
+        layers before, from a whole block on.  Rows without the room are replaced by a copy with room for `layers`."""
+        old, room = src.kv8, -(-self.max_new // BLK) * BLK
+        sharing = [c for c in self.cache if c.kv8 is old]
+        at = -(-(src.n + self.max_new) // BLK) * BLK + (len(sharing) - 1) * room
+        if at + room > old.cap:
+            new = KVCache8(self.B, self.Hkv, at + layers * room, old.device, host=old.host)
+            new.rows[:, :old.cap].copy_(old.rows)
+            new.scales[:, :old.nblk].copy_(old.scales)
+            for c in sharing:
+                c.kv8 = new
+                c.owned = [new if o is old else o for o in c.owned]
+            torch.cuda.synchronize(old.device)
+            old.free()
+        return at
 
     def _finish_offload(self):
         BH, n = self.B * self.Hkv, self.cache[0].n
@@ -370,7 +390,7 @@ class OffloadedDecoder:
         n = c.n
         if c.kv8 is not None:                    # the new token goes where the sequence ends
             pos = self._pos_s.view(-1) if self._graph_mode else n + c.nrec
-            c.kv8.write(k, v, pos)
+            c.kv8.write(k, v, pos if c.at == n else pos + (c.at - n))
             if not self._graph_mode:
                 c.nrec += 1
             m = n + c.nrec + (1 if self._graph_mode else 0)
@@ -403,6 +423,9 @@ class OffloadedDecoder:
         # the local window [m - local, m): one add into the strided tail of the index rows
         torch.add(self._arange_local.expand(BH, G, local), self._wbase_s if self._graph_mode else m - local,
                   out=idx[..., kk + sink:])
+        if c.at > n:                             # this layer's own tokens lie past those of the layer whose rows it reads
+            window = idx[..., kk + sink:]
+            window += (window >= n) * (c.at - n)
         if c.kv8 is not None:
             return c.kv8.attend_picks(q.reshape(BH, G, D), idx).view(B, Hq, 1, D)
         out = decode_attention(qf, idx, c.K_src, c.V_src, n, n, c.Krec, c.Vrec, self.max_new,
