@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           tc::Tmem<32>::ld(tm_s + 32 * u, x);
-          tc::wait_ld32(x);
+          tc::wait_ld<32>(x);
           if (masked) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
             for (int i = 0; i < 64; i += 16) {
               uint32_t o[16];
               tc::Tmem<16>::ld(tm_o + i, o);
-              tc::wait_ld();
+              tc::wait_ld<16>(o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tc::Tmem<16>::st(tm_o + i, o);
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
           const int u = v ^ 1;                     // the second 32 are still in registers
           if (v == 1) {
             tc::Tmem<32>::ld(tm_s + 32 * u, x);
-            tc::wait_ld32(x);
+            tc::wait_ld<32>(x);
             if (masked) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
         uint32_t o[16];
         __syncwarp();
         tc::Tmem<16>::ld(tm_o + i, o);
-        tc::wait_ld();
+        tc::wait_ld<16>(o);
         if (!real) continue;
         if (whole) {
 #pragma unroll

@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
           uint32_t c[QT][NC];
 #pragma unroll
           for (int term = 0; term < QT; ++term) tc::Tmem<NC>::ld(tm_s + k * S::NQ + term * RT, c[term]);
-          tc::wait_ld();
+          tc::wait_ld<QT * NC>(c[0]);
           tc::fence_before();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(s_free(k));
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             for (int term = 0; term < TERMS; ++term) {
               uint32_t o[NC];
               tc::Tmem<NC>::ld(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
-              tc::wait_ld();
+              tc::wait_ld<NC>(o);
 #pragma unroll
               for (int r = 0; r < NR; ++r) o[r] = __float_as_uint(__uint_as_float(o[r]) * f[r]);
               tc::Tmem<NC>::st(tm_o + (SPLIT ? 0 : g * S::NP) + term * RT, o);
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
 #pragma unroll
           for (int term = 0; term < TERMS; ++term) tc::Tmem<4>::ld(tm_o + k * S::NP + term * RT + r0, c[k][term]);
         }
-        tc::wait_ld();
+        tc::wait_ld<NO * TERMS * 4>(c[0][0]);
 #pragma unroll
         for (int rr = 0; rr < 4; ++rr) {
           const int r = first + r0 + rr;
