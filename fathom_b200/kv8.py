@@ -41,7 +41,7 @@ class KVCache8:
     into pinned mapped host memory (the scales stay on the device; free() or garbage collection releases
     the rows): written and read over the host link, attended to over picks only.  Tokens past the last written
     one are void: no call reads them.  Which tokens a sequence has is the caller's to know: a write says where it
-    begins, a read or an attention where it ends."""
+    begins, a read or an attention where it ends.  Calls run on the rows' device, whichever is the current one."""
 
     def __init__(self, B, Hkv, cap, device="cuda", rows=None, scales=None, host=False):
         if B < 1 or Hkv < 1 or cap < 1:
@@ -104,6 +104,9 @@ class KVCache8:
         alone and tokens past cap are dropped).  The scale of a block covers every token written to it in
         this and in earlier calls; a block written from its first token on starts afresh.  NaN and infinities
         are stored as NaN and do not enter the scale."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.write(K, V, start)
         self._check_on("KVCache8.write", K, V)
         shape = K.shape
         if len(shape) != 4 or shape[0] != self.B or shape[1] != self.Hkv or shape[3] != D or V.shape != shape:
@@ -128,6 +131,9 @@ class KVCache8:
     def read(self, start=0, n=None, dtype=torch.bfloat16):
         """Tokens [start, start + n) (to the end of the cache by default) as (K, V) [B, Hkv, n, 128] in dtype: fp32
         and bf16 hold the cached values exactly, fp16 rounds."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.read(start, n, dtype)
         n = self.cap - start if n is None else n
         if not 0 <= start <= self.cap or not 0 <= n <= self.cap - start:
             raise ValueError(f"KVCache8.read: tokens [{start}, {start + n}) are outside the cache's {self.cap}")
@@ -147,6 +153,9 @@ class KVCache8:
         [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
         that sees no key gives 0; a NaN in a key or value reaches the queries that see it and no others.  Returns
         [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.attend(q, end)
         self._check_on("KVCache8.attend", q)
         if self.host:
             raise ValueError("KVCache8.attend: the rows are in host memory (attend_picks reads those)")
@@ -178,6 +187,9 @@ class KVCache8:
         for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  fp32
         arithmetic; returns [BH, G, 128] in q's dtype.  Of rows in host memory each distinct one of a KV head is
         fetched once."""
+        if torch._C._cuda_getDevice() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.attend_picks(q, idx, end)
         self._check_on("KVCache8.attend_picks", q, idx)
         qs, ks = q.shape, idx.shape
         if len(qs) != 3 or qs[0] != self.BH or qs[1] < 1 or qs[2] != D:
