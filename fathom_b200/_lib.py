@@ -117,6 +117,11 @@ def ptr(x):
 
 
 def stream_of(device):
+    """The raw current stream of the tensors' device, for a launch.  The library launches on the current device, so with
+    another one current the kernel would run there, on addresses of this one: refused."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        raise ValueError(f"fathom_b200: the tensors are on {device} but the current device is cuda:"
+                         f"{torch.cuda.current_device()}; call torch.cuda.set_device or use `with torch.cuda.device(...)`")
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -39,3 +39,13 @@ def test_calls_run_on_the_device_of_the_rows(monkeypatch):
     assert {n for n, _ in seen} == {"fathom_kv8_write", "fathom_kv8_read", "fathom_kv8_attend",
                                     "fathom_kv8_attend_workspace_bytes", "fathom_kv8_attend_picks"}
     assert all(d == 0 for _, d in seen) and now == [1]
+
+
+def test_launches_elsewhere_are_refused(monkeypatch):
+    import pytest
+    from fathom_b200 import _lib
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: type("Stream", (), {"cuda_stream": 7}))
+    assert _lib.stream_of(torch.device("cuda", 0)) == _lib.stream_of(torch.device("cuda")) == 7
+    with pytest.raises(ValueError, match="current device"):
+        _lib.stream_of(torch.device("cuda", 1))
