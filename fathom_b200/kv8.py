@@ -12,6 +12,8 @@ step over the cache can be captured in a CUDA graph.
     out = cache.attend_picks(q, idx, end)   # the listed keys of each query head
     K, V = cache.read(0, n)
 """
+import operator
+
 import torch
 
 from . import _lib
@@ -24,7 +26,7 @@ BLK, D = 64, 128
 def _position(x, B, device, what):
     """(number, device tensor or None) of a position given as an int or as int64 [B] (or [1]) on `device`."""
     if not isinstance(x, torch.Tensor):
-        return int(x), None
+        return operator.index(x), None                 # (a float is a TypeError, not a position rounded down)
     if x.dtype == torch.int64 and x.dim() == 1 and x.shape[0] == B and x.device == device and x.is_contiguous():
         return 0, x
     if x.device != device or x.dtype != torch.int64 or x.numel() not in (1, B) or x.dim() > 1:
