@@ -4,9 +4,12 @@
 // rows is 2 x 2 products of 128 x 128 x 128, ~2048 cycles, and 32768 exponentials at 16 a cycle.  Rows are
 // the (token, head) pairs of one KV head, token-major, so G heads share every tile.  Per CTA:
 //
-//   S_i [128 rows x 128 tokens] = (q1 + q2 [+ q3]) K^T   e4m3 x e4m3: q as a sum of e4m3 terms (2 hold a bf16, 3 an
-//                                                        fp16), the key tile straight from TMA; 2 terms at twice
-//                                                        the rate cost one 16-bit product, and no key is converted
+//   S_i [128 rows x 128 tokens] = (q1 + q2 [+ q3]) K^T   8-bit products: q as a sum of an e4m3 term (4 bits) and e5m2
+//                                                        ones, whose 3 bits each hold what a rounding leaves of 8 and
+//                                                        of 11, and whose range goes on where e4m3's ends: a bf16
+//                                                        exactly or to 2^-21 of its row's largest, an fp16 to 2^-25.
+//                                                        The key tile comes straight from TMA; 2 terms at twice the
+//                                                        rate cost one 16-bit product, and no key is converted
 //   O_i [128 rows x 128 dims]  += P_i V                  f16 x f16: an e4m3 value is exact in f16; weights in
 //                                                        tensor memory over the scores they came from
 //
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       const bool real = row < total;
       const int rr = real ? row : total - 1, tt = rr / a.G, hq = (w.bh % a.Hkv) * a.G + rr - tt * a.G;
       const int limit = w.end - (int)a.T + 1 + tt;               // keys that the row sees
-      // the half's queries as e4m3 terms of their own scales: 16 lanes per row, a lane 8 dims; a warp takes rows
+      // the half's queries as 8-bit terms of their own scales: 16 lanes per row, a lane 8 dims; a warp takes rows
       // 2 (warp mod 8) and the next of every 16, 8 at a time.  What a term leaves of 11 bits is exact in f16.
       const int first = w.it * ROWS + h2 * HALF, rows = min(HALF, total - first), piece = lane & 15;
       const T* const qb = reinterpret_cast<const T*>(a.q) + w.b * a.qb + (int64_t)(w.bh % a.Hkv) * a.G * a.qh + 8 * piece;
@@ -184,8 +187,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
             uint32_t code[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              code[k] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y[k]), __NV_SATFINITE, __NV_E4M3);
-              const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code[k], __NV_E4M3);
+              const __nv_fp8_interpretation_t type = term == 0 ? __NV_E4M3 : __NV_E5M2;
+              code[k] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y[k]), __NV_SATFINITE, type);
+              const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)code[k], type);
               y[k] = __hsub2(y[k], *reinterpret_cast<const __half2*>(&d));
             }
             *reinterpret_cast<uint2*>(at + term * HALF * D) = make_uint2(code[0] | code[1] << 16, code[2] | code[3] << 16);
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
       }
     } else if (warp == 20) {
       // ---- products (the whole warp: elect_one)
-      constexpr uint32_t id_s = tc::instr(TILE, false, false), id_o = tc::instr(D, false, true);
+      constexpr uint32_t id_s = tc::instr(TILE, false, false), id_t = tc::instr(TILE, false, false, true), id_o = tc::instr(D, false, true);
       const uint32_t tmu = tc::uniform(tm);
       uint32_t i = 0;                              // tiles done
       uint32_t pn[2] = {0, 0}, seg[2] = {0, 0};    // by half: weight tiles done, pieces begun
@@ -452,8 +456,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const __grid_constan
           for (int term = 0; term < QT; ++term) {
 #pragma unroll
             for (int kk = 0; kk < D / 32; ++kk)
-              tc::mma_fp8(tmu + h * 128, tc::operand(sbase + S::Q + (h * QT + term) * HALF * D) + kk * 2, dk + kk * 2, id_s,
-                          term > 0 || kk > 0);
+              tc::mma_fp8(tmu + h * 128, tc::operand(sbase + S::Q + (h * QT + term) * HALF * D) + kk * 2, dk + kk * 2,
+                          term > 0 ? id_t : id_s, term > 0 || kk > 0);
           }
           if (spent) tc::mma_commit(bar + 8 * (KSTAGES + ks));
           tc::mma_commit(s_full(h));

@@ -121,9 +121,9 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead = 16) {
          1ull << 46 | 2ull << 61;
 }
 // fp32 accumulators, M = 128; a_mn / b_mn: the operand is MN-major.  Types: kind::f16 f16 x f16, kind::f8f6f4
-// e4m3 x e4m3 (both coded 0).
-constexpr uint32_t instr(uint32_t N, bool a_mn, bool b_mn) {
-  return 1u << 4 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (N >> 3) << 17 | (128u >> 4) << 24;
+// e4m3 x e4m3 (both coded 0) or, a_e5m2, e5m2 x e4m3.
+constexpr uint32_t instr(uint32_t N, bool a_mn, bool b_mn, bool a_e5m2 = false) {
+  return 1u << 4 | (a_e5m2 ? 1u << 7 : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (N >> 3) << 17 | (128u >> 4) << 24;
 }
 __device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }\n" ::"r"(d),

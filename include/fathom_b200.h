@@ -338,7 +338,7 @@ size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t 
 /* out = softmax(q K^T / sqrt(128)) V over the cache, for q, out [B][Hkv*G][T][128] (bf16 or fp16; strides in
  * elements, last dimension contiguous): the T queries of a sequence are its last T tokens, query t sees
  * the keys [0, end - (T - 1 - t)).  A query that sees no key gives 0.  end above cap is read as cap.  Scores and
- * sums in fp32; queries enter the products to 2^-18 of a row's largest element (bf16) or to 12 bits (fp16); weights, with
+ * sums in fp32; queries enter the products exactly or to 2^-21 (bf16) or 2^-25 (fp16) of a row's largest element; weights, with
  * their value scales, to 11 bits down to 2^-15 of a row's largest and in steps of 2^-26 of it below.  A NaN or infinity of
  * a query, a key or a value makes the queries that see it NaN (of a value: in its dim at least) and no others. */
 int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,

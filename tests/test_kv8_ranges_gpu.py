@@ -185,3 +185,22 @@ def test_scores_of_millions(G, T, amp):
         for dtype in (torch.float32, torch.bfloat16):
             out = c.attend_picks(q.view(H, G, 128).to(dtype), idx).view_as(ref)
             _close(out[lead], ref[lead], mag[lead], 2.0 ** -17)
+
+
+@pytest.mark.parametrize("dtype,bits", [("bf16", 21), ("f16", 25)])
+@pytest.mark.parametrize("G,T", [(4, 1), (16, 1), (4, 5), (1, 40), (4, 80)])
+def test_queries_of_wide_ranges(G, T, dtype, bits):
+    """Elements of q from 2^-16 of the row's largest on, which alone decide the scores: they enter to 2^-bits of the largest
+    at least, so a score is off by 2^-bits * max|q| * sum|k| / sqrt(128) at most, and an output by e^(2 * that) - 1 of
+    sum(weight * |V|)."""
+    n, H = 300, 2
+    K, V = torch.zeros(1, H, n, 128, device="cuda"), _normal(1, H, n, 128, seed=T)
+    K[..., 1:5] = _normal(1, H, n, 4, seed=T + 1) * 2.0 ** 17
+    c = _cache(K, V)
+    q = _normal(1, H * G, T, 128, seed=G) * 2.0 ** -14
+    q[..., 0] = 1.0
+    q = q.to(DT[dtype])
+    ref, mag = _exact(q, c, [n])
+    Kc = torch.from_numpy(O.values(c.rows.cpu().numpy(), c.scales.cpu().numpy())[0]).cuda()[:, :n]
+    off = 2.0 ** -bits * float(q.abs().max()) * float(Kc.abs().sum(-1).max()) / 128 ** 0.5
+    _close(c.attend(q, n), ref, mag, 2.0 ** -10 + np.expm1(2 * off))
