@@ -19,7 +19,6 @@ namespace fathom {
 constexpr int KV8_ROW = 2 * D;          // bytes of one token's key and value codes
 constexpr int64_t KV8_MAX_CAP = 1 << 30;      // tokens: positions and tile ends fit 32 bits
 constexpr int KV8_EMIN = -120, KV8_EMAX = 120;   // 2^e and 2^-e are normal fp32 numbers
-constexpr uint32_t KV8_NAN = 0x7Fu;     // the code of every non-finite input
 
 // Smallest e in [KV8_EMIN, KV8_EMAX] with amax <= 448 * 2^e, from the bits of amax (finite, >= 0): 448 is
 // 1.75 * 2^8, so the exponent of amax less 8, one more when its mantissa is above 1.75.

@@ -47,7 +47,6 @@ __device__ __forceinline__ int seq_end(const Args& a, int b) {
   return e > 0 ? (int)e : 0;
 }
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ void from_f32(float x, float* p) { *p = x; }

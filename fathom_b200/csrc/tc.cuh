@@ -130,11 +130,6 @@ __device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint
                "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
                : "memory");
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }\n" ::"r"(d),
-               "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-               : "memory");
-}
 // A from tensor memory.
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }\n" ::"r"(d),
