@@ -186,7 +186,7 @@ class OffloadedDecoder:
             self._reset(K.shape[0])
         c = self.cache[L]
         c.Kdev, c.Vdev, c.len = K, V, K.shape[2]
-        if self.kv == "e4m3" and rows_of is None:
+        if self.kv == "e4m3" and (rows_of is None or not offload):     # (rows are shared by what offload builds)
             c.kv8 = KVCache8(self.B, self.Hkv, c.len + self.max_new, K.device)
             c.kv8.write(K, V)
             c.Kdev = c.Vdev = None

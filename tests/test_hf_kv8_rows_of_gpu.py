@@ -86,3 +86,20 @@ def test_graph_decode_over_shared_rows_matches_eager():
             dec.free()
             dec.unpatch()
     assert torch.equal(logits[0], logits[1])
+
+
+def test_rows_of_without_offload_keeps_the_layers_own_rows():
+    """As over bf16 rows: rows_of takes effect with offload=True only; offload() afterwards builds every layer's own."""
+    from fathom_b200.hf import OffloadedDecoder
+    outs = []
+    for rows_of in (None, 0):
+        dec = OffloadedDecoder(_model(), k=300, sink=4, local=32, index="hbm", rows="hbm", max_new=4, kv="e4m3")
+        try:
+            for L in range(2):
+                dec.load_kv(L, _randn(1, 2, 700, 128, seed=L), _randn(1, 2, 700, 128, seed=10 + L), rows_of=rows_of if L else None)
+            dec.offload()
+            outs.append(dec.decode(torch.zeros(1, 1, dtype=torch.long, device="cuda")))
+        finally:
+            dec.free()
+            dec.unpatch()
+    assert torch.equal(outs[0], outs[1])
