@@ -204,3 +204,16 @@ def test_queries_of_wide_ranges(G, T, dtype, bits):
     Kc = torch.from_numpy(O.values(c.rows.cpu().numpy(), c.scales.cpu().numpy())[0]).cuda()[:, :n]
     off = 2.0 ** -bits * float(q.abs().max()) * float(Kc.abs().sum(-1).max()) / 128 ** 0.5
     _close(c.attend(q, n), ref, mag, 2.0 ** -10 + np.expm1(2 * off))
+
+
+@pytest.mark.parametrize("G,T", [(4, 1), (8, 1), (4, 5), (4, 40), (4, 80)])
+def test_more_sequences_than_a_warp_has_lanes(G, T):
+    """40 sequences at their own device lengths, some empty, some a few tiles long, some in many CTAs."""
+    B, H, n = 40, 2, 6000
+    K, V = _normal(1, H, n, 128, seed=T), _normal(1, H, n, 128, seed=T + 1)
+    c = _cache(K.expand(B, H, n, 128), V.expand(B, H, n, 128))
+    q = _normal(B, H * G, T, 128, seed=G, dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(T)
+    ends = [0, 1, n, 128, 129] + torch.randint(0, n + 1, (B - 5,), generator=g).tolist()
+    ref, mag = _exact(q, c, ends)
+    _close(c.attend(q, torch.tensor(ends, device="cuda")), ref, mag)
