@@ -71,7 +71,8 @@ struct WriteArgs {
 //
 // Bound by HBM: a bf16 element is 2 bytes read, 1 written.  The conversion is kept to ~3 instructions an element
 // (packed maximum, no test for infinities unless the block has one): at ~8 its issue showed, 200 us for 128k tokens of
-// 8 KV heads in bf16.  Measured: 120 us, 6.7 TB/s, the copy rate.  One token: 2.2 us, launch and latency.
+// 8 KV heads in bf16.  Measured: 117-128 us, 6.3-6.9 TB/s, the copy rate (token-major input 138).  One token:
+// 1.7-1.9 us in a graph, launch and latency.
 template <typename T>
 __global__ void __launch_bounds__(WT) kv8_write_kernel(WriteArgs a) {
   __shared__ uint32_t s_max[WT / 32];

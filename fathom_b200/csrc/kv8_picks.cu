@@ -15,11 +15,12 @@
 // for the output and of s for the denominator.  The warps of a (batch, query head) lie in one CTA or a cluster; their
 // states are joined in warp order in the first CTA's shared memory.
 //
-// Measured over 128k: 2116 picks for each of 224 heads 26 us, 4.7 TB/s of rows (34 with 16-bit matrix instructions on
-// rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24.
-// ~5 us of it begin and join; the rest is 32 picks per 340 cycles and SM, 6 TB/s.  12 warps per SM, or 3 stages, are
+// Measured over 128k: 2116 picks for each of 224 heads 24.4-25.7 us, 4.7 TB/s of rows (34 with 16-bit matrix instructions on
+// rows turned to f16, 58 on the fp32 pipes; 32.5 while a step waited for its entry of the list); with the rows in L2 24,
+// so the bound is a warp's chain of steps at 8 warps per SM (issue 47% busy), not HBM.  ~5 us of it begin and join; the rest is
+// 32 picks per 340 cycles and SM, 6 TB/s.  12 warps per SM, or 3 stages, are
 // slower (29 us), so are TMA gathers of 4 rows (28; for the keys alone 28.5), bulk copies of one (34) and rows loaded into
-// registers (29).  580 picks for 32 heads: 5.1 us in a graph.
+// registers (29).  580 picks for 32 heads: 4.9-5.1 us in a graph.
 #include "dedupe.cuh"
 #include "kv8_attn.cuh"
 

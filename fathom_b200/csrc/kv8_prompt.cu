@@ -18,14 +18,14 @@
 // constant of each 64-token block, enters the weight's exponent, so a row sees its own range whatever other blocks
 // hold.  Softmax, two threads per row, one for each block of a tile: m, the reference of s + ev, follows the row's
 // maximum only when that exceeds it by 2^12 (then O is rescaled; at 2^7 that cost 3%); weights are 2^(s + ev - m + 3), at
-// most 2^15 in f16, rounded to 11 bits down to 2^-17 of the reference and to steps of 2^-27 of it below; sums in fp32.  The
+// most 2^15 in f16 (the product's other operand is f16, and the outputs have 8 or 11 bits), rounded to 11 bits down to 2^-17 of the reference and to steps of 2^-27 of it below; sums in fp32.  The
 // denominator has a reference of its own, without the value scales: each block's sum of weights enters it once.  Parts
 // and outputs are weighted means, whatever the values' range is.  (One thread per row, 8 softmax warps instead
 // of 16: 1.34 ms against 0.95 for the chunk below, the steps of a tile waiting for each other; exponentials partly by
 // polynomial: slower, the warps' issue is as near its limit as the special-function units.)
 //
-// Measured, 2048 queries at 32k, 8 KV heads, G = 4, bf16: 0.93 ms = 1.22 PFLOP/s, 0.74 of the measured 16-bit product
-// rate; back to back 1.08 ms under the power cap, 0.74 of the sustained rate.
+// Measured, 2048 queries at 32k, 8 KV heads, G = 4, bf16: single calls 1.04-1.07 ms = 1.06-1.09 PFLOP/s, 0.65 of the
+// measured 16-bit product rate; back to back 1.04-1.13 ms under the power cap, 0.71-0.77 of the sustained rate.
 //
 // Work: the tiles of all (bh, 256 rows) items in a line, cut into equal contiguous shares, one per CTA; an item cut
 // by a share's end leaves parts in the workspace, which a second kernel joins in a fixed order.

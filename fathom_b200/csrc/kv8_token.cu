@@ -26,8 +26,8 @@
 //
 // A row's parts in different CTAs (kv8_line.cuh) are joined by a second kernel in a fixed order.
 //
-// Measured (8 KV heads, G = 4, bf16): one token over 128k 43.6 us, 6.2 TB/s or 0.94 of the copy rate; 8 sequences of 80k,
-// 4 KV heads, G = 7: 99 us, 6.8 TB/s; over 700 tokens 6.3 us, a chain of latencies.  With one softmax warpgroup the
+// Measured in graphs (8 KV heads, G = 4, bf16): one token over 128k 45-46 us with the join, 5.9 TB/s or 0.9 of the copy
+// rate; 8 sequences of 80k (mean), 4 KV heads, G = 7: 107 us, 0.96; over 700 tokens 6.2 us, a chain of latencies.  With one softmax warpgroup the
 // softmax was the bound: 58 us and 150 us.
 #include "kv8_line.cuh"
 
@@ -43,7 +43,10 @@ constexpr int STAGE_BYTES = 2 * TILE * D;        // key tile, value tile
 constexpr float SLACK = 5.0f;                    // a tile may exceed the reference by 2^5
 constexpr float HEAD = 3.0f;                     // weights at the reference are 8: 2^(HEAD + SLACK) = 256 <= 448
 constexpr int PIECE = 6;                         // tiles (~0.4 us each) that beginning and ending a piece takes: ~2.5 us
-constexpr int SHORT = 8;                         // tiles that take less than the second kernel (~4 us)
+// Tiles up to which a row is whole in one CTA and not joined.  In a graph, whole against joined: one token of 32 KV heads,
+// G = 7, over 1024 tokens 7.9 against 8.7 us; of 8 KV heads, G = 4, over 512 5.1 / 6.1, over 1024 6.7 / 6.1; drafts of 20
+// rows over 384 10.2 / 10.3, over 1024 15.5 / 10.3 (there 3 tiles would be the rule).
+constexpr int SHORT = 8;
 constexpr int MAX_CTAS = 512;                    // shares that the join kernel has room for
 
 constexpr int up16(int n) { return (n + 15) / 16 * 16; }
@@ -385,7 +388,8 @@ __global__ void __launch_bounds__(THREADS, 1) token_kernel(const __grid_constant
             tc::wait_st();
           }
         }
-        // weights as terms into the operand buffer, by way of f16: 11 bits, whose remainders after e4m3 are exact
+        // weights as terms into the operand buffer, by way of f16: 11 bits, whose remainders after e4m3 are exact.  (More would
+        // be lost in the outputs' 8 or 11: weights round independently.  fp16 drafts: 2.3e-4 off, in 32 bits 2.1e-4.)
         uint32_t codes[TERMS * NC / 4] = {};
 #pragma unroll
         for (int r = 0; r < NR; r += 2) {
@@ -603,7 +607,7 @@ int launch_rows(const CUtensorMap& map, const Args& a, int ctas, cudaStream_t st
   if (R <= 4) return launch<T, 4, QT, false>(map, a, ctas, st);
   if (R <= 8) return launch<T, 8, QT, false>(map, a, ctas, st);
   if (R <= 16) return launch<T, 16, QT, false>(map, a, ctas, st);
-  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);      // 20 rows over 16k: 19.2 us, with 16 per thread ~22
+  if (R <= 24) return launch<T, 12, QT, true>(map, a, ctas, st);      // 20 rows over 16k: with 16 per thread ~2.5 us more
   return launch<T, 16, QT, true>(map, a, ctas, st);
 }
 

@@ -153,7 +153,8 @@ class KVCache8:
         """softmax(q K^T / sqrt(128)) V of q [B, Hq, T, 128] (bf16 or fp16, any strides; Hq a multiple of Hkv):
         the T queries of a sequence are its last T tokens, already written, and query t sees the keys
         [0, end - (T - 1 - t)).  end: an int, or int64 [B] on the device (values above cap mean cap).  A query
-        that sees no key gives 0; a NaN in a key or value reaches the queries that see it and no others.  Returns
+        that sees no key gives 0; a NaN in a key or value reaches the queries that see it and no others.  Sums in fp32;
+        q enters exactly or to 2^-21 (bf16) or 2^-25 (fp16) of its row's largest element, weights to 11 bits.  Returns
         [B, Hq, T, 128] in q's dtype, laid out as [B, T, Hq, 128]."""
         if torch._C._cuda_getDevice() != self.device.index:
             with torch.cuda.device(self.device):
@@ -186,9 +187,10 @@ class KVCache8:
     def attend_picks(self, q, idx, end=None):
         """Attention over listed tokens, as decode_attention over bf16 rows: q [BH, G, 128] (fp32, bf16 or fp16),
         idx [BH, G, k] int64.  Picks outside [0, end) are ignored (end: an int, int64 [B] on the device, or None
-        for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  fp32
-        arithmetic; returns [BH, G, 128] in q's dtype.  Of rows in host memory each distinct one of a KV head is
-        fetched once."""
+        for the whole cache); a pick listed twice counts twice; a head with no pick left gives 0.  Sums in fp32; q
+        enters to 24 bits of its row's largest element, weights to 24 bits of the row's largest.  Returns [BH, G, 128]
+        in q's dtype.  Of rows in host memory each distinct one of a KV head is fetched once over the link where
+        G * k <= 16384; longer lists fetch a row for every pick."""
         if torch._C._cuda_getDevice() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.attend_picks(q, idx, end)

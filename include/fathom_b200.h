@@ -339,7 +339,7 @@ size_t fathom_kv8_attend_workspace_bytes(int64_t B, int64_t Hkv, int G, int64_t 
  * elements, last dimension contiguous): the T queries of a sequence are its last T tokens, query t sees
  * the keys [0, end - (T - 1 - t)).  A query that sees no key gives 0.  end above cap is read as cap.  Scores and
  * sums in fp32; queries enter the products exactly or to 2^-21 (bf16) or 2^-25 (fp16) of a row's largest element; weights, with
- * their value scales, to 11 bits down to 2^-15 of a row's largest and in steps of 2^-26 of it below.  A NaN or infinity of
+ * their value scales, to 11 bits down to 2^-17 of a row's largest and in steps of 2^-27 of it below.  A NaN or infinity of
  * a query, a key or a value makes the queries that see it NaN (of a value: in its dim at least) and no others. */
 int fathom_kv8_attend(const void* q, int dtype, int64_t B, int64_t Hkv, int G, int64_t T, int64_t q_stride_b,
                       int64_t q_stride_h, int64_t q_stride_t, const uint8_t* rows, const float* scales, int64_t cap,
